@@ -685,6 +685,65 @@ int smx_maxpool2_bwd_f32(const float* x, int ldx, const float* gy, int ldg, floa
 /* y[p][c] = x[p][c] * scale[c] + shift[c] (shift may be NULL): the (x - mean) / std input normalisation (vgg_arch.py:203) and its backward */
 int smx_chan_affine_f32(const float* x, int ldx, const float* scale, const float* shift, float* y, int ldy, int64_t P, int C, void* stream);
 
+/* =======================================================================================
+ * ATTENTION WITH A LEARNED RELATIVE POSITION BIAS BY BUCKETS (csrc/relpos_attn*.hip), forward on fp32 / bf16 storage and backward on
+ * fp32 storage.  Beside smx_attention_* for sequences without a fixed length: frames of a clip, streamed one token at a time.
+ *   position of query i of sample b: pos = q_start + i (has_q_start), else n_b - L + i: the queries are the last L of the sample's
+ *   n_b = kv_len[b] (clamped to 0..S) keys, n_b = S without kv_len;  delta = j - pos;
+ *   s_ij = scale * q_i . k_j + table[map[clamp(delta - map_lo, 0, map_n - 1)]][head];  P = softmax over the keys that are left (j < n_b,
+ *   not masked, delta <= 0 if causal);  o_i = sum_j P_ij v_j.  A query with no key left: o = 0 and no gradient.
+ * What the places of masked keys and of keys behind n_b hold is never used (NaN and infinities too); their dk / dv are written as 0.
+ * q [B][L] rows of H*dh, k / v [B][S] rows of Hkv*dh (head h reads kv head h / (H / Hkv)), row strides ld*, sample strides *_bs in
+ * elements (k / v sample stride 0: one context for all samples).  dh % 4 == 0, dh <= 128; strides % 4 == 0, pointers aligned to four
+ * elements.  table [num_buckets][H] fp32, map [map_n] int32 device array with values in 0..num_buckets-1, map_n <= 2049,
+ * map_lo <= 0 <= map_lo + map_n - 1; mask [B][S] bytes (1 = masked) or NULL; kv_len [B] int32 device or NULL.
+ * lse: [B][H][L] floats or NULL: log2 of the row's softmax sum (+inf for a row with no key), what the backward reads.
+ * ws: smx_attention_relpos_ws_bytes(d) bytes, 16-byte aligned (backward: smx_attention_relpos_bwd_ws_bytes).
+ * Backward (fp32): o and d_o dense [B][L][H*dh]; dq dense [B][L][H*dh], dk / dv dense [B][S][Hkv*dh] per sample, written; dtable
+ * [num_buckets][H] ACCUMULATED into.  Fixed summation orders, no atomics.
+ * ===================================================================================== */
+typedef struct smx_relpos_desc {
+  const void* q; const void* k; const void* v; void* o;
+  const float* table; const int32_t* map; const uint8_t* mask; const int32_t* kv_len;
+  float* lse; void* ws;
+  const float* d_o; float* dq; float* dk; float* dv; float* dtable;   /* backward only */
+  int64_t q_bs, k_bs, v_bs, o_bs, ws_bytes;
+  int32_t ldq, ldk, ldv, ldo;
+  int32_t B, H, Hkv, L, S, dh;
+  int32_t map_lo, map_n, num_buckets;
+  int32_t causal, has_q_start, q_start;
+  int32_t bf16;                                                      /* storage of q, k, v, o: 0 fp32, 1 bf16 */
+  float scale;
+} smx_relpos_desc;
+int64_t smx_attention_relpos_ws_bytes(const smx_relpos_desc* d);       /* -1: rejected arguments */
+int smx_attention_relpos(const smx_relpos_desc* d, void* stream);
+int64_t smx_attention_relpos_bwd_ws_bytes(const smx_relpos_desc* d);
+int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stream);
+
+/* =======================================================================================
+ * THE NORMS AROUND A BLOCK, ITS GATE AND RESIDUAL IN ONE PASS (csrc/norm_residual.hip), forward on fp32 / bf16 storage and backward on
+ * fp32 storage.  Beside smx_layernorm_pos_*: what stands between two blocks of a transformer layer.
+ *   n = Norm(h; post) (n = h without post_gamma);  x' = res_scale * x + gate[t / (T / groups)] * n (no gate: 1);  y = Norm(x'; pre)
+ *   rms = 0: (v - mean) / sqrt(var + eps) * gamma + beta;  rms = 1: v / sqrt(mean v^2 + eps) * gamma (+ beta);  beta may be NULL.
+ * x, h, xo, y dense [T][E]; y and pre_gamma both NULL: no second norm.  y is the norm of x' as it is stored (rounded to bf16 on bf16
+ * storage).  gamma / beta / gate fp32; gate [groups][E], T % groups == 0.  E <= 16384.
+ * Backward: gx / gy gradients of x' / y (either may be NULL), xo the forward's x'; dx, dh written (either may be NULL); dpost_* / dpre_*
+ * (may be NULL) ACCUMULATED into; dgate [groups][E] (may be NULL) written, or accumulated into with gate_accumulate.
+ * ws: smx_norm_residual_bwd_ws_floats floats, 16-byte aligned.  Fixed summation orders, no atomics.
+ * ===================================================================================== */
+typedef struct smx_norm_residual_desc {
+  const void* x; const void* h; void* xo; void* y;
+  const float* post_gamma; const float* post_beta; const float* pre_gamma; const float* pre_beta; const float* gate;
+  const float* gx; const float* gy; float* dx; float* dh; float* dgate;   /* backward only */
+  float* dpost_gamma; float* dpost_beta; float* dpre_gamma; float* dpre_beta; float* ws;
+  int64_t T, groups, ws_floats;
+  int32_t E, rms, bf16, gate_accumulate;
+  float res_scale, eps;
+} smx_norm_residual_desc;
+int smx_norm_residual(const smx_norm_residual_desc* d, void* stream);
+int64_t smx_norm_residual_bwd_ws_floats(int64_t T, int64_t groups, int E);
+int smx_norm_residual_bwd_f32(const smx_norm_residual_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

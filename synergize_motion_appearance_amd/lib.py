@@ -61,6 +61,24 @@ class Gemm16Desc(C.Structure):
     ]
 
 
+class RelposDesc(C.Structure):
+    """mirror of `smx_relpos_desc` (include/smx.h)."""
+    _fields_ = ([(n, _p) for n in ("q", "k", "v", "o", "table", "map", "mask", "kv_len", "lse", "ws", "d_o", "dq", "dk", "dv", "dtable")]
+                + [(n, _i64) for n in ("q_bs", "k_bs", "v_bs", "o_bs", "ws_bytes")]
+                + [(n, C.c_int32) for n in ("ldq", "ldk", "ldv", "ldo", "B", "H", "Hkv", "L", "S", "dh", "map_lo", "map_n", "num_buckets",
+                                            "causal", "has_q_start", "q_start", "bf16")]
+                + [("scale", _f)])
+
+
+class NormResidualDesc(C.Structure):
+    """mirror of `smx_norm_residual_desc` (include/smx.h)."""
+    _fields_ = ([(n, _p) for n in ("x", "h", "xo", "y", "post_gamma", "post_beta", "pre_gamma", "pre_beta", "gate", "gx", "gy", "dx", "dh", "dgate",
+                                   "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta", "ws")]
+                + [(n, _i64) for n in ("T", "groups", "ws_floats")]
+                + [(n, C.c_int32) for n in ("E", "rms", "bf16", "gate_accumulate")]
+                + [("res_scale", _f), ("eps", _f)])
+
+
 # name -> (restype, argtypes); every symbol include/smx.h declares
 SIGNATURES = {
     "smx_version": (C.c_char_p, []),
@@ -168,6 +186,13 @@ SIGNATURES = {
     "smx_antialias_nhwc_bwd_f32": (_i, [_p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
     "smx_maxpool2_f32": (_i, [_p, _i, _p, _i, _i, _i, _i, _i, _p]),
     "smx_maxpool2_bwd_f32": (_i, [_p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _p]),
+    "smx_attention_relpos_ws_bytes": (_i64, [C.POINTER(RelposDesc)]),
+    "smx_attention_relpos": (_i, [C.POINTER(RelposDesc), _p]),
+    "smx_attention_relpos_bwd_ws_bytes": (_i64, [C.POINTER(RelposDesc)]),
+    "smx_attention_relpos_bwd_f32": (_i, [C.POINTER(RelposDesc), _p]),
+    "smx_norm_residual": (_i, [C.POINTER(NormResidualDesc), _p]),
+    "smx_norm_residual_bwd_ws_floats": (_i64, [_i64, _i64, _i]),
+    "smx_norm_residual_bwd_f32": (_i, [C.POINTER(NormResidualDesc), _p]),
     "smx_chan_affine_f32": (_i, [_p, _i, _p, _p, _p, _i, _i64, _i, _p]),
     "smx_gemm_rp_f16_pack_bytes": (_i64, [_i, _i]),
     "smx_gemm_rp_f16_pack": (_i, [_p, _i, _p, _i, _i, _p]),

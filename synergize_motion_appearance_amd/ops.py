@@ -5,6 +5,7 @@ fp32 tensors `[B,H,W,C]`; a channel slice `buf[..., a:b]` is a legal operand (it
 stride is the channel count of `buf`), which is how concatenations are built in place.
 Every launcher raises on CPU tensors: there is no fallback path."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -840,6 +841,72 @@ def layernorm(x, gamma, beta, pos=None, eps=1e-5):
     return y, yp
 
 
+def _call(t, fn, *args):
+    """fn(*args, stream) on the device that holds t and that device's current stream."""
+    if t.device.index == torch.cuda.current_device():
+        return fn(*args, _stream())
+    with torch.cuda.device(t.device):
+        return fn(*args, _stream())
+
+
+def _vec(t, what, shape, like, dtype=torch.float32):
+    """address of a dense tensor of this shape and type on like's device."""
+    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device or not t.is_contiguous():
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if torch.is_tensor(t) else type(t).__name__
+        raise L.SmxError(f"{what}: a contiguous {dtype} tensor {shape} on {like.device} expected, got {got}")
+    return t.data_ptr()
+
+
+def _norm_weights(w, what, kind, E, like):
+    """(gamma, beta) addresses of a norm given as (gamma, beta) or (gamma,), or None."""
+    if w is None:
+        return None, None
+    if not isinstance(w, (tuple, list)) or len(w) not in (1, 2):
+        raise L.SmxError(f"{what}: (gamma, beta) or (gamma,) expected")
+    beta = w[1] if len(w) == 2 else None
+    return _vec(w[0], f"{what} gamma", (E,), like), None if beta is None else _vec(beta, f"{what} beta", (E,), like)
+
+
+def _norm_residual_desc(x, h, post, gate, res_scale, pre, kind, eps):
+    """the fields of smx_norm_residual_desc that forward and backward share."""
+    _dev(x, "norm_residual x", _ANY)
+    _dev(h, "norm_residual h", _ANY)
+    if kind not in ("layer", "rms"):
+        raise L.SmxError(f"norm_residual: kind 'layer' or 'rms' expected, got {kind!r}")
+    if x.shape != h.shape or x.dtype != h.dtype or x.device != h.device or x.dim() < 2 or not x.is_contiguous() or not h.is_contiguous():
+        raise L.SmxError(f"norm_residual: x and h must be contiguous tokens of one shape, type and device "
+                         f"({tuple(x.shape)} {x.dtype} {x.device}, {tuple(h.shape)} {h.dtype} {h.device})")
+    E = x.shape[-1]
+    if not 1 <= E <= 16384:
+        raise L.SmxError(f"norm_residual: 1 to 16384 channels expected, got {E}")
+    T = x.numel() // E
+    d = L.NormResidualDesc(h=h.data_ptr(), T=T, groups=1, E=E, rms=int(kind == "rms"), bf16=int(x.dtype == BF16), res_scale=res_scale, eps=eps)
+    d.post_gamma, d.post_beta = _norm_weights(post, "norm_residual post", kind, E, x)
+    d.pre_gamma, d.pre_beta = _norm_weights(pre, "norm_residual pre", kind, E, x)
+    if gate is not None:
+        d.groups = gate.numel() // E if torch.is_tensor(gate) else 0
+        if d.groups < 1 or T % d.groups:
+            raise L.SmxError(f"norm_residual: the gate's rows must divide the {T} tokens")
+        d.gate = _vec(gate, "norm_residual gate", (E,) if gate.dim() == 1 else (d.groups, E), x)
+    return d
+
+
+def norm_residual(x, h, *, post=None, gate=None, res_scale=1.0, pre=None, kind="layer", eps=1e-5):
+    """What stands between two blocks of a transformer layer, in one pass over the tokens: x' = res_scale * x + gate * Norm(h; post) and
+    y = Norm(x'; pre), the next block's input.  x (residual stream) and h (the block's output): contiguous tokens [..., E] of one storage
+    type (fp32 or bf16), E <= 16384.  post / pre: (gamma, beta) or (gamma,), fp32 [E]; post None: h as it is; pre None: no y.
+    gate: fp32 [E], or [G, E] with G dividing the tokens (row g gates the g-th run of T / G tokens: a sample, a frame, a token); None: 1.
+    kind: "layer" (mean and variance) or "rms" (root mean square).  -> (x', y or None); y is the norm of x' as it is stored."""
+    d = _norm_residual_desc(x, h, post, gate, res_scale, pre, kind, eps)
+    xo = torch.empty_like(x)
+    y = torch.empty_like(x) if pre is not None else None
+    if x.numel():
+        d.x, d.xo, d.y = x.data_ptr(), xo.data_ptr(), None if y is None else y.data_ptr()
+        L.check(_timed("norm_residual", {"bytes": x.element_size() * (3.0 + (y is not None)) * x.numel()}, _call, x, L.load().smx_norm_residual, C.byref(d)),
+                "norm_residual")
+    return xo, y
+
+
 def softmax_rows(s, S, scale=1.0, mask=None, rows_per_mask=0):
     """in-place softmax over the last dim (S) of contiguous s."""
     _dev(s, "softmax", _ANY)
@@ -1180,4 +1247,124 @@ def attention(q, k, v, nhead, dh, S, *, k_shared=False, mask=None, k_off=0, scal
     L.check(_timed(f"attention_d{dh}", meta, _fn("smx_attention", q), qp, ldq, Lq * ldq, kp + es * k_off, ldk, kbs, vp, ldv, vbs,
                    o.data_ptr(), E, Lq * E, None if mask is None else mask.data_ptr(), B, nhead, Lq, S, dh,
                    dh ** -0.5 if scale is None else scale, _stream()), "attention")
+    return o
+
+
+class RelPos:
+    """Buckets of relative positions delta = key position - query position, for `attention_relpos`: the first half of a side's buckets holds
+    one distance each, the second half ranges that grow by a constant factor up to `max_distance`; everything beyond shares the last.
+    two_sided: half of the buckets for delta <= 0, half for delta > 0; else delta > 0 shares bucket 0 with delta = 0 (causal use).
+    The borders are found in whole numbers: no logarithm decides on which side of one a distance falls."""
+    __slots__ = ("num_buckets", "max_distance", "two_sided", "lo", "map", "_on")
+
+    def __init__(self, num_buckets, max_distance, two_sided=True):
+        nb = num_buckets // 2 if two_sided else num_buckets
+        half = nb // 2
+        if num_buckets % (2 if two_sided else 1) or not 1 <= half < max_distance <= 1024 or num_buckets > 4096:
+            raise L.SmxError(f"RelPos: {num_buckets} buckets to distance {max_distance}: at least two per side, and a distance of at most 1024 that "
+                             "is larger than a quarter (one-sided: half) of the buckets")
+        self.num_buckets, self.max_distance, self.two_sided = num_buckets, max_distance, bool(two_sided)
+        side = list(range(half))
+        for n in range(half, max_distance + 1):               # bucket half + t from the smallest n with (n / half)^(nb - half) >= (max / half)^t
+            t = side[-1] + 1 - half if n > half else 0
+            t = max(0, min(t, nb - half - 1))
+            while t > 0 and n ** (nb - half) * half ** t < max_distance ** t * half ** (nb - half):
+                t -= 1
+            while t < nb - half - 1 and n ** (nb - half) * half ** (t + 1) >= max_distance ** (t + 1) * half ** (nb - half):
+                t += 1
+            side.append(half + t)
+            if half + t == nb - 1:
+                break
+        self.lo = 1 - len(side)                               # map[delta - lo], its ends stand for every distance beyond them
+        self.map = tuple(side[::-1] + ([nb + b for b in side[1:]] if two_sided else []))
+        self._on = {}
+
+    def bucket(self, delta):
+        return self.map[max(0, min(int(delta) - self.lo, len(self.map) - 1))]
+
+    def on(self, device):
+        """the map as an int32 tensor on this device (made at the first call there, which must not be inside a graph capture)"""
+        t = self._on.get(device)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise L.SmxError("RelPos: its map is copied to a device at the first use there: call it once before the capture")
+            t = self._on[device] = torch.tensor(self.map, dtype=torch.int32, device=device)
+            torch.cuda.current_stream(device).synchronize()   # whole before any stream reads it
+        return t
+
+
+@functools.lru_cache(maxsize=None)
+def relpos(num_buckets=32, max_distance=128, two_sided=True):
+    """the RelPos of these numbers, one object for all callers."""
+    return RelPos(num_buckets, max_distance, two_sided)
+
+
+def _rows3(t, what, B, width, like):
+    """(address, row stride, sample stride) of [B, N, width] rows: dense channels, any row and sample strides that are multiples of four"""
+    if t.dim() != 3 or t.shape[0] != B or t.shape[2] != width or t.dtype != like.dtype or t.device != like.device:
+        raise L.SmxError(f"{what}: [{B}, N, {width}] {like.dtype} on {like.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    bs, ld, one = t.stride()
+    ld = ld if t.shape[1] > 1 else width
+    bs = bs if B > 1 else 0
+    if (one != 1 and width > 1) or ld < width or ld % 4 or bs % 4 or t.data_ptr() % (4 * t.element_size()) or ld > 0x7fffffff:
+        raise L.SmxError(f"{what}: dense channels, row and sample strides in multiples of four elements and rows that start on one are needed, "
+                         f"got strides {t.stride()} at {t.data_ptr():#x}")
+    return t.data_ptr(), ld, bs
+
+
+def _relpos_desc(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale):
+    """the fields of smx_relpos_desc that forward and backward share."""
+    _dev(q, "attention_relpos q", _ANY)
+    _dev(k, "attention_relpos k", _ANY)
+    _dev(v, "attention_relpos v", _ANY)
+    if not isinstance(rp, RelPos):
+        raise L.SmxError(f"attention_relpos: a RelPos expected, got {type(rp).__name__}")
+    nkv = nhead if nkv is None else nkv
+    if q.dim() != 3 or k.dim() != 3 or nhead < 1 or nkv < 1 or nhead % nkv or q.shape[2] % nhead:
+        raise L.SmxError(f"attention_relpos: q [B, L, heads * dh] and k / v [B, S, kv heads * dh] expected, got {tuple(q.shape)} / {tuple(k.shape)} with "
+                         f"{nhead} heads on {nkv}")
+    B, Lq, E = q.shape
+    S, dh = k.shape[1], E // nhead
+    if dh % 4 or not 4 <= dh <= 128 or E > 1 << 20 or B * nhead > 1 << 24 or max(Lq, S) > 1 << 30:
+        raise L.SmxError(f"attention_relpos: a head size of 4 to 128 in steps of four expected, got {dh} (B {B}, L {Lq}, S {S}, {nhead} heads)")
+    d = L.RelposDesc(B=B, H=nhead, Hkv=nkv, L=Lq, S=S, dh=dh, map_lo=rp.lo, map_n=len(rp.map), num_buckets=rp.num_buckets, causal=int(bool(causal)),
+                     bf16=int(q.dtype == BF16), scale=dh ** -0.5 if scale is None else scale)
+    d.q, d.ldq, d.q_bs = _rows3(q, "attention_relpos q", B, E, q)
+    d.k, d.ldk, d.k_bs = _rows3(k, "attention_relpos k", B, nkv * dh, q)
+    d.v, d.ldv, d.v_bs = _rows3(v, "attention_relpos v", B, nkv * dh, q)
+    if v.shape[1] != S:
+        raise L.SmxError(f"attention_relpos: k and v have {S} and {v.shape[1]} rows")
+    d.table = _vec(table, "attention_relpos table", (rp.num_buckets, nhead), q)
+    d.map = rp.on(q.device).data_ptr()
+    if mask is not None:
+        d.mask = _vec(mask.view(torch.uint8) if torch.is_tensor(mask) and mask.dtype == torch.bool else mask, "attention_relpos mask", (B, S), q, torch.uint8)
+    if kv_len is not None:
+        d.kv_len = _vec(kv_len, "attention_relpos kv_len", (B,), q, torch.int32)
+    if q_start is not None:
+        if abs(q_start) > 1 << 30:
+            raise L.SmxError(f"attention_relpos: q_start {q_start} is out of range")
+        d.has_q_start, d.q_start = 1, q_start
+    return d
+
+
+def attention_relpos(q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None, _lse=None):
+    """Attention with a learned relative position bias: o_i = softmax_j(scale q_i . k_j + table[rp.bucket(j - pos_i)][head]) v_j per head.
+    q [B, L, nhead * dh], k / v [B, S, nkv * dh] (fp32 or bf16; views of a fused projection are fine; head h reads kv head
+    h // (nhead / nkv)), dh a multiple of four up to 128; table fp32 [rp.num_buckets, nhead]; scale: dh^-1/2 by default.
+    kv_len int32 [B]: sample b has the first kv_len[b] of the S keys (clamped to 0..S).  Positions: key j is at j, query i at q_start + i,
+    by default the queries are the last L of the sample's keys -- all of them in self attention, the newest one with L = 1.
+    causal: keys behind the query's position are left out; mask uint8 or bool [B, S], nonzero: key left out.  What left-out keys of `mask` and
+    `kv_len` hold is not used, whatever it is.  A query with no key left answers zeros.  -> o [B, L, nhead * dh]."""
+    d = _relpos_desc(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale)
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if not d.S or not o.numel():
+        return o.zero_()
+    lib = L.load()
+    d.o, d.ldo, d.o_bs = o.data_ptr(), q.shape[2], q.shape[1] * q.shape[2]
+    d.lse = None if _lse is None else _lse.data_ptr()
+    n = lib.smx_attention_relpos_ws_bytes(C.byref(d))
+    ws = torch.empty((n,), device=q.device, dtype=torch.uint8) if n > 0 else None
+    d.ws, d.ws_bytes = None if ws is None else ws.data_ptr(), n
+    meta = {"flops": 4.0 * d.B * nhead * d.L * d.S * d.dh, "bytes": q.element_size() * 2.0 * (q.numel() + k.numel())}
+    L.check(_timed(f"attention_relpos_d{d.dh}", meta, _call, q, lib.smx_attention_relpos, C.byref(d)), "attention_relpos")
     return o

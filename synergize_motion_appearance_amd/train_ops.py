@@ -475,6 +475,48 @@ def layernorm(tp, x, gamma, beta, pos=None, eps=1e-5):
     return y, yp
 
 
+def norm_residual(tp, x, h, *, post=None, gate=None, res_scale=1.0, pre=None, kind="layer", eps=1e-5):
+    """ops.norm_residual (fp32) -> (x', y or None).  post / pre: (gamma, beta) or (gamma,) as parameter references; gate: a parameter
+    reference ([E] or [G, E]) or a tensor whose gradient the tape collects (a projection's output, a `leaf`)."""
+    if x.dtype != F32 or h.dtype != F32:
+        raise L.SmxError(f"norm_residual: the training step is fp32, got {x.dtype} / {h.dtype}")
+    xc = x if x.is_contiguous() else _dense(tp.lib, x)
+    hc = h if h.is_contiguous() else _dense(tp.lib, h)
+    pv, pg = zip(*((_param(tp, r)[:2]) for r in post)) if post is not None else (None, ())
+    nv, ng = zip(*((_param(tp, r)[:2]) for r in pre)) if pre is not None else (None, ())
+    gv, gg = (gate, None) if gate is None or torch.is_tensor(gate) else _param(tp, gate)[:2]
+    xo, y = ops.norm_residual(xc, hc, post=pv, gate=gv, res_scale=res_scale, pre=nv, kind=kind, eps=eps)
+
+    def bwd():
+        gx, gy = tp.take(xo), (tp.take(y) if y is not None else None)
+        if (gx is None and gy is None) or not xo.numel():
+            return
+        lib = tp.lib
+        gx = gx if gx is None or gx.is_contiguous() else _dense(lib, gx)
+        gy = gy if gy is None or gy.is_contiguous() else _dense(lib, gy)
+        d = ops._norm_residual_desc(xc, hc, pv, gv, res_scale, nv, kind, eps)
+        dx = _empty(x.shape, x) if tp.needs(x) else None
+        dh = _empty(h.shape, h) if tp.needs(h) else None
+        dgate = gg if gg is not None else _empty(gv.shape, gv) if gv is not None and torch.is_tensor(gate) and tp.needs(gate) else None
+        d.xo, d.gate_accumulate = xo.data_ptr(), int(gg is not None)
+        for n, t in (("gx", gx), ("gy", gy), ("dx", dx), ("dh", dh), ("dgate", dgate)):
+            setattr(d, n, None if t is None else t.data_ptr())
+        for n, t in list(zip(("dpost_gamma", "dpost_beta"), pg)) + (list(zip(("dpre_gamma", "dpre_beta"), ng)) if gy is not None else []):
+            setattr(d, n, None if t is None else t.data_ptr())
+        n = int(lib.smx_norm_residual_bwd_ws_floats(d.T, d.groups, d.E))
+        ws = torch.empty((n,), device=x.device, dtype=F32)
+        d.ws, d.ws_floats = ws.data_ptr(), n
+        L.check(ops._call(x, lib.smx_norm_residual_bwd_f32, C.byref(d)), "norm_residual_bwd")
+        if dx is not None:
+            tp.acc(x, dx)
+        if dh is not None:
+            tp.acc(h, dh)
+        if gg is None and dgate is not None:
+            tp.acc(gate, dgate)
+    tp.record(bwd)
+    return xo, y
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 def attention(tp, q, k, v, nhead, dh, S, *, mask=None, ctx=None):
     """o = softmax(q k^T / sqrt(dh) [+ key mask]) v per head.  Self attention: q, k, v dense [B,L,E].  Cross attention against a
@@ -517,6 +559,41 @@ def attention(tp, q, k, v, nhead, dh, S, *, mask=None, ctx=None):
         else:
             tp.acc(k, dk.view(k.shape))
             tp.acc(v, dv.view(v.shape))
+    tp.record(bwd)
+    return o
+
+
+def attention_relpos(tp, q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None):
+    """ops.attention_relpos (fp32); table: parameter reference [rp.num_buckets, nhead].  The gradients of masked keys and of keys behind
+    kv_len are zeros, those of a query with no key left too; shared kv heads collect the sums over their heads."""
+    tv, tg, _ = _param(tp, table)
+    if q.dtype != F32:
+        raise L.SmxError(f"attention_relpos: the training step is fp32, got {q.dtype}")
+    lse = _empty((q.shape[0], nhead, q.shape[1]), q)
+    o = ops.attention_relpos(q, k, v, tv, rp, nhead, nkv=nkv, causal=causal, mask=mask, kv_len=kv_len, q_start=q_start, scale=scale, _lse=lse)
+
+    def bwd():
+        g = tp.take(o)
+        if g is None:
+            return
+        if not o.numel() or not k.numel():
+            for t in (q, k, v):
+                tp.acc(t, _zeros(t.shape, t))
+            return
+        lib = tp.lib
+        g = g if g.is_contiguous() and g.data_ptr() % 16 == 0 else _dense(lib, g)
+        d = ops._relpos_desc(q, k, v, tv, rp, nhead, nkv, causal, mask, kv_len, q_start, scale)
+        dq, dk, dv = _empty(q.shape, q), _empty(k.shape, k), _empty(v.shape, v)
+        dt = tg if tg is not None else _zeros(tv.shape, tv)
+        d.o, d.ldo, d.o_bs, d.lse, d.d_o = o.data_ptr(), q.shape[2], q.shape[1] * q.shape[2], lse.data_ptr(), g.data_ptr()
+        d.dq, d.dk, d.dv, d.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
+        n = int(lib.smx_attention_relpos_bwd_ws_bytes(C.byref(d)))
+        ws = torch.empty((max(n, 16),), device=q.device, dtype=torch.uint8)
+        d.ws, d.ws_bytes = ws.data_ptr(), n
+        L.check(ops._call(q, lib.smx_attention_relpos_bwd_f32, C.byref(d)), "attention_relpos_bwd")
+        tp.acc(q, dq)
+        tp.acc(k, dk)
+        tp.acc(v, dv)
     tp.record(bwd)
     return o
 
