@@ -1,0 +1,154 @@
+// What the forward and backward kernels of the attention with a relative position bias share (relpos_attn.hip, relpos_attn_bwd.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <math.h>
+#include "smx.h"
+#include "smx_common.h"
+#include "bf16.h"
+
+namespace relpos {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int MAP_MAX = 2049;         // entries of a bucket map
+constexpr int TABLE_PAD = 96;         // entries a 64-key x 32-query tile can reach beyond the map's ends while it touches the map
+
+// ---- fp32 operands on the half-precision matrix pipe ("f16x3") ----------------------------------------------------------------
+// x = (h1 + h2) 2^-k with two IEEE halves: 22 significand bits; a product is h1 g1 + h1 g2 + h2 g1, the dropped h2 g2 is 2^-22 of it.  k is one number per
+// (sample, head) that brings the largest |x| to [2^14, 2^15): values down to 2^-16 of the largest keep all 22 bits, smaller ones are off by at most
+// 2^-40 of the largest.  A first pass finds the largest values, a second writes the halves: planes [B][heads][rows rounded up to 64][DHP] of h1 and of h2,
+// rows that nobody may see and the columns from dh on as zeros.  That is read by every tile of the other side, so splitting here once costs less than
+// splitting in the kernels (a 128-query block would split every key of its head again).
+struct Split {
+  const float* src; long long bs; int ld, heads, rows, kv;      // kv: rows of keys (masks and lengths apply)
+  _Float16* hi; _Float16* lo;                                   // planes
+  float* top;                                                   // [B][heads][nch] largest |x| of each chunk of CH rows
+  const float* o;                                               // gradient rows: the output, for D_i = dO_i . o_i (dense, as src)
+  float* dd;                                                    // [B][heads][rows rounded up to 64]
+};
+constexpr int CH = 512;
+
+struct RP {
+  const void* q; const void* k; const void* v; void* o;
+  const float* table; const int* map; const uint8_t* mask; const int* kv_len;
+  float* lse; const float* d_o; float* dq; float* dk; float* dv; float* dtable;
+  long long q_bs, k_bs, v_bs, o_bs;
+  int ldq, ldk, ldv, ldo;
+  int B, H, Hkv, G, L, S, dh, map_lo, map_n, nb, causal, has_start, q_start;
+  float scale;
+  __device__ __forceinline__ int keys(int b) const { return kv_len ? max(0, min(kv_len[b], S)) : S; }
+  __device__ __forceinline__ int pos0(int n) const { return has_start ? q_start : n - L; }
+  __device__ __forceinline__ int entry(int delta) const { return max(0, min(delta - map_lo, map_n - 1)); }
+};
+
+static inline int up64(int n) { return (n + 63) & ~63; }
+static inline int dhp(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : 128; }
+static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
+// 2^k and 2^-k of a head from its chunks' largest values
+__device__ __forceinline__ float head_pow2(const float* top, int nch, float& inv) {
+  float m = 0.f;
+  for (int c = 0; c < nch; ++c) m = fmaxf(m, top[c]);
+  const int e = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;     // floor(log2 m); 2^(14 - e) stays a normal number
+  inv = __uint_as_float((unsigned)(e - 14 + 127) << 23);
+  return __uint_as_float((unsigned)(14 - e + 127) << 23);
+}
+
+// the launchers of relpos_attn.hip
+int check(const smx_relpos_desc* d, RP& p, bool bwd);
+int64_t split_bytes(int B, int heads, int rows, int dhp);       // planes + chunk maxima
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dhp, bool kv);
+int split_launch(const RP& p, const Split* s, int n, hipStream_t st);
+
+// ---- matrix operands -----------------------------------------------------------------------------------------------------------
+template <int NL>
+__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+  if constexpr (NL == 1) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+// c += a b over the levels, the smallest products first
+template <int NL>
+__device__ __forceinline__ f32x16 mfma_levels(const uint4 (&a)[NL], const uint4 (&b)[NL], f32x16 c) {
+  if constexpr (NL == 2) {
+    c = mfma<2>(a[1], b[0], c);
+    c = mfma<2>(a[0], b[1], c);
+  }
+  return mfma<NL>(a[0], b[0], c);
+}
+// eight fp32 -> the levels' fragments (bf16: one, rounded to nearest; halves: two)
+template <int NL>
+__device__ __forceinline__ void to_levels(const float* v, uint4 (&f)[NL]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (NL == 1) h[i] = cvt2_bf16(v[2 * i], v[2 * i + 1]);
+    else {
+      h[i] = cvt2_f16(v[2 * i], v[2 * i + 1]);
+      l[i] = cvt2_f16(v[2 * i] - f16lo(h[i]), v[2 * i + 1] - f16hi(h[i]));
+    }
+  }
+  f[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  if constexpr (NL == 2) f[1] = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// a tile's row r of the 32x32 accumulator layout that a lane's register i holds: (i & 3) + 8 (i >> 2) + 4 (lane >> 5)
+__device__ __forceinline__ constexpr int crow(int i) { return (i & 3) + 8 * (i >> 2); }
+
+// Tiles in LDS: [row][DHP] 16-bit values, rows 16 bytes further apart than they are long: both the row fragments (16 B at row lane & 31) and the transposed
+// reads (8 B at four rows by four columns a lane group) then fall on different banks.
+template <int DHP> constexpr int ROWB = DHP * 2 + 16;
+
+// operand fragment of 16 columns kk of the tile's row r0 + (lane & 31)
+template <int DHP>
+__device__ __forceinline__ uint4 row_frag(const char* tile, int r0, int kk) {
+  const int lane = threadIdx.x & 63;
+  return *reinterpret_cast<const uint4*>(tile + (r0 + (lane & 31)) * ROWB<DHP> + kk * 32 + (lane >> 5) * 16);
+}
+// the transposed fragment: lane holds column 32 dt + (lane & 31) at the 16 rows from r0 on that an accumulator's eight registers hold
+// (4 hh + 0..3 and 8 + 4 hh + 0..3): two transposing reads of 4 rows x 16 columns a lane group
+template <int DHP>
+__device__ __forceinline__ uint4 col_frag(char* tile, int r0, int dt) {
+  const int lane = threadIdx.x & 63, l = lane & 15;
+  char* at = tile + (r0 + (lane >> 5) * 4 + (l >> 2)) * ROWB<DHP> + dt * 64 + ((lane >> 4) & 1) * 32 + (l & 3) * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * ROWB<DHP>));
+  return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// the other 32 lanes' value
+__device__ __forceinline__ float other_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float other_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Work order: consecutive block ids go to the 8 XCDs in turn; this gives each XCD a run of consecutive work items, so that the blocks that read the
+// same keys share an L2.
+__device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned n) {
+  const unsigned x = id & 7, s = id >> 3, q = n >> 3, r = n & 7;
+  return x < r ? x * (q + 1) + s : r * (q + 1) + (x - r) * q + s;
+}
+
+// the head's bias in log2 units by map entry, TABLE_PAD more of its ends' values on both sides
+__device__ __forceinline__ void fill_bias(float* lut, const RP& p, int h) {
+  for (int t = threadIdx.x; t < p.map_n + 2 * TABLE_PAD; t += blockDim.x) {
+    const int e = max(0, min(t - TABLE_PAD, p.map_n - 1));
+    lut[t] = p.table[(long long)p.map[e] * p.H + h] * LOG2E;
+  }
+}
+
+}  // namespace relpos

@@ -1,216 +1,113 @@
-// Attention with a learned relative position bias by buckets (include/smx.h: smx_attention_relpos, smx_attention_relpos_bwd_f32).
+// Attention with a learned relative position bias by buckets, forward (include/smx.h: smx_attention_relpos):
 //   s_ij = scale q_i . k_j + table[map[clamp(j - pos_i - map_lo)]][h],  P = softmax over the keys that are left,  o_i = sum_j P_ij v_j
-//   D_i = sum_d dO_id o_id,  dS_ij = P_ij (dO_i . v_j - D_i),  dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
-//   dv_j = sum_i P_ij dO_i,  dtable[b][h] = sum of dS_ij over the pairs of bucket b
-// Scores are kept in log2 units; lse_i = log2 sum_j 2^{s_ij}, +inf for a row with no key left, so that 2^{s - lse} is 0 there.
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-#include <math.h>
-#include "smx.h"
-#include "smx_common.h"
-#include "bf16.h"
+// One pass over the keys with the running maximum and sum of the softmax, scores in log2 units.  Two kernels and what they need:
+//   relpos_tile_kernel   queries in tiles of 32 a wave on the matrix cores (bf16 storage: bf16 products; fp32 storage: f16x3, relpos.h)
+//   relpos_token_kernel  a few queries per sample (decoding): bound by reading the cache, plain fp32 products on the vector units
+//   relpos_join_kernel   joins the parts where the keys were split over blocks
+//   relpos_top / split   the fp32 operands as two halves each
+#include "relpos.h"
 
-namespace {
+namespace relpos {
 
-constexpr float LOG2E = 1.44269504088896340736f;
+// ---- fp32 operands as halves (relpos.h: Split) ---------------------------------------------------------------------------------
+struct Splits { Split s[4]; int end[4]; };                       // end: running sum of blocks
 
-struct RP {
-  const void* q; const void* k; const void* v; void* o;
-  const float* table; const int* map; const uint8_t* mask; const int* kv_len;
-  float* lse; const float* d_o; float* dq; float* dk; float* dv; float* dtable;
-  long long q_bs, k_bs, v_bs, o_bs;
-  int ldq, ldk, ldv, ldo;
-  int B, H, Hkv, G, L, S, dh, map_lo, map_n, nb, causal, has_start, q_start;
-  float scale;
-  __device__ __forceinline__ int keys(int b) const { return kv_len ? max(0, min(kv_len[b], S)) : S; }
-  __device__ __forceinline__ int pos0(int n) const { return has_start ? q_start : n - L; }
-  __device__ __forceinline__ int entry(int delta) const { return max(0, min(delta - map_lo, map_n - 1)); }
-};
+__device__ __forceinline__ bool row_seen(const RP& p, const Split& s, int b, int r) {
+  if (r >= s.rows) return false;
+  return !s.kv || (r < p.keys(b) && !(p.mask && p.mask[(long long)b * p.S + r]));
+}
 
-__device__ __forceinline__ float wave_sum(float v) {
+// largest |x| of CH rows of one head; NaN and rows nobody sees do not count
+__global__ __launch_bounds__(256) void relpos_top_kernel(RP p, Splits a) {
+  __shared__ float red[4];
+  int t = 0, id = blockIdx.x;
+  while (id >= a.end[t]) ++t;
+  const Split& s = a.s[t];
+  id -= t ? a.end[t - 1] : 0;
+  const int nch = (s.rows + CH - 1) / CH, c = id % nch, h = id / nch % s.heads, b = id / nch / s.heads;
+  const int q4 = p.dh >> 2, n = min(CH, s.rows - c * CH) * q4;
+  const float* src = s.src + b * s.bs + (long long)c * CH * s.ld + h * p.dh;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = i / q4;
+    if (!row_seen(p, s, b, c * CH + r)) continue;
+    const float4 x = *reinterpret_cast<const float4*>(src + (long long)r * s.ld + (i - r * q4) * 4);
+    m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
-// the log2-unit score of one pair, -inf where the key is not left
-template <typename T>
-__device__ __forceinline__ float score(const RP& p, const T* Q, const T* K, int b, int h, int j, int n, int pos) {
-  const int delta = j - pos;
-  if (j >= n || (p.causal && delta > 0) || (p.mask && p.mask[(long long)b * p.S + j])) return -INFINITY;
-  const T* kr = K + (long long)j * p.ldk;
-  float a = 0.f;
-  for (int d = 0; d < p.dh; d += 4) {
-    const float4 x = St<T>::ld4(Q + d), y = St<T>::ld4(kr + d);
-    a += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-  }
-  return (a * p.scale + p.table[(long long)p.map[p.entry(delta)] * p.H + h]) * LOG2E;
-}
-
-// one wave per query row: lane = key for the scores, lane = head column (two of them) for the output
-template <typename T>
-__global__ __launch_bounds__(256) void relpos_rows_kernel(RP p) {
-  const int lane = threadIdx.x & 63;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
-  if (row >= (long long)p.B * p.H * p.L) return;
-  const int i = (int)(row % p.L), h = (int)(row / p.L % p.H), b = (int)(row / p.L / p.H), hk = h / p.G;
-  const int n = p.keys(b), pos = p.pos0(n) + i;
-  const T* Q = (const T*)p.q + b * p.q_bs + (long long)i * p.ldq + h * p.dh;
-  const T* K = (const T*)p.k + b * p.k_bs + hk * p.dh;
-  const T* V = (const T*)p.v + b * p.v_bs + hk * p.dh;
-  float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int j0 = 0; j0 < n; j0 += 64) {
-    const float s = score<T>(p, Q, K, b, h, j0 + lane, n, pos);
-    const float mn = fmaxf(m, wave_max(s));
-    if (mn == -INFINITY) continue;
-    const float al = exp2f(m - mn), e = exp2f(s - mn);
-    l = l * al + wave_sum(e); a0 *= al; a1 *= al; m = mn;
-    for (int t = 0; t < 64; ++t) {
-      const float pt = __shfl(e, t, 64);
-      if (pt == 0.f) continue;
-      const T* vr = V + (long long)(j0 + t) * p.ldv;
-      if (lane < p.dh) a0 += pt * St<T>::ld(vr + lane);
-      if (lane + 64 < p.dh) a1 += pt * St<T>::ld(vr + lane + 64);
-    }
-  }
-  T* O = (T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh;
-  const float il = l > 0.f ? 1.f / l : 0.f;
-  if (lane < p.dh) St<T>::st(O + lane, a0 * il);
-  if (lane + 64 < p.dh) St<T>::st(O + lane + 64, a1 * il);
-  if (p.lse && lane == 0) p.lse[row] = l > 0.f ? m + log2f(l) : INFINITY;
-}
-
-__device__ __forceinline__ float dot(const float* a, const float* b, int n) {
-  float s = 0.f;
-  for (int d = 0; d < n; d += 4) {
-    const float4 x = St<float>::ld4(a + d), y = St<float>::ld4(b + d);
-    s += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-  }
-  return s;
-}
-
-// dq: one wave per query row; the row's D goes to `dd` for the other two kernels
-__global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RP p, float* __restrict__ dd) {
-  const int lane = threadIdx.x & 63;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
-  if (row >= (long long)p.B * p.H * p.L) return;
-  const int i = (int)(row % p.L), h = (int)(row / p.L % p.H), b = (int)(row / p.L / p.H), hk = h / p.G;
-  const int n = p.keys(b), pos = p.pos0(n) + i;
-  const float* Q = (const float*)p.q + b * p.q_bs + (long long)i * p.ldq + h * p.dh;
-  const float* K = (const float*)p.k + b * p.k_bs + hk * p.dh;
-  const float* V = (const float*)p.v + b * p.v_bs + hk * p.dh;
-  const long long od = ((long long)b * p.L + i) * p.H * p.dh + h * p.dh;
-  const float D = dot(p.d_o + od, (const float*)p.o + od, p.dh), lse = p.lse[row];
-  float a0 = 0.f, a1 = 0.f;
-  for (int j0 = 0; j0 < n; j0 += 64) {
-    const float s = score<float>(p, Q, K, b, h, j0 + lane, n, pos);
-    const float ds = s == -INFINITY ? 0.f : exp2f(s - lse) * (dot(p.d_o + od, V + (long long)(j0 + lane) * p.ldv, p.dh) - D);
-    for (int t = 0; t < 64; ++t) {
-      const float w = __shfl(ds, t, 64);
-      if (w == 0.f) continue;
-      const float* kr = K + (long long)(j0 + t) * p.ldk;
-      if (lane < p.dh) a0 += w * kr[lane];
-      if (lane + 64 < p.dh) a1 += w * kr[lane + 64];
-    }
-  }
-  if (lane < p.dh) p.dq[od + lane] = a0 * p.scale;
-  if (lane + 64 < p.dh) p.dq[od + lane + 64] = a1 * p.scale;
-  if (lane == 0) dd[row] = D;
-}
-
-// dk, dv: one wave per key row, over the queries of the heads that share it
-__global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RP p, const float* __restrict__ dd) {
-  const int lane = threadIdx.x & 63;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
-  if (row >= (long long)p.B * p.Hkv * p.S) return;
-  const int j = (int)(row % p.S), hk = (int)(row / p.S % p.Hkv), b = (int)(row / p.S / p.Hkv);
-  const int n = p.keys(b);
-  const float* K = (const float*)p.k + b * p.k_bs + hk * p.dh;
-  const float* V = (const float*)p.v + b * p.v_bs + hk * p.dh;
-  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  if (j < n)
-    for (int h = hk * p.G; h < (hk + 1) * p.G; ++h)
-      for (int i0 = 0; i0 < p.L; i0 += 64) {
-        const int i = i0 + lane;
-        float pij = 0.f, ds = 0.f;
-        if (i < p.L) {
-          const long long r = ((long long)b * p.H + h) * p.L + i;
-          const float s = score<float>(p, (const float*)p.q + b * p.q_bs + (long long)i * p.ldq + h * p.dh, K, b, h, j, n, p.pos0(n) + i);
-          if (s != -INFINITY) {
-            pij = exp2f(s - p.lse[r]);
-            ds = pij * (dot(p.d_o + ((long long)b * p.L + i) * p.H * p.dh + h * p.dh, V + (long long)j * p.ldv, p.dh) - dd[r]);
-          }
-        }
-        for (int t = 0; t < 64; ++t) {
-          const float pt = __shfl(pij, t, 64), dt = __shfl(ds, t, 64);
-          if (pt == 0.f) continue;
-          const float* qr = (const float*)p.q + b * p.q_bs + (long long)(i0 + t) * p.ldq + h * p.dh;
-          const float* gr = p.d_o + ((long long)b * p.L + i0 + t) * p.H * p.dh + h * p.dh;
-          if (lane < p.dh) { k0 += dt * qr[lane]; v0 += pt * gr[lane]; }
-          if (lane + 64 < p.dh) { k1 += dt * qr[lane + 64]; v1 += pt * gr[lane + 64]; }
-        }
-      }
-  const long long od = ((long long)b * p.S + j) * p.Hkv * p.dh + hk * p.dh;
-  if (lane < p.dh) { p.dk[od + lane] = k0 * p.scale; p.dv[od + lane] = v0; }
-  if (lane + 64 < p.dh) { p.dk[od + lane + 64] = k1 * p.scale; p.dv[od + lane + 64] = v1; }
-}
-
-// sums of dS per (map entry, head): one block per pair of them, threads over the samples' queries whose key of that distance exists
-// (the two ends of the map stand for all distances beyond them)
-__global__ __launch_bounds__(256) void relpos_bwd_entry_kernel(RP p, const float* __restrict__ dd, float* __restrict__ part) {
-  __shared__ float red[256];
-  const int e = blockIdx.x, h = blockIdx.y, hk = h / p.G;
-  float a = 0.f;
-  for (int b = 0; b < p.B; ++b) {
-    const int n = p.keys(b);
-    const float* K = (const float*)p.k + b * p.k_bs + hk * p.dh;
-    const float* V = (const float*)p.v + b * p.v_bs + hk * p.dh;
-    for (int i = threadIdx.x; i < p.L; i += 256) {
-      const int pos = p.pos0(n) + i;
-      const long long r = ((long long)b * p.H + h) * p.L + i;
-      int j0 = pos + p.map_lo + e, j1 = j0 + 1;
-      if (e == 0) j0 = 0;
-      if (e == p.map_n - 1) j1 = n;
-      for (int j = max(j0, 0); j < min(j1, n); ++j) {
-        const float s = score<float>(p, (const float*)p.q + b * p.q_bs + (long long)i * p.ldq + h * p.dh, K, b, h, j, n, pos);
-        if (s != -INFINITY)
-          a += exp2f(s - p.lse[r]) * (dot(p.d_o + ((long long)b * p.L + i) * p.H * p.dh + h * p.dh, V + (long long)j * p.ldv, p.dh) - dd[r]);
-      }
-    }
-  }
-  red[threadIdx.x] = a;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  for (int s = 128; s > 0; s >>= 1) {
-    if (threadIdx.x < s) red[threadIdx.x] += red[threadIdx.x + s];
-    __syncthreads();
+  if (threadIdx.x == 0) s.top[((long long)b * s.heads + h) * nch + c] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// 64 rows of one head -> both planes; gradient rows: D_i = dO_i . o_i too
+template <int DHP>
+__global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
+  int t = 0, id = blockIdx.x;
+  while (id >= a.end[t]) ++t;
+  const Split& s = a.s[t];
+  id -= t ? a.end[t - 1] : 0;
+  const int nch = (s.rows + CH - 1) / CH, nt = (s.rows + 63) / 64, c = id % nt, h = id / nt % s.heads, b = id / nt / s.heads;
+  float inv;
+  const float sc = head_pow2(s.top + ((long long)b * s.heads + h) * nch, nch, inv);
+  constexpr int Q4 = DHP / 4;
+  const long long out = (((long long)b * s.heads + h) * nt + c) * 64 * DHP;
+#pragma unroll
+  for (int it = 0; it < 64 * Q4 / 256; ++it) {
+    const int i = it * 256 + threadIdx.x, r = i / Q4, d = i % Q4 * 4, row = c * 64 + r;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long at = b * s.bs + (long long)row * s.ld + h * p.dh + d;
+    const bool in = d < p.dh && row_seen(p, s, b, row);
+    if (in) x = *reinterpret_cast<const float4*>(s.src + at);
+    if (s.dd) {
+      float D = 0.f;
+      if (in) { const float4 y = *reinterpret_cast<const float4*>(s.o + at); D = (x.x * y.x + x.y * y.y) + (x.z * y.z + x.w * y.w); }
+#pragma unroll
+      for (int o = 1; o < Q4; o <<= 1) D += __shfl_xor(D, o, 64);
+      if (d == 0) s.dd[((long long)b * s.heads + h) * nt * 64 + row] = D;
+    }
+    x.x *= sc; x.y *= sc; x.z *= sc; x.w *= sc;
+    const uint2 h2 = make_uint2(cvt2_f16(x.x, x.y), cvt2_f16(x.z, x.w));
+    const uint2 l2 = make_uint2(cvt2_f16(x.x - f16lo(h2.x), x.y - f16hi(h2.x)), cvt2_f16(x.z - f16lo(h2.y), x.w - f16hi(h2.y)));
+    *reinterpret_cast<uint2*>(s.hi + out + i * 4) = h2;
+    *reinterpret_cast<uint2*>(s.lo + out + i * 4) = l2;
   }
-  if (threadIdx.x == 0) part[(long long)h * p.map_n + e] = red[0];
 }
 
-// dtable[bucket][h] += the entries of that bucket
-__global__ __launch_bounds__(256) void relpos_bwd_table_kernel(RP p, const float* __restrict__ part) {
-  const int at = blockIdx.x * 256 + threadIdx.x;
-  if (at >= p.nb * p.H) return;
-  const int bucket = at / p.H, h = at - bucket * p.H;
-  float a = 0.f;
-  for (int e = 0; e < p.map_n; ++e)
-    if (p.map[e] == bucket) a += part[(long long)h * p.map_n + e];
-  p.dtable[at] += a;
+int64_t split_bytes(int B, int heads, int rows, int dh) {
+  return (int64_t)B * heads * ((int64_t)up64(rows) * dhp(dh) * 4 + (((rows + CH - 1) / CH + 3) / 4 * 16));
 }
 
-bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dh, bool kv) {
+  const int64_t plane = (int64_t)B * heads * up64(rows) * dhp(dh);
+  s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.rows = rows; s.kv = kv;
+  s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.top = (float*)(s.lo + plane);
+  s.o = nullptr; s.dd = nullptr;
+  return ws + split_bytes(B, heads, rows, dh);
+}
 
-// what both entry points ask of their arguments; fills RP
+int split_launch(const RP& p, const Split* s, int n, hipStream_t st) {
+  Splits a, c;
+  long long na = 0, nc = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (i < n) { a.s[i] = c.s[i] = s[i]; na += (long long)p.B * s[i].heads * ((s[i].rows + CH - 1) / CH); nc += (long long)p.B * s[i].heads * (up64(s[i].rows) / 64); }
+    if (na > 0x7fffffffLL || nc > 0x7fffffffLL) return SMX_EINVAL;
+    a.end[i] = (int)na; c.end[i] = (int)nc;
+  }
+  SMX_LAUNCH(relpos_top_kernel, dim3((unsigned)na), dim3(256), 0, st, p, a);
+  const int w = dhp(p.dh);
+  if (w == 32) SMX_LAUNCH(relpos_split_kernel<32>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
+  else if (w == 64) SMX_LAUNCH(relpos_split_kernel<64>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
+  else SMX_LAUNCH(relpos_split_kernel<128>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
+  return smx_launch_status();
+}
+
 int check(const smx_relpos_desc* d, RP& p, bool bwd) {
   if (!d || !d->q || !d->k || !d->v || !d->o || !d->table || !d->map) return SMX_EINVAL;
   if (d->B <= 0 || d->H <= 0 || d->Hkv <= 0 || d->H % d->Hkv || d->L <= 0 || d->S <= 0 || d->dh <= 0 || d->dh % 4 || d->dh > 128) return SMX_EINVAL;
-  if ((long long)d->H * d->dh > (1 << 20) || (long long)d->B * d->H > (1 << 24) || d->L > (1 << 30) || d->S > (1 << 30)) return SMX_EINVAL;
-  if (d->map_n <= 0 || d->map_n > 2049 || d->map_lo > 0 || d->map_lo + d->map_n <= 0 || d->num_buckets <= 0 || d->num_buckets > 4096) return SMX_EINVAL;
+  if ((long long)d->H * d->dh > (1 << 20) || (long long)d->B * d->H > (1 << 24) || d->L > (1 << 29) || d->S > (1 << 29)) return SMX_EINVAL;
+  if (d->map_n <= 0 || d->map_n > MAP_MAX || d->map_lo > 0 || d->map_lo + d->map_n <= 0 || d->num_buckets <= 0 || d->num_buckets > 4096) return SMX_EINVAL;
   if (d->has_q_start && (d->q_start > (1 << 30) || d->q_start < -(1 << 30))) return SMX_EINVAL;
   if (!(d->scale == d->scale) || (d->bf16 != 0 && d->bf16 != 1) || (bwd && d->bf16)) return SMX_EINVAL;
   if (d->ldq < d->H * d->dh || d->ldk < d->Hkv * d->dh || d->ldv < d->Hkv * d->dh || d->ldo < d->H * d->dh) return SMX_EINVAL;
@@ -229,42 +126,523 @@ int check(const smx_relpos_desc* d, RP& p, bool bwd) {
   return SMX_OK;
 }
 
+}  // namespace relpos
+
+namespace {
+using namespace relpos;
+
+// ---- queries in tiles ----------------------------------------------------------------------------------------------------------
+// where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage the planes; parts: m, l [row][part], o [row][part][dh] when the keys are split
+struct Src {
+  Split q, k, v;
+  int nparts, per;                    // parts of the keys, keys of a part (a multiple of 64)
+  float* part_ml; float* part_o;
+};
+
+// A wave owns 32 queries as the columns of swapped products: S^T = K Q^T (a lane: one query, 16 of 32 keys), O^T += V^T P^T with P taken from the score
+// registers as they are -- the transposing LDS reads fetch V's columns in the order of an accumulator's rows.  The statistics are lane-local but for one
+// exchange between the two half waves.  Four waves share the staged keys: 64 (32 for DHP = 128) a step, double buffered, the next tile's loads in flight
+// during the products.  The running maximum follows only when a row outgrows it by 2^8: P stays below 2^8 (with fp32 storage P carries 2^6 more, below
+// the largest half by 2^1, its second half then off by at most 2^-31 of the row's largest weight).
+// The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
+template <int DHP, int NL>
+__global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
+  constexpr int TK = DHP == 128 ? 32 : 64, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>;
+  constexpr int PLANE = TK * RB, STAGE = 2 * NL * PLANE;         // K levels, V levels
+  constexpr int CPR = DHP / 8, NCH = TK * CPR / 256;             // 16-byte chunks of a row; of a plane, a thread
+  constexpr float PSH = NL == 2 ? 6.f : 0.f;
+  extern __shared__ __attribute__((aligned(16))) char sm[];      // two stages, bias, masks
+  float* lut = reinterpret_cast<float*>(sm + 2 * STAGE);
+  unsigned long long* seen = reinterpret_cast<unsigned long long*>(sm + 2 * STAGE + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int nq = (p.L + 127) / 128;
+  unsigned id = xcd_order(blockIdx.x, gridDim.x);
+  const int qb = nq - 1 - id % nq;                               // causal: the longest rows first
+  id /= nq;
+  const int part = id % a.nparts;
+  id /= a.nparts;
+  const int h = id % p.H, b = id / p.H, hk = h / p.G;
+  const int n = p.keys(b), pos0 = p.pos0(n);
+  const int q0 = qb * 128 + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
+  const int wlast = pos0 + min(q0 + 31, p.L - 1);                // the wave's last position; none if q0 >= L
+  int kend = p.causal ? min(n, pos0 + min(qb * 128 + 127, p.L - 1) + 1) : n;
+  const int kbeg = a.nparts > 1 ? part * a.per : 0;
+  if (a.nparts > 1) kend = min(kend, kbeg + a.per);
+  const int ntiles = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
+
+  fill_bias(lut, p, h);
+  const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
+  float sc = p.scale * LOG2E, inv_v = 1.f;
+  uint4 qf[KS][NL];
+  if constexpr (NL == 2) {
+    float iq, ik;
+    const int cq = (p.L + CH - 1) / CH, ck = (p.S + CH - 1) / CH;
+    head_pow2(a.q.top + ((long long)b * p.H + h) * cq, cq, iq);
+    head_pow2(a.k.top + ((long long)b * p.Hkv + hk) * ck, ck, ik);
+    head_pow2(a.v.top + ((long long)b * p.Hkv + hk) * ck, ck, inv_v);
+    sc = sc * iq * ik;
+    const int up = (p.L + 63) & ~63;
+    const long long at = (((long long)b * p.H + h) * up + qi) * DHP + hh * 8;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      qf[kk][0] = qi < up ? *reinterpret_cast<const uint4*>(a.q.hi + at + kk * 16) : make_uint4(0, 0, 0, 0);
+      qf[kk][1] = qi < up ? *reinterpret_cast<const uint4*>(a.q.lo + at + kk * 16) : make_uint4(0, 0, 0, 0);
+    }
+  } else {
+    const bf16_t* Q = (const bf16_t*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      const int d = kk * 16 + hh * 8;
+      uint2 x = make_uint2(0, 0), y = make_uint2(0, 0);
+      if (qi < p.L && d < p.dh) x = *reinterpret_cast<const uint2*>(Q + d);
+      if (qi < p.L && d + 4 < p.dh) y = *reinterpret_cast<const uint2*>(Q + d + 4);
+      qf[kk][0] = make_uint4(x.x, x.y, y.x, y.y);
+    }
+  }
+
+  uint4 kreg[NL][NCH], vreg[NL][NCH];
+  unsigned long long sreg = 0;
+  auto load_tile = [&](int key0) {
+    if constexpr (NL == 2) {
+      const long long at = (((long long)b * p.Hkv + hk) * ((p.S + 63) & ~63) + key0) * DHP;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int e = (c * 256 + threadIdx.x) * 8;
+        kreg[0][c] = *reinterpret_cast<const uint4*>(a.k.hi + at + e); kreg[1][c] = *reinterpret_cast<const uint4*>(a.k.lo + at + e);
+        vreg[0][c] = *reinterpret_cast<const uint4*>(a.v.hi + at + e); vreg[1][c] = *reinterpret_cast<const uint4*>(a.v.lo + at + e);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int e = c * 256 + threadIdx.x, key = key0 + e / CPR, d = e % CPR * 8;
+        const bf16_t* K = (const bf16_t*)p.k + b * p.k_bs + (long long)key * p.ldk + hk * p.dh + d;
+        const bf16_t* V = (const bf16_t*)p.v + b * p.v_bs + (long long)key * p.ldv + hk * p.dh + d;
+        uint2 x = make_uint2(0, 0), y = x, z = x, w = x;
+        if (key < n && !(p.mask && p.mask[(long long)b * p.S + key])) {        // what a left-out place holds must not meet a zero weight: zeros instead
+          if (d < p.dh) { x = *reinterpret_cast<const uint2*>(K); z = *reinterpret_cast<const uint2*>(V); }
+          if (d + 4 < p.dh) { y = *reinterpret_cast<const uint2*>(K + 4); w = *reinterpret_cast<const uint2*>(V + 4); }
+        }
+        kreg[0][c] = make_uint4(x.x, x.y, y.x, y.y);
+        vreg[0][c] = make_uint4(z.x, z.y, w.x, w.y);
+      }
+    }
+    if (wave == 0) {
+      const int key = key0 + lane;
+      sreg = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
+    }
+  };
+  auto store_tile = [&](int buf) {
+    char* st = sm + buf * STAGE;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int e = c * 256 + threadIdx.x, off = e / CPR * RB + e % CPR * 16;
+#pragma unroll
+      for (int l = 0; l < NL; ++l) {
+        *reinterpret_cast<uint4*>(st + l * PLANE + off) = kreg[l][c];
+        *reinterpret_cast<uint4*>(st + (NL + l) * PLANE + off) = vreg[l][c];
+      }
+    }
+    if (threadIdx.x == 0) seen[buf] = sreg;
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const unsigned long long ALL = TK == 64 ? ~0ull : 0xffffffffull;
+  if (ntiles > 0) { load_tile(kbeg); store_tile(0); }
+  __syncthreads();
+  for (int t = 0; t < ntiles; ++t) {
+    const int buf = t & 1, key0 = kbeg + t * TK;
+    if (t + 1 < ntiles) load_tile(key0 + TK);
+    char* st = sm + buf * STAGE;
+    const unsigned long long left = seen[buf];
+    if (left && q0 < p.L && !(p.causal && key0 > wlast)) {
+      f32x16 s[NU];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) s[u] = zero16();
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          uint4 kf[NL];
+#pragma unroll
+          for (int x = 0; x < NL; ++x) kf[x] = row_frag<DHP>(st + x * PLANE, u * 32, kk);
+          s[u] = mfma_levels<NL>(kf, qf[kk], s[u]);
+        }
+      const int e0 = key0 - (pos0 + q0) - p.map_lo;              // entry of the tile's first key and first query; the others: + key - query
+      if (e0 + TK - 1 <= 0 || e0 - 31 >= p.map_n - 1) {
+        const float c = e0 + TK - 1 <= 0 ? first_bias : last_bias;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], sc, c);
+      } else {
+        const float* lp = lut + TABLE_PAD + e0 - (lane & 31) + 4 * hh;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], sc, lp[u * 32 + crow(r)]);
+      }
+      if (left != ALL) {
+        const unsigned long long mine = left >> (4 * hh);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!((mine >> (u * 32 + crow(r))) & 1)) s[u][r] = -INFINITY;
+      }
+      if (p.causal && key0 + TK - 1 > pos0 + q0) {
+        const int d = key0 + 4 * hh - pos;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (d + u * 32 + crow(r) > 0) s[u][r] = -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+      top = other_max(top);
+      if (__ballot(top > m + 8.f)) {
+        const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn; l *= al;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= al;
+      }
+      const float mo = m == -INFINITY ? 0.f : m - PSH;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        float e[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { e[r] = __builtin_amdgcn_exp2f(s[u][r] - mo); l += e[r]; }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint4 pf[NL];
+          to_levels<NL>(e + 8 * g, pf);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            uint4 vf[NL];
+#pragma unroll
+            for (int x = 0; x < NL; ++x) vf[x] = col_frag<DHP>(st + (NL + x) * PLANE, u * 32 + g * 16, d);
+            o[d] = mfma_levels<NL>(vf, pf, o[d]);
+          }
+        }
+      }
+    }
+    if (t + 1 < ntiles) store_tile(buf ^ 1);
+    __syncthreads();
+  }
+  if (qi >= p.L) return;
+  l = other_sum(l);
+  const long long row = ((long long)b * p.H + h) * p.L + qi;
+  if (a.nparts > 1) {
+    float* O = a.part_o + (row * a.nparts + part) * p.dh;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = d * 32 + 8 * g + 4 * hh;
+        if (c < p.dh) *reinterpret_cast<float4*>(O + c) = make_float4(o[d][4 * g] * inv_v, o[d][4 * g + 1] * inv_v, o[d][4 * g + 2] * inv_v, o[d][4 * g + 3] * inv_v);
+      }
+    if (hh == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.nparts + part) * 2) = make_float2(m == -INFINITY ? m : m - PSH, l);
+    return;
+  }
+  const float il = l > 0.f ? inv_v / l : 0.f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = d * 32 + 8 * g + 4 * hh;
+      const float4 w = make_float4(o[d][4 * g] * il, o[d][4 * g + 1] * il, o[d][4 * g + 2] * il, o[d][4 * g + 3] * il);
+      if (c < p.dh) {
+        if constexpr (NL == 2) St<float>::st4((float*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);
+        else St<bf16_t>::st4((bf16_t*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);
+      }
+    }
+  if (p.lse && hh == 0) p.lse[row] = l > 0.f ? m - PSH + __log2f(l) : INFINITY;
+}
+
+// ---- a few queries per sample ---------------------------------------------------------------------------------------------------
+// A block takes a part of one (sample, kv head)'s keys for RT of its G * L query rows.  LPK lanes hold a key's row, EPL values each, and the same columns of the
+// RT queries and running outputs; every group of LPK lanes walks keys of its own, four a step, with a running maximum and sum of its own: the only
+// exchanges are the LPK-lane sums of the scores.  The groups are joined through LDS at the end, the parts by relpos_join_kernel.
+template <typename T, int EPL> struct Row;
+template <> struct Row<float, 4> {
+  static __device__ __forceinline__ void ld(const float* p, float (&f)[4]) { const float4 v = *reinterpret_cast<const float4*>(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+};
+template <> struct Row<bf16_t, 4> {
+  static __device__ __forceinline__ void ld(const bf16_t* p, float (&f)[4]) { const float4 v = St<bf16_t>::ld4(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+};
+template <> struct Row<bf16_t, 8> {
+  static __device__ __forceinline__ void ld(const bf16_t* p, float (&f)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), f); }
+};
+
+template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+// sum over the LPK neighbouring lanes, in all of them
+template <int LPK> __device__ __forceinline__ float lanes_sum(float x) {
+  if constexpr (LPK >= 2) x = dpp_add<0xB1>(x);                  // quad_perm 1 0 3 2
+  if constexpr (LPK >= 4) x = dpp_add<0x4E>(x);                  // quad_perm 2 3 0 1
+  if constexpr (LPK >= 8) x = dpp_add<0x141>(x);                 // row_half_mirror
+  if constexpr (LPK >= 16) x = dpp_add<0x140>(x);                // row_mirror
+  if constexpr (LPK >= 32) x += __shfl_xor(x, 16, 64);
+  return x;
+}
+
+template <typename T, int EPL, int LPK, int RT>
+__global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
+  constexpr int GPB = 256 / LPK, U = 4;                          // groups of a block
+  extern __shared__ __attribute__((aligned(16))) char sm[];
+  float* red = reinterpret_cast<float*>(sm);                     // [GPB][RT][2 + LPK * EPL]
+  const int sub = threadIdx.x % LPK, grp = threadIdx.x / LPK, c0 = sub * EPL;
+  const int rows = p.G * p.L, nr = (rows + RT - 1) / RT;
+  unsigned id = blockIdx.x;
+  const int rc = id % nr; id /= nr;
+  const int part = id % a.nparts; id /= a.nparts;
+  const int hk = id % p.Hkv, b = id / p.Hkv;
+  const int n = p.keys(b), pos0 = p.pos0(n);
+  const bool in = c0 < p.dh;
+  float q[RT][EPL], o[RT][EPL], m[RT], l[RT], fb[RT], lb[RT];
+  int pos[RT], hd[RT];
+  int pmax = -0x7fffffff, pmin = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = rc * RT + r, ok = row < rows, rr = ok ? row : 0;
+    const int i = rr % p.L;
+    hd[r] = hk * p.G + rr / p.L;
+    pos[r] = pos0 + i;
+    pmax = max(pmax, pos[r]); pmin = min(pmin, pos[r]);
+    m[r] = -INFINITY; l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) { q[r][e] = 0.f; o[r][e] = 0.f; }
+    if (in) Row<T, EPL>::ld((const T*)p.q + b * p.q_bs + (long long)i * p.ldq + hd[r] * p.dh + c0, q[r]);
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) q[r][e] *= p.scale * LOG2E;
+    fb[r] = p.table[(long long)p.map[0] * p.H + hd[r]] * LOG2E;
+    lb[r] = p.table[(long long)p.map[p.map_n - 1] * p.H + hd[r]] * LOG2E;
+  }
+  const int k0 = part * a.per, k1 = min(min(k0 + a.per, n), p.causal ? pmax + 1 : n);
+  const T* K = (const T*)p.k + b * p.k_bs + hk * p.dh + c0;
+  const T* V = (const T*)p.v + b * p.v_bs + hk * p.dh + c0;
+  for (int j0 = k0; j0 < k1; j0 += GPB * U) {
+    float kf[U][EPL], vf[U][EPL];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * GPB + grp;
+      ok[u] = j < k1 && !(p.mask && p.mask[(long long)b * p.S + j]);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) { kf[u][e] = 0.f; vf[u][e] = 0.f; }
+      if (ok[u] && in) {
+        Row<T, EPL>::ld(K + (long long)j * p.ldk, kf[u]);
+        Row<T, EPL>::ld(V + (long long)j * p.ldv, vf[u]);
+      }
+    }
+    // the step's keys all beyond one end of the map for all rows: the bias is one number a row
+    const bool far_lo = j0 + GPB * U - 1 - pmin - p.map_lo <= 0, far_hi = j0 - pmax - p.map_lo >= p.map_n - 1;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float s[U], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x = fmaf(q[r][e], kf[u][e], x);
+        x = lanes_sum<LPK>(x);
+        const int delta = j0 + u * GPB + grp - pos[r];
+        x += far_lo ? fb[r] : far_hi ? lb[r] : p.table[(long long)p.map[p.entry(delta)] * p.H + hd[r]] * LOG2E;
+        s[u] = ok[u] && !(p.causal && delta > 0) ? x : -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      const float mn = fmaxf(m[r], top);
+      if (mn == -INFINITY) continue;
+      const float al = __builtin_amdgcn_exp2f(m[r] - mn);
+      m[r] = mn; l[r] *= al;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[r][e] *= al;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = __builtin_amdgcn_exp2f(s[u] - mn);
+        l[r] += w;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(w, vf[u][e], o[r][e]);
+      }
+    }
+  }
+  // join the groups: first those of a wave, lane by lane, then the waves through LDS
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int x = LPK; x < 64; x <<= 1) {
+      const float m2 = __shfl_xor(m[r], x, 64), l2 = __shfl_xor(l[r], x, 64), mn = fmaxf(m[r], m2);
+      const float f1 = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - mn), f2 = mn == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mn);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[r][e] = o[r][e] * f1 + __shfl_xor(o[r][e], x, 64) * f2;
+      l[r] = l[r] * f1 + l2 * f2; m[r] = mn;
+    }
+  constexpr int W = LPK * EPL + 2;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (lane < LPK) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float* w = red + (wave * RT + r) * W;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) w[2 + c0 + e] = o[r][e];
+      if (sub == 0) { w[0] = m[r]; w[1] = l[r]; }
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < RT * p.dh; t += 256) {
+    const int r = t / p.dh, c = t - r * p.dh, row = rc * RT + r;
+    if (row >= rows) break;
+    float mm = -INFINITY, ll = 0.f, oo = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, red[(w * RT + r) * W]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(red[(w * RT + r) * W] - mm);
+      ll += f * red[(w * RT + r) * W + 1]; oo += f * red[(w * RT + r) * W + 2 + c];
+    }
+    const int h = hk * p.G + row / p.L, i = row % p.L;
+    const long long at = ((long long)b * p.H + h) * p.L + i;
+    if (a.nparts > 1) {
+      a.part_o[(at * a.nparts + part) * p.dh + c] = oo;
+      if (c == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.nparts + part) * 2) = make_float2(mm, ll);
+    } else {
+      St<T>::st((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, ll > 0.f ? oo / ll : 0.f);
+      if (p.lse && c == 0) p.lse[at] = ll > 0.f ? mm + __log2f(ll) : INFINITY;
+    }
+  }
+}
+
+// o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts; a thread four columns of a row
+template <typename T>
+__global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
+  const int q4 = p.dh >> 2;
+  const long long t = blockIdx.x * 256LL + threadIdx.x, row = t / q4;
+  if (row >= (long long)p.B * p.H * p.L) return;
+  const int c = (int)(t - row * q4) * 4;
+  const float* ml = a.part_ml + row * a.nparts * 2;
+  float m = -INFINITY;
+  for (int s = 0; s < a.nparts; ++s) m = fmaxf(m, ml[2 * s]);
+  float l = 0.f, x = 0.f, y = 0.f, z = 0.f, w = 0.f;
+  if (m != -INFINITY)
+    for (int s = 0; s < a.nparts; ++s) {
+      const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
+      if (f == 0.f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (row * a.nparts + s) * p.dh + c);
+      l += f * ml[2 * s + 1]; x += f * v.x; y += f * v.y; z += f * v.z; w += f * v.w;
+    }
+  const float il = l > 0.f ? 1.f / l : 0.f;
+  const int i = (int)(row % p.L), h = (int)(row / p.L % p.H);
+  const long long b = row / p.L / p.H;
+  St<T>::st4((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, make_float4(x * il, y * il, z * il, w * il));
+  if (p.lse && c == 0) p.lse[row] = l > 0.f ? m + __log2f(l) : INFINITY;
+}
+
+// ---- which kernel, in how many parts ---------------------------------------------------------------------------------------------
+struct Plan { bool token; int nparts, per; long long blocks; int rt; int64_t split_ws, part_ws; };
+
+Plan plan(const smx_relpos_desc* d, const RP& p) {
+  Plan w;
+  w.token = p.L <= 8;
+  w.split_ws = 0;
+  const int rows = p.G * p.L;
+  w.rt = rows >= 8 ? 8 : rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
+  const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
+  // parts until the chip's 256 CUs have two blocks each, a part no shorter than 256 keys
+  long long np = (512 + base - 1) / base, most = (p.S + 255) / 256;
+  if (base >= 256) np = 1;
+  if (np > most) np = most;
+  w.per = (int)(((p.S + np - 1) / np + 63) / 64 * 64);
+  w.nparts = (p.S + w.per - 1) / w.per;
+  w.blocks = base * w.nparts;
+  if (!w.token && !d->bf16) w.split_ws = split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh);
+  w.part_ws = w.nparts > 1 ? (int64_t)p.B * p.H * p.L * w.nparts * (p.dh + 4) * 4 : 0;
+  return w;
+}
+
+template <int DHP, int NL>
+int tile_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
+  constexpr int TK = DHP == 128 ? 32 : 64;
+  const int fixed = 2 * 2 * NL * TK * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
+  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
+  SMX_LAUNCH((relpos_tile_kernel<DHP, NL>), dim3((unsigned)w.blocks), dim3(256), lds, st, p, a);
+  return smx_launch_status();
+}
+
+template <typename T, int EPL, int LPK>
+int token_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
+  const int lds = 4 * w.rt * (LPK * EPL + 2) * 4;
+  const dim3 grid((unsigned)w.blocks), block(256);
+  if (w.rt == 8) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 8>), grid, block, lds, st, p, a);
+  else if (w.rt == 4) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 4>), grid, block, lds, st, p, a);
+  else if (w.rt == 2) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 2>), grid, block, lds, st, p, a);
+  else SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 1>), grid, block, lds, st, p, a);
+  return smx_launch_status();
+}
+
+template <typename T, int EPL>
+int token_width(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
+  if (p.dh <= 4 * EPL) return token_launch<T, EPL, 4>(p, a, w, st);
+  if (p.dh <= 8 * EPL) return token_launch<T, EPL, 8>(p, a, w, st);
+  if (p.dh <= 16 * EPL) return token_launch<T, EPL, 16>(p, a, w, st);
+  return token_launch<T, EPL, 32>(p, a, w, st);
+}
+
 }  // namespace
 
 extern "C" int64_t smx_attention_relpos_ws_bytes(const smx_relpos_desc* d) {
   RP p;
-  return check(d, p, false) == SMX_OK ? 0 : -1;
+  if (check(d, p, false) != SMX_OK) return -1;
+  const Plan w = plan(d, p);
+  return w.split_ws + w.part_ws;
 }
 
 extern "C" int smx_attention_relpos(const smx_relpos_desc* d, void* stream) {
   RP p;
-  const int rc = check(d, p, false);
+  int rc = check(d, p, false);
   if (rc != SMX_OK) return rc;
-  const long long blocks = ((long long)p.B * p.H * p.L + 3) / 4;
-  if (blocks > 0x7fffffffLL) return SMX_EINVAL;
-  if (d->bf16) SMX_LAUNCH(relpos_rows_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
-  else SMX_LAUNCH(relpos_rows_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
-  return smx_launch_status();
-}
-
-extern "C" int64_t smx_attention_relpos_bwd_ws_bytes(const smx_relpos_desc* d) {
-  RP p;
-  if (check(d, p, true) != SMX_OK) return -1;
-  return 4 * ((int64_t)p.B * p.H * p.L + (int64_t)p.H * p.map_n);
-}
-
-extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stream) {
-  RP p;
-  const int rc = check(d, p, true);
-  if (rc != SMX_OK) return rc;
-  const long long qb = ((long long)p.B * p.H * p.L + 3) / 4, kb = ((long long)p.B * p.Hkv * p.S + 3) / 4;
-  if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < smx_attention_relpos_bwd_ws_bytes(d) || qb > 0x7fffffffLL || kb > 0x7fffffffLL || p.H > 65535) return SMX_EINVAL;
-  float* dd = (float*)d->ws;
-  float* part = dd + (int64_t)p.B * p.H * p.L;
+  const Plan w = plan(d, p);
+  if (w.blocks > 0x7fffffffLL || (w.split_ws + w.part_ws && (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < w.split_ws + w.part_ws))) return SMX_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  SMX_LAUNCH(relpos_bwd_q_kernel, dim3((unsigned)qb), dim3(256), 0, st, p, dd);
-  SMX_LAUNCH(relpos_bwd_kv_kernel, dim3((unsigned)kb), dim3(256), 0, st, p, (const float*)dd);
-  SMX_LAUNCH(relpos_bwd_entry_kernel, dim3(p.map_n, p.H), dim3(256), 0, st, p, (const float*)dd, part);
-  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(smx_cdiv((long long)p.nb * p.H, 256)), dim3(256), 0, st, p, (const float*)part);
+  Src a{};
+  a.nparts = w.nparts; a.per = w.per;
+  char* ws = (char*)d->ws;
+  if (w.part_ws) {
+    a.part_o = (float*)(ws + w.split_ws);
+    a.part_ml = a.part_o + (int64_t)p.B * p.H * p.L * w.nparts * p.dh;
+  }
+  if (w.token) {
+    if (!d->bf16) rc = token_width<float, 4>(p, a, w, st);
+    else if (p.dh % 8 == 0 && (p.ldq | p.ldk | p.ldv) % 8 == 0 && (p.q_bs | p.k_bs | p.v_bs) % 8 == 0 && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16))
+      rc = token_width<bf16_t, 8>(p, a, w, st);
+    else rc = token_width<bf16_t, 4>(p, a, w, st);
+  } else {
+    if (!d->bf16) {
+      ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.L, p.dh, false);
+      ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, p.S, p.dh, true);
+      ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, p.S, p.dh, true);
+      const Split all[3] = {a.q, a.k, a.v};
+      rc = split_launch(p, all, 3, st);
+      if (rc != SMX_OK) return rc;
+    }
+    switch (dhp(p.dh)) {
+      case 32: rc = d->bf16 ? tile_launch<32, 1>(p, a, w, st) : tile_launch<32, 2>(p, a, w, st); break;
+      case 64: rc = d->bf16 ? tile_launch<64, 1>(p, a, w, st) : tile_launch<64, 2>(p, a, w, st); break;
+      default: rc = d->bf16 ? tile_launch<128, 1>(p, a, w, st) : tile_launch<128, 2>(p, a, w, st); break;
+    }
+  }
+  if (rc != SMX_OK || w.nparts == 1) return rc;
+  const long long nj = ((long long)p.B * p.H * p.L * (p.dh / 4) + 255) / 256;
+  if (nj > 0x7fffffffLL) return SMX_EINVAL;
+  if (d->bf16) SMX_LAUNCH(relpos_join_kernel<bf16_t>, dim3((unsigned)nj), dim3(256), 0, st, p, a);
+  else SMX_LAUNCH(relpos_join_kernel<float>, dim3((unsigned)nj), dim3(256), 0, st, p, a);
   return smx_launch_status();
 }

@@ -1325,7 +1325,7 @@ def _relpos_desc(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, 
                          f"{nhead} heads on {nkv}")
     B, Lq, E = q.shape
     S, dh = k.shape[1], E // nhead
-    if dh % 4 or not 4 <= dh <= 128 or E > 1 << 20 or B * nhead > 1 << 24 or max(Lq, S) > 1 << 30:
+    if dh % 4 or not 4 <= dh <= 128 or E > 1 << 20 or B * nhead > 1 << 24 or max(Lq, S) > 1 << 29:
         raise L.SmxError(f"attention_relpos: a head size of 4 to 128 in steps of four expected, got {dh} (B {B}, L {Lq}, S {S}, {nhead} heads)")
     d = L.RelposDesc(B=B, H=nhead, Hkv=nkv, L=Lq, S=S, dh=dh, map_lo=rp.lo, map_n=len(rp.map), num_buckets=rp.num_buckets, causal=int(bool(causal)),
                      bf16=int(q.dtype == BF16), scale=dh ** -0.5 if scale is None else scale)
