@@ -11,7 +11,7 @@ namespace relpos {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));        // (HIP's own uint4 is a struct: its copies kept staging registers in scratch memory)
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -20,13 +20,14 @@ constexpr int TABLE_PAD = 96;         // entries a 64-key x 32-query tile can re
 
 // ---- fp32 operands on the half-precision matrix pipe ("f16x3") ----------------------------------------------------------------
 // x = (h1 + h2) 2^-k with two IEEE halves: 22 significand bits; a product is h1 g1 + h1 g2 + h2 g1, the dropped h2 g2 is 2^-22 of it.  k is one number per
-// (sample, head) that brings the largest |x| to [2^14, 2^15): values down to 2^-16 of the largest keep all 22 bits, smaller ones are off by at most
+// (sample, kv head) that brings the largest |x| of the heads on it to [2^14, 2^15): values down to 2^-16 of the largest keep all 22 bits, smaller ones are off by at most
 // 2^-40 of the largest.  A first pass finds the largest values, a second writes the halves: planes [B][heads][rows rounded up to 64][DHP] of h1 and of h2,
 // rows that nobody may see and the columns from dh on as zeros.  That is read by every tile of the other side, so splitting here once costs less than
 // splitting in the kernels (a 128-query block would split every key of its head again).
 struct Split {
-  const float* src; long long bs; int ld, heads, rows, kv;      // kv: rows of keys (masks and lengths apply)
+  const float* src; long long bs; int ld, heads, group, rows, kv;  // group: heads of a kv head; kv: rows of keys (masks and lengths apply)
   _Float16* hi; _Float16* lo;                                   // planes
+  float* pow2;                                                  // [B][heads / group][2]: 2^k, 2^-k
   float* top;                                                   // [B][heads][nch] largest |x| of each chunk of CH rows
   const float* o;                                               // gradient rows: the output, for D_i = dO_i . o_i (dense, as src)
   float* dd;                                                    // [B][heads][rows rounded up to 64]
@@ -50,30 +51,21 @@ static inline int up64(int n) { return (n + 63) & ~63; }
 static inline int dhp(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : 128; }
 static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-// 2^k and 2^-k of a head from its chunks' largest values
-__device__ __forceinline__ float head_pow2(const float* top, int nch, float& inv) {
-  float m = 0.f;
-  for (int c = 0; c < nch; ++c) m = fmaxf(m, top[c]);
-  const int e = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;     // floor(log2 m); 2^(14 - e) stays a normal number
-  inv = __uint_as_float((unsigned)(e - 14 + 127) << 23);
-  return __uint_as_float((unsigned)(14 - e + 127) << 23);
-}
-
 // the launchers of relpos_attn.hip
 int check(const smx_relpos_desc* d, RP& p, bool bwd);
-int64_t split_bytes(int B, int heads, int rows, int dhp);       // planes + chunk maxima
-char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dhp, bool kv);
+int64_t split_bytes(int B, int heads, int rows, int dh);        // planes, scales, chunk maxima
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int group, int rows, int dh, bool kv);
 int split_launch(const RP& p, const Split* s, int n, hipStream_t st);
 
 // ---- matrix operands -----------------------------------------------------------------------------------------------------------
 template <int NL>
-__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (NL == 1) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 // c += a b over the levels, the smallest products first
 template <int NL>
-__device__ __forceinline__ f32x16 mfma_levels(const uint4 (&a)[NL], const uint4 (&b)[NL], f32x16 c) {
+__device__ __forceinline__ f32x16 mfma_levels(const u32x4 (&a)[NL], const u32x4 (&b)[NL], f32x16 c) {
   if constexpr (NL == 2) {
     c = mfma<2>(a[1], b[0], c);
     c = mfma<2>(a[0], b[1], c);
@@ -82,7 +74,7 @@ __device__ __forceinline__ f32x16 mfma_levels(const uint4 (&a)[NL], const uint4 
 }
 // eight fp32 -> the levels' fragments (bf16: one, rounded to nearest; halves: two)
 template <int NL>
-__device__ __forceinline__ void to_levels(const float* v, uint4 (&f)[NL]) {
+__device__ __forceinline__ void to_levels(const float* v, u32x4 (&f)[NL]) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -92,8 +84,8 @@ __device__ __forceinline__ void to_levels(const float* v, uint4 (&f)[NL]) {
       l[i] = cvt2_f16(v[2 * i] - f16lo(h[i]), v[2 * i + 1] - f16hi(h[i]));
     }
   }
-  f[0] = make_uint4(h[0], h[1], h[2], h[3]);
-  if constexpr (NL == 2) f[1] = make_uint4(l[0], l[1], l[2], l[3]);
+  f[0] = u32x4{h[0], h[1], h[2], h[3]};
+  if constexpr (NL == 2) f[1] = u32x4{l[0], l[1], l[2], l[3]};
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -112,18 +104,18 @@ template <int DHP> constexpr int ROWB = DHP * 2 + 16;
 
 // operand fragment of 16 columns kk of the tile's row r0 + (lane & 31)
 template <int DHP>
-__device__ __forceinline__ uint4 row_frag(const char* tile, int r0, int kk) {
+__device__ __forceinline__ u32x4 row_frag(const char* tile, int r0, int kk) {
   const int lane = threadIdx.x & 63;
-  return *reinterpret_cast<const uint4*>(tile + (r0 + (lane & 31)) * ROWB<DHP> + kk * 32 + (lane >> 5) * 16);
+  return *reinterpret_cast<const u32x4*>(tile + (r0 + (lane & 31)) * ROWB<DHP> + kk * 32 + (lane >> 5) * 16);
 }
 // the transposed fragment: lane holds column 32 dt + (lane & 31) at the 16 rows from r0 on that an accumulator's eight registers hold
 // (4 hh + 0..3 and 8 + 4 hh + 0..3): two transposing reads of 4 rows x 16 columns a lane group
 template <int DHP>
-__device__ __forceinline__ uint4 col_frag(char* tile, int r0, int dt) {
+__device__ __forceinline__ u32x4 col_frag(char* tile, int r0, int dt) {
   const int lane = threadIdx.x & 63, l = lane & 15;
   char* at = tile + (r0 + (lane >> 5) * 4 + (l >> 2)) * ROWB<DHP> + dt * 64 + ((lane >> 4) & 1) * 32 + (l & 3) * 8;
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * ROWB<DHP>));
-  return __builtin_bit_cast(uint4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // the other 32 lanes' value

@@ -44,13 +44,24 @@ __global__ __launch_bounds__(256) void relpos_top_kernel(RP p, Splits a) {
 // 64 rows of one head -> both planes; gradient rows: D_i = dO_i . o_i too
 template <int DHP>
 __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
+  __shared__ float red[4];
   int t = 0, id = blockIdx.x;
   while (id >= a.end[t]) ++t;
   const Split& s = a.s[t];
   id -= t ? a.end[t - 1] : 0;
   const int nch = (s.rows + CH - 1) / CH, nt = (s.rows + 63) / 64, c = id % nt, h = id / nt % s.heads, b = id / nt / s.heads;
-  float inv;
-  const float sc = head_pow2(s.top + ((long long)b * s.heads + h) * nch, nch, inv);
+  const float* top = s.top + ((long long)b * s.heads + h / s.group * s.group) * nch;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < s.group * nch; i += 256) m = fmaxf(m, top[i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;    // floor(log2 m); 2^(14 - ex) stays a normal number
+  const float sc = __uint_as_float((unsigned)(14 - ex + 127) << 23);
+  if (threadIdx.x == 0 && c == 0 && h % s.group == 0)
+    *reinterpret_cast<float2*>(s.pow2 + ((long long)b * (s.heads / s.group) + h / s.group) * 2) = make_float2(sc, __uint_as_float((unsigned)(ex - 14 + 127) << 23));
   constexpr int Q4 = DHP / 4;
   const long long out = (((long long)b * s.heads + h) * nt + c) * 64 * DHP;
 #pragma unroll
@@ -76,13 +87,13 @@ __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
 }
 
 int64_t split_bytes(int B, int heads, int rows, int dh) {
-  return (int64_t)B * heads * ((int64_t)up64(rows) * dhp(dh) * 4 + (((rows + CH - 1) / CH + 3) / 4 * 16));
+  return (int64_t)B * heads * ((int64_t)up64(rows) * dhp(dh) * 4 + 16 + ((rows + CH - 1) / CH + 3) / 4 * 16);
 }
 
-char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dh, bool kv) {
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int group, int rows, int dh, bool kv) {
   const int64_t plane = (int64_t)B * heads * up64(rows) * dhp(dh);
-  s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.rows = rows; s.kv = kv;
-  s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.top = (float*)(s.lo + plane);
+  s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.group = group; s.rows = rows; s.kv = kv;
+  s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.pow2 = (float*)(s.lo + plane); s.top = s.pow2 + 4 * (int64_t)B * heads;
   s.o = nullptr; s.dd = nullptr;
   return ws + split_bytes(B, heads, rows, dh);
 }
@@ -173,20 +184,17 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   fill_bias(lut, p, h);
   const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
   float sc = p.scale * LOG2E, inv_v = 1.f;
-  uint4 qf[KS][NL];
+  u32x4 qf[KS][NL];
   if constexpr (NL == 2) {
-    float iq, ik;
-    const int cq = (p.L + CH - 1) / CH, ck = (p.S + CH - 1) / CH;
-    head_pow2(a.q.top + ((long long)b * p.H + h) * cq, cq, iq);
-    head_pow2(a.k.top + ((long long)b * p.Hkv + hk) * ck, ck, ik);
-    head_pow2(a.v.top + ((long long)b * p.Hkv + hk) * ck, ck, inv_v);
-    sc = sc * iq * ik;
+    const int at2 = (b * p.Hkv + hk) * 2 + 1;
+    sc = sc * a.q.pow2[at2] * a.k.pow2[at2];
+    inv_v = a.v.pow2[at2];
     const int up = (p.L + 63) & ~63;
     const long long at = (((long long)b * p.H + h) * up + qi) * DHP + hh * 8;
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
-      qf[kk][0] = qi < up ? *reinterpret_cast<const uint4*>(a.q.hi + at + kk * 16) : make_uint4(0, 0, 0, 0);
-      qf[kk][1] = qi < up ? *reinterpret_cast<const uint4*>(a.q.lo + at + kk * 16) : make_uint4(0, 0, 0, 0);
+      qf[kk][0] = qi < up ? *reinterpret_cast<const u32x4*>(a.q.hi + at + kk * 16) : u32x4{0, 0, 0, 0};
+      qf[kk][1] = qi < up ? *reinterpret_cast<const u32x4*>(a.q.lo + at + kk * 16) : u32x4{0, 0, 0, 0};
     }
   } else {
     const bf16_t* Q = (const bf16_t*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh;
@@ -196,11 +204,11 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
       uint2 x = make_uint2(0, 0), y = make_uint2(0, 0);
       if (qi < p.L && d < p.dh) x = *reinterpret_cast<const uint2*>(Q + d);
       if (qi < p.L && d + 4 < p.dh) y = *reinterpret_cast<const uint2*>(Q + d + 4);
-      qf[kk][0] = make_uint4(x.x, x.y, y.x, y.y);
+      qf[kk][0] = u32x4{x.x, x.y, y.x, y.y};
     }
   }
 
-  uint4 kreg[NL][NCH], vreg[NL][NCH];
+  u32x4 kreg[NL][NCH], vreg[NL][NCH];
   unsigned long long sreg = 0;
   auto load_tile = [&](int key0) {
     if constexpr (NL == 2) {
@@ -208,8 +216,8 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int e = (c * 256 + threadIdx.x) * 8;
-        kreg[0][c] = *reinterpret_cast<const uint4*>(a.k.hi + at + e); kreg[1][c] = *reinterpret_cast<const uint4*>(a.k.lo + at + e);
-        vreg[0][c] = *reinterpret_cast<const uint4*>(a.v.hi + at + e); vreg[1][c] = *reinterpret_cast<const uint4*>(a.v.lo + at + e);
+        kreg[0][c] = *reinterpret_cast<const u32x4*>(a.k.hi + at + e); kreg[1][c] = *reinterpret_cast<const u32x4*>(a.k.lo + at + e);
+        vreg[0][c] = *reinterpret_cast<const u32x4*>(a.v.hi + at + e); vreg[1][c] = *reinterpret_cast<const u32x4*>(a.v.lo + at + e);
       }
     } else {
 #pragma unroll
@@ -222,8 +230,8 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
           if (d < p.dh) { x = *reinterpret_cast<const uint2*>(K); z = *reinterpret_cast<const uint2*>(V); }
           if (d + 4 < p.dh) { y = *reinterpret_cast<const uint2*>(K + 4); w = *reinterpret_cast<const uint2*>(V + 4); }
         }
-        kreg[0][c] = make_uint4(x.x, x.y, y.x, y.y);
-        vreg[0][c] = make_uint4(z.x, z.y, w.x, w.y);
+        kreg[0][c] = u32x4{x.x, x.y, y.x, y.y};
+        vreg[0][c] = u32x4{z.x, z.y, w.x, w.y};
       }
     }
     if (wave == 0) {
@@ -238,8 +246,8 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
       const int e = c * 256 + threadIdx.x, off = e / CPR * RB + e % CPR * 16;
 #pragma unroll
       for (int l = 0; l < NL; ++l) {
-        *reinterpret_cast<uint4*>(st + l * PLANE + off) = kreg[l][c];
-        *reinterpret_cast<uint4*>(st + (NL + l) * PLANE + off) = vreg[l][c];
+        *reinterpret_cast<u32x4*>(st + l * PLANE + off) = kreg[l][c];
+        *reinterpret_cast<u32x4*>(st + (NL + l) * PLANE + off) = vreg[l][c];
       }
     }
     if (threadIdx.x == 0) seen[buf] = sreg;
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
       for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-          uint4 kf[NL];
+          u32x4 kf[NL];
 #pragma unroll
           for (int x = 0; x < NL; ++x) kf[x] = row_frag<DHP>(st + x * PLANE, u * 32, kk);
           s[u] = mfma_levels<NL>(kf, qf[kk], s[u]);
@@ -322,11 +330,11 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
         for (int r = 0; r < 16; ++r) { e[r] = __builtin_amdgcn_exp2f(s[u][r] - mo); l += e[r]; }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          uint4 pf[NL];
+          u32x4 pf[NL];
           to_levels<NL>(e + 8 * g, pf);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            uint4 vf[NL];
+            u32x4 vf[NL];
 #pragma unroll
             for (int x = 0; x < NL; ++x) vf[x] = col_frag<DHP>(st + (NL + x) * PLANE, u * 32 + g * 16, d);
             o[d] = mfma_levels<NL>(vf, pf, o[d]);
@@ -626,9 +634,9 @@ extern "C" int smx_attention_relpos(const smx_relpos_desc* d, void* stream) {
     else rc = token_width<bf16_t, 4>(p, a, w, st);
   } else {
     if (!d->bf16) {
-      ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.L, p.dh, false);
-      ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, p.S, p.dh, true);
-      ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, p.S, p.dh, true);
+      ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.G, p.L, p.dh, false);
+      ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, 1, p.S, p.dh, true);
+      ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, 1, p.S, p.dh, true);
       const Split all[3] = {a.q, a.k, a.v};
       rc = split_launch(p, all, 3, st);
       if (rc != SMX_OK) return rc;
