@@ -25,7 +25,7 @@ constexpr int TABLE_PAD = 96;         // entries a 64-key x 32-query tile can re
 // rows that nobody may see and the columns from dh on as zeros.  That is read by every tile of the other side, so splitting here once costs less than
 // splitting in the kernels (a 128-query block would split every key of its head again).
 struct Split {
-  const float* src; long long bs; int ld, heads, group, rows, kv;  // group: heads of a kv head; kv: rows of keys (masks and lengths apply)
+  const float* src; long long bs; int ld, heads, group, rows, kv, flip;  // group: heads of a kv head; kv: rows of keys (masks and lengths apply); flip: odd rows negated
   _Float16* hi; _Float16* lo;                                   // planes
   float* pow2;                                                  // [B][heads / group][2]: 2^k, 2^-k
   float* top;                                                   // [B][heads][nch] largest |x| of each chunk of CH rows

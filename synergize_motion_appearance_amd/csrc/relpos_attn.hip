@@ -78,7 +78,8 @@ __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
       for (int o = 1; o < Q4; o <<= 1) D += __shfl_xor(D, o, 64);
       if (d == 0) s.dd[((long long)b * s.heads + h) * nt * 64 + row] = D;
     }
-    x.x *= sc; x.y *= sc; x.z *= sc; x.w *= sc;
+    const float w = s.flip && (r & 1) ? -sc : sc;
+    x.x *= w; x.y *= w; x.z *= w; x.w *= w;
     const uint2 h2 = make_uint2(cvt2_f16(x.x, x.y), cvt2_f16(x.z, x.w));
     const uint2 l2 = make_uint2(cvt2_f16(x.x - f16lo(h2.x), x.y - f16hi(h2.x)), cvt2_f16(x.z - f16lo(h2.y), x.w - f16hi(h2.y)));
     *reinterpret_cast<uint2*>(s.hi + out + i * 4) = h2;
@@ -94,7 +95,7 @@ char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, in
   const int64_t plane = (int64_t)B * heads * up64(rows) * dhp(dh);
   s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.group = group; s.rows = rows; s.kv = kv;
   s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.pow2 = (float*)(s.lo + plane); s.top = s.pow2 + 4 * (int64_t)B * heads;
-  s.o = nullptr; s.dd = nullptr;
+  s.o = nullptr; s.dd = nullptr; s.flip = 0;
   return ws + split_bytes(B, heads, rows, dh);
 }
 

@@ -4,6 +4,9 @@
 // P is computed again from q, k and the rows' lse (log2 units; +inf for a row with no key left, so that 2^{s - lse} is 0 there).  All products in the
 // f16x3 arithmetic of relpos.h.  Two passes over the pairs, one that owns queries (dq, dtable) and one that owns keys (dk, dv): seven products
 // instead of five, but no sum crosses blocks, so that nothing is atomic and results repeat bit for bit.
+// The matrix cores cut the bits below an accumulator's last towards -inf (some 0.1 of its last bit on average): dP as a whole is a little low, D is not,
+// and a bucket's sum over millions of pairs of mixed signs shows it (dtable off by 3e-6 to 5e-6 of its norm at 1024 x 1024).  V's odd rows enter with
+// the opposite sign, so that the cuts of neighbouring keys cancel in every such sum.
 #include "relpos.h"
 
 namespace {
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
       }
       float ds[16], top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * (dp[r] - D); top = fmaxf(top, fabsf(ds[r])); }
+      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * ((r & 1 ? -dp[r] : dp[r]) - D); top = fmaxf(top, fabsf(ds[r])); }
       if (lo || hi) {
         float sum = 0.f;
 #pragma unroll
@@ -261,6 +264,7 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = zero16();
   float f = F0;
+  const float sign = key & 1 ? -1.f : 1.f;                       // V's odd rows are negated
   // causal: the first query that stands at this block's first key or behind it
   const int t0 = p.causal ? max(0, kb * 128 - pos0) / TQ : 0, t1 = kb * 128 < n ? (p.L + TQ - 1) / TQ : 0;
   const int per = max(0, t1 - t0), ntiles = per * p.G;
@@ -319,7 +323,7 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(
       }
       float ds[16], top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * (dp[r] - dd[r]); top = fmaxf(top, fabsf(ds[r])); }
+      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * fmaf(dp[r], sign, -dd[r]); top = fmaxf(top, fabsf(ds[r])); }
       follow(top, f, dk);
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] *= f;
@@ -413,6 +417,7 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
   ws = split_setup(a.g, ws, p.d_o, (long long)p.L * p.H * p.dh, p.H * p.dh, p.B, p.H, p.G, p.L, p.dh, false);
   ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, 1, p.S, p.dh, true);
   ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, 1, p.S, p.dh, true);
+  a.v.flip = 1;
   a.part = (float*)ws;
   a.g.o = (const float*)p.o;
   a.g.dd = (float*)(ws + part_bytes(p));
