@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <math.h>
+#include <initializer_list>
 #include "smx.h"
 #include "smx_common.h"
 #include "bf16.h"
@@ -17,162 +18,337 @@ struct NRP {
   const void* x; const void* h; void* xo; void* y;
   const float* pg; const float* pb; const float* ng; const float* nb; const float* gate;
   const float* gx; const float* gy; float* dx; float* dh; float* part;
-  long long T, per; int E, rms, nblk, rows;      // per: tokens of a gate row; nblk blocks of `rows` tokens walk each gate row's tokens
+  long long T, per; int E, rms, nblk, rows, want; // want: which parameter sums; per: tokens of a gate row; nblk blocks of `rows` tokens walk each gate row's tokens
   float rs, eps;
 };
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
+// LPR lanes hold a row: lane `sub` the V columns of chunks sub, sub + LPR, ... (N of them); a block of BT threads BT / LPR rows at a time.  V is 16 bytes
+// of the storage type, 1 where rows do not start on 16 bytes.
+template <int LPR>
+struct Lanes {
+  static constexpr int BT = LPR > 256 ? LPR : 256, RPB = BT / LPR, W = LPR / 64;
+  int sub, row, turn = 0;
+  float2* red;                                                    // [2][W], rows of more than a wave
+  __device__ __forceinline__ Lanes(float2* r) : sub(threadIdx.x % LPR), row(threadIdx.x / LPR), red(r) {}
+  // a row's sums of x and y, in all its lanes.  The two halves of `red` take turns: one barrier a sum
+  __device__ __forceinline__ void sum(float& x, float& y) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
-}
-
-// mean and 1 / sqrt(var + eps) of a row held as v[k] at columns threadIdx.x + 256 k
-template <int N>
-__device__ __forceinline__ void row_stats(const float (&v)[N], int E, int rms, float eps, float* red, float& mean, float& r) {
-  float s = 0.f;
-  mean = 0.f;
-  if (!rms) {
+    for (int o = LPR < 64 ? LPR / 2 : 32; o > 0; o >>= 1) { x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); }
+    if constexpr (LPR > 64) {
+      float2* r = red + turn * W;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = make_float2(x, y);
+      __syncthreads();
+      x = y = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s += v[k];
-    mean = block_sum(s, red) / E;
-  }
-  float q = 0.f;
-#pragma unroll
-  for (int k = 0; k < N; ++k) { const float d = (int)threadIdx.x + 256 * k < E ? v[k] - mean : 0.f; q += d * d; }
-  r = 1.f / sqrtf(block_sum(q, red) / E + eps);
-}
-
-template <typename TS, int N>
-__global__ __launch_bounds__(256) void norm_residual_kernel(NRP p) {
-  __shared__ float red[4];
-  const long long t = blockIdx.x, at = t * p.E;
-  const float* gate = p.gate ? p.gate + t / p.per * p.E : nullptr;
-  float v[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) { const int c = threadIdx.x + 256 * k; v[k] = c < p.E ? St<TS>::ld((const TS*)p.h + at + c) : 0.f; }
-  float mean, r;
-  if (p.pg) {
-    row_stats<N>(v, p.E, p.rms, p.eps, red, mean, r);
-#pragma unroll
-    for (int k = 0; k < N; ++k) { const int c = threadIdx.x + 256 * k; if (c < p.E) v[k] = (v[k] - mean) * r * p.pg[c] + (p.pb ? p.pb[c] : 0.f); }
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int c = threadIdx.x + 256 * k;
-    if (c < p.E) {
-      TS w;
-      St<TS>::st(&w, p.rs * St<TS>::ld((const TS*)p.x + at + c) + (gate ? gate[c] : 1.f) * v[k]);
-      ((TS*)p.xo)[at + c] = w;
-      v[k] = St<TS>::ld(&w);                       // y is the norm of what is stored
+      for (int w = 0; w < W; ++w) { x += r[w].x; y += r[w].y; }
     }
   }
-  if (!p.y) return;
-  row_stats<N>(v, p.E, p.rms, p.eps, red, mean, r);
+};
+
+template <typename TS, int V> __device__ __forceinline__ void ldv(const TS* p, float* f) {
+  if constexpr (V == 8) { float g[8]; unpack8(*reinterpret_cast<const uint4*>(p), g);
 #pragma unroll
-  for (int k = 0; k < N; ++k) { const int c = threadIdx.x + 256 * k; if (c < p.E) St<TS>::st((TS*)p.y + at + c, (v[k] - mean) * r * p.ng[c] + (p.nb ? p.nb[c] : 0.f)); }
+    for (int e = 0; e < 8; ++e) f[e] = g[e]; }
+  else if constexpr (V == 4) { const float4 v = St<TS>::ld4(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  else f[0] = St<TS>::ld(p);
+}
+template <typename TS, int V> __device__ __forceinline__ void stv(TS* p, const float* f) {
+  if constexpr (V == 8) { const float g[8] = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}; *reinterpret_cast<uint4*>(p) = pack8(g); }
+  else if constexpr (V == 4) St<TS>::st4(p, make_float4(f[0], f[1], f[2], f[3]));
+  else St<TS>::st(p, f[0]);
+}
+// V fp32 parameters, `other` without them
+template <int V> __device__ __forceinline__ void ldp(const float* p, int c, float other, float* f) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = other;
+  } else if constexpr (V == 8) { ldv<float, 4>(p + c, f); ldv<float, 4>(p + c + 4, f + 4); }
+  else ldv<float, V>(p + c, f);
 }
 
-// a block walks `rows` tokens of one gate row, keeping its columns' parameter sums in registers; part [groups][nblk][5][E]:
-// dpre gamma, dpre beta, dpost gamma, dpost beta, dgate
-template <int N>
-__global__ __launch_bounds__(256) void norm_residual_bwd_kernel(NRP p) {
-  __shared__ float red[4];
+// mean and 1 / sqrt(var + eps) of two rows at a time (b unused: pass zeros): the sums first, then the squares of the deviations -- never a difference of
+// squares
+template <int NV, int LPR>
+__device__ __forceinline__ void stats2(Lanes<LPR>& ln, const float (&a)[NV], const float (&b)[NV], const bool (&in)[NV], int E, int rms, float eps, float& ma, float& ra,
+                                       float& mb, float& rb) {
+  const float iE = 1.f / E;
+  ma = mb = 0.f;
+  if (!rms) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) { ma += a[k]; mb += b[k]; }
+    ln.sum(ma, mb);
+    ma *= iE; mb *= iE;
+  }
+  float qa = 0.f, qb = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) { const float x = in[k] ? a[k] - ma : 0.f, y = in[k] ? b[k] - mb : 0.f; qa = fmaf(x, x, qa); qb = fmaf(y, y, qb); }
+  ln.sum(qa, qb);
+  ra = 1.f / sqrtf(qa * iE + eps); rb = 1.f / sqrtf(qb * iE + eps);
+}
+
+// Forward: x and h are read once, x' and y written once; a row stays in its lanes' registers between the two norms.  With up to 8 columns a lane
+// the parameters stay there too (five rows of fp32 against four of data: read again for every row they would be most of a CU's loads).
+template <typename TS, int V, int LPR, int N>
+__global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
+  constexpr int NV = N * V;
+  constexpr bool HOLD = NV <= 8;
+  __shared__ float2 red[2 * (LPR > 64 ? LPR / 64 : 1)];
+  Lanes<LPR> ln(red);
+  float pg[HOLD ? NV : 1], pb[HOLD ? NV : 1], ng[HOLD ? NV : 1], nb[HOLD ? NV : 1], gt[HOLD ? NV : 1];
+  bool in[NV];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int c = (ln.sub + LPR * k) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) in[k * V + e] = c < p.E;
+    if constexpr (HOLD)
+      if (c < p.E) { ldp<V>(p.pg, c, 1.f, pg + k * V); ldp<V>(p.pb, c, 0.f, pb + k * V); ldp<V>(p.ng, c, 1.f, ng + k * V); ldp<V>(p.nb, c, 0.f, nb + k * V);
+                     ldp<V>(p.per == p.T ? p.gate : nullptr, c, 1.f, gt + k * V); }
+  }
+  const bool same_gate = HOLD && p.per == p.T;
+  for (long long t = blockIdx.x * (long long)Lanes<LPR>::RPB + ln.row; t < p.T; t += (long long)gridDim.x * Lanes<LPR>::RPB) {
+    const long long at = t * p.E;
+    const float* gate = p.gate ? p.gate + (p.per == p.T ? 0 : t / p.per * p.E) : nullptr;
+    float x[NV], v[NV], zero[NV];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int c = (ln.sub + LPR * k) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[k * V + e] = v[k * V + e] = zero[k * V + e] = 0.f;
+      if (c < p.E) { ldv<TS, V>((const TS*)p.x + at + c, x + k * V); ldv<TS, V>((const TS*)p.h + at + c, v + k * V); }
+    }
+    float mean = 0.f, r = 1.f, m2, r2;
+    if (p.pg) stats2<NV, LPR>(ln, v, zero, in, p.E, p.rms, p.eps, mean, r, m2, r2);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int c = (ln.sub + LPR * k) * V;
+      if (c < p.E) {
+        float a[V], b[V], g[V];
+        if constexpr (HOLD) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) { a[e] = pg[k * V + e]; b[e] = pb[k * V + e]; g[e] = gt[k * V + e]; }
+        } else { ldp<V>(p.pg, c, 1.f, a); ldp<V>(p.pb, c, 0.f, b); }
+        if (!same_gate) ldp<V>(gate, c, 1.f, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float n = fmaf((v[k * V + e] - mean) * r, a[e], b[e]);
+          TS w;
+          St<TS>::st(&w, fmaf(g[e], n, p.rs * x[k * V + e]));
+          v[k * V + e] = St<TS>::ld(&w);             // y is the norm of what is stored
+        }
+        stv<TS, V>((TS*)p.xo + at + c, v + k * V);
+      }
+    }
+    if (!p.y) continue;
+    stats2<NV, LPR>(ln, v, zero, in, p.E, p.rms, p.eps, mean, r, m2, r2);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int c = (ln.sub + LPR * k) * V;
+      if (c < p.E) {
+        float a[V], b[V];
+        if constexpr (HOLD) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) { a[e] = ng[k * V + e]; b[e] = nb[k * V + e]; }
+        } else { ldp<V>(p.ng, c, 1.f, a); ldp<V>(p.nb, c, 0.f, b); }
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k * V + e] = fmaf((v[k * V + e] - mean) * r, a[e], b[e]);
+        stv<TS, V>((TS*)p.y + at + c, v + k * V);
+      }
+    }
+  }
+}
+
+// Backward: a block walks `rows` tokens of one gate row, each thread keeping its columns' five parameter sums in registers; the block's sums go to
+// part [groups * nblk][5][E] (dpre gamma, dpre beta, dpost gamma, dpost beta, dgate; those that are wanted), norm_residual_sum_kernel adds the blocks.
+template <int V, int LPR, int N>
+__global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p) {
+  constexpr int NV = N * V, BT = Lanes<LPR>::BT, RPB = Lanes<LPR>::RPB;
+  __shared__ float2 red[2 * (LPR > 64 ? LPR / 64 : 1)];
+  __shared__ float join[LPR > 64 ? 1 : 4 * LPR * NV];
+  Lanes<LPR> ln(red);
   const long long g = blockIdx.x / p.nblk, blk = blockIdx.x - g * p.nblk;
   const float* gate = p.gate ? p.gate + g * p.E : nullptr;
-  float a[5][N];
+  float a[5][NV];
+  bool in[NV];
 #pragma unroll
   for (int i = 0; i < 5; ++i)
 #pragma unroll
-    for (int k = 0; k < N; ++k) a[i][k] = 0.f;
-  const long long t1 = g * p.per + min(p.per, (blk + 1) * (long long)p.rows);
-  for (long long t = g * p.per + blk * p.rows; t < t1; ++t) {
-    const long long at = t * p.E;
-    float v[N], c[N];
-    float mean = 0.f, r = 1.f;
+    for (int k = 0; k < NV; ++k) a[i][k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; c[k] = e < p.E && p.gx ? p.gx[at + e] : 0.f; }
+  for (int k = 0; k < NV; ++k) in[k] = (ln.sub + LPR * (k / V)) * V < p.E;
+  const long long t1 = g * p.per + min(p.per, (blk + 1) * (long long)p.rows);
+  const float iE = 1.f / p.E;
+  for (long long t = g * p.per + blk * p.rows + ln.row; t < t1; t += RPB) {
+    const long long at = t * p.E;
+    float x[NV], h[NV], c[NV], gy[NV];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int col = (ln.sub + LPR * k) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[k * V + e] = h[k * V + e] = c[k * V + e] = gy[k * V + e] = 0.f;
+      if (col < p.E) {
+        ldv<float, V>((const float*)p.h + at + col, h + k * V);
+        if (p.gx) ldv<float, V>(p.gx + at + col, c + k * V);
+        if (p.gy) { ldv<float, V>((const float*)p.xo + at + col, x + k * V); ldv<float, V>(p.gy + at + col, gy + k * V); }
+      }
+    }
+    float mx, rx, mh, rh, s1 = 0.f, s2 = 0.f;
+    stats2<NV, LPR>(ln, x, h, in, p.E, p.rms, p.eps, mx, rx, mh, rh);
     if (p.gy) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; v[k] = e < p.E ? ((const float*)p.xo)[at + e] : 0.f; }
-      row_stats<N>(v, p.E, p.rms, p.eps, red, mean, r);
-      float s1 = 0.f, s2 = 0.f;
-#pragma unroll
       for (int k = 0; k < N; ++k) {
-        const int e = threadIdx.x + 256 * k;
-        if (e < p.E) {
-          const float gy = p.gy[at + e], hat = (v[k] - mean) * r, gw = gy * p.ng[e];
-          a[0][k] += gy * hat; a[1][k] += gy;
-          s1 += gw; s2 += gw * hat;
+        const int col = (ln.sub + LPR * k) * V;
+        float w[V];
+        if (col < p.E) {
+          ldp<V>(p.ng, col, 1.f, w);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int i = k * V + e;
+            const float hat = (x[i] - mx) * rx;
+            a[0][i] = fmaf(gy[i], hat, a[0][i]); a[1][i] += gy[i];
+            gy[i] *= w[e]; x[i] = hat;
+            s1 += gy[i]; s2 = fmaf(gy[i], hat, s2);
+          }
         }
       }
-      s1 = p.rms ? 0.f : block_sum(s1, red) / p.E;
-      s2 = block_sum(s2, red) / p.E;
+      ln.sum(s1, s2);
+      s1 = p.rms ? 0.f : s1 * iE; s2 *= iE;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int e = threadIdx.x + 256 * k;
-        if (e < p.E) c[k] += r * (p.gy[at + e] * p.ng[e] - s1 - (v[k] - mean) * r * s2);
-      }
+      for (int k = 0; k < NV; ++k) if (in[k]) c[k] = fmaf(rx, gy[k] - s1 - x[k] * s2, c[k]);
     }
     if (p.dx) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; if (e < p.E) p.dx[at + e] = p.rs * c[k]; }
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; v[k] = e < p.E ? ((const float*)p.h)[at + e] : 0.f; }
-    if (!p.pg) {
-#pragma unroll
       for (int k = 0; k < N; ++k) {
-        const int e = threadIdx.x + 256 * k;
-        if (e < p.E) { a[4][k] += v[k] * c[k]; if (p.dh) p.dh[at + e] = (gate ? gate[e] : 1.f) * c[k]; }
+        const int col = (ln.sub + LPR * k) * V;
+        float w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = p.rs * c[k * V + e];
+        if (col < p.E) stv<float, V>(p.dx + at + col, w);
       }
-      continue;
     }
-    row_stats<N>(v, p.E, p.rms, p.eps, red, mean, r);
-    float s1 = 0.f, s2 = 0.f;
+    s1 = s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int e = threadIdx.x + 256 * k;
-      if (e < p.E) {
-        const float hat = (v[k] - mean) * r, dn = (gate ? gate[e] : 1.f) * c[k], gw = dn * p.pg[e];
-        a[4][k] += c[k] * (hat * p.pg[e] + (p.pb ? p.pb[e] : 0.f));
-        a[2][k] += dn * hat; a[3][k] += dn;
-        s1 += gw; s2 += gw * hat;
-        c[k] = gw; v[k] = hat;
+      const int col = (ln.sub + LPR * k) * V;
+      float w[V], b[V], gt[V];
+      if (col < p.E) {
+        ldp<V>(p.pg, col, 1.f, w); ldp<V>(p.pb, col, 0.f, b); ldp<V>(gate, col, 1.f, gt);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int i = k * V + e;
+          if (!p.pg) { a[4][i] = fmaf(c[i], h[i], a[4][i]); c[i] *= gt[e]; continue; }
+          const float hat = (h[i] - mh) * rh, dn = gt[e] * c[i];
+          a[4][i] = fmaf(c[i], fmaf(hat, w[e], b[e]), a[4][i]);
+          a[2][i] = fmaf(dn, hat, a[2][i]); a[3][i] += dn;
+          c[i] = dn * w[e]; h[i] = hat;
+          s1 += c[i]; s2 = fmaf(c[i], hat, s2);
+        }
       }
     }
-    s1 = p.rms ? 0.f : block_sum(s1, red) / p.E;
-    s2 = block_sum(s2, red) / p.E;
+    if (p.pg) {
+      ln.sum(s1, s2);
+      s1 = p.rms ? 0.f : s1 * iE; s2 *= iE;
 #pragma unroll
-    for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; if (e < p.E && p.dh) p.dh[at + e] = r * (c[k] - s1 - v[k] * s2); }
+      for (int k = 0; k < NV; ++k) c[k] = rh * (c[k] - s1 - h[k] * s2);
+    }
+    if (p.dh) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V>(p.dh + at + col, c + k * V); }
+    }
   }
+  float* part = p.part + (long long)blockIdx.x * 5 * p.E;
 #pragma unroll
-  for (int i = 0; i < 5; ++i)
+  for (int i = 0; i < 5; ++i) {
+    if (!(p.want >> i & 1)) continue;
+    if constexpr (LPR > 64) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) { const int e = threadIdx.x + 256 * k; if (e < p.E) p.part[((long long)blockIdx.x * 5 + i) * p.E + e] = a[i][k]; }
+      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V>(part + (long long)i * p.E + col, a[i] + k * V); }
+    } else {                                         // the rows of a wave by shuffles, its four waves through LDS
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1) a[i][k] += __shfl_xor(a[i][k], o, 64);
+      __syncthreads();
+      if ((threadIdx.x & 63) < LPR) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) join[((threadIdx.x >> 6) * LPR + ln.sub) * NV + k] = a[i][k];
+      }
+      __syncthreads();
+      for (int j = threadIdx.x; j < LPR * NV; j += BT) {
+        const int col = (j / NV + LPR * (j % NV / V)) * V + j % V;
+        if (col < p.E) part[(long long)i * p.E + col] = (join[j] + join[LPR * NV + j]) + (join[2 * LPR * NV + j] + join[3 * LPR * NV + j]);
+      }
+    }
+  }
 }
 
 struct Outs { float* p[5]; };
 
-// the blocks' sums in block order: grid.y 0..3 the parameters (over all blocks), 4 + g the gate row g (over its own)
-__global__ __launch_bounds__(256) void norm_residual_sum_kernel(const float* __restrict__ part, Outs o, int E, long long nall, int nblk, int gate_acc) {
-  const int e = blockIdx.x * 256 + threadIdx.x, which = min((int)blockIdx.y, 4);
+// the blocks' sums in a fixed order: 32 columns by 32 runs of blocks a thread block; grid.y 0..3 the parameters (over all blocks), 4 + g the gate row g (over
+// its own)
+__global__ __launch_bounds__(1024) void norm_residual_sum_kernel(const float* __restrict__ part, Outs o, int E, long long nall, int nblk, int gate_acc, long long g0) {
+  __shared__ float red[32][33];
+  const int which = min((int)blockIdx.y, 4), cl = threadIdx.x & 31, run = threadIdx.x >> 5, e = blockIdx.x * 32 + cl;
   float* out = o.p[which];
-  if (e >= E || !out) return;
-  const long long g = (int)blockIdx.y - which, n0 = which < 4 ? 0 : g * nblk, n1 = which < 4 ? nall : n0 + nblk;
+  if (!out) return;
+  const long long g = g0 + (int)blockIdx.y - which, n0 = which < 4 ? 0 : g * nblk, n1 = which < 4 ? nall : n0 + nblk;
   float s = 0.f;
-  for (long long n = n0; n < n1; ++n) s += part[(n * 5 + which) * E + e];
+  if (e < E) {
+#pragma unroll 8
+    for (long long n = n0 + run; n < n1; n += 32) s += part[(n * 5 + which) * E + e];
+  }
+  red[run][cl] = s;
+  __syncthreads();
+  if (run || e >= E) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s += red[i][cl];
   if (which < 4) out[e] += s;
   else out[g * E + e] = gate_acc ? out[g * E + e] + s : s;
 }
 
-// tokens a block walks: enough blocks to fill the chip
-int rows_of(long long T, long long per) {
-  long long r = T / 1024;
-  if (r < 1) r = 1;
+// Lanes a row and chunks a lane, by the row's 16-byte chunks (columns where rows do not start on 16 bytes): up to a wave's 64 lanes one chunk each, then up to 4
+// a lane, then rows over a block -- of 256 threads for up to 1024 chunks, 512 beyond, so that the backward's five sums of a thread's columns stay
+// in registers.
+template <typename TS, int V, template <typename, int, int, int> class K>
+int by_width(const NRP& p, hipStream_t st) {
+  const int n = smx_cdiv(p.E, V);
+  if (n <= 8) return K<TS, V, 8, 1>::go(p, st);
+  if (n <= 16) return K<TS, V, 16, 1>::go(p, st);
+  if (n <= 32) return K<TS, V, 32, 1>::go(p, st);
+  if (n <= 64) return K<TS, V, 64, 1>::go(p, st);
+  if (n <= 128) return K<TS, V, 64, 2>::go(p, st);
+  if (n <= 256) return K<TS, V, 64, 4>::go(p, st);
+  if (n <= 512) return K<TS, V, 256, 2>::go(p, st);
+  if (n <= 1024) return K<TS, V, 256, 4>::go(p, st);
+  if (n <= 2048) return K<TS, V, 512, 4>::go(p, st);
+  if constexpr (V < 8) {
+    if (n <= 4096) return K<TS, V, 512, 8>::go(p, st);
+    if constexpr (V == 1) return n <= 8192 ? K<TS, V, 512, 16>::go(p, st) : K<TS, V, 512, 32>::go(p, st);
+  }
+  return SMX_EINVAL;
+}
+
+template <typename TS, int V, int LPR, int N> struct Fwd {
+  static int go(const NRP& p, hipStream_t st) {
+    const long long need = (p.T + Lanes<LPR>::RPB - 1) / Lanes<LPR>::RPB;
+    SMX_LAUNCH((norm_residual_kernel<TS, V, LPR, N>), dim3((unsigned)(need < 4096 ? need : 4096)), dim3(Lanes<LPR>::BT), 0, st, p);
+    return smx_launch_status();
+  }
+};
+template <typename TS, int V, int LPR, int N> struct Bwd {
+  static int go(const NRP& p, hipStream_t st) {
+    SMX_LAUNCH((norm_residual_bwd_kernel<V, LPR, N>), dim3((unsigned)(p.T / p.per * p.nblk)), dim3(Lanes<LPR>::BT), 0, st, p);
+    return smx_launch_status();
+  }
+};
+
+// tokens a backward block walks: about 512 blocks (their sums are written and read once more), but not fewer tokens than it has rows at a time
+int rows_of(long long T, long long per, int E) {
+  long long r = (T + 511) / 512;
+  const int at_a_time = E <= 32 ? 32 : E <= 64 ? 16 : E <= 128 ? 8 : E <= 1024 ? 4 : 1;
+  if (r < at_a_time) r = at_a_time;
   if (r > per) r = per;
   return (int)r;
 }
@@ -188,18 +364,16 @@ NRP params(const smx_norm_residual_desc* d) {
   NRP p;
   p.x = d->x; p.h = d->h; p.xo = d->xo; p.y = d->y; p.pg = d->post_gamma; p.pb = d->post_beta; p.ng = d->pre_gamma; p.nb = d->pre_beta; p.gate = d->gate;
   p.gx = d->gx; p.gy = d->gy; p.dx = d->dx; p.dh = d->dh; p.part = d->ws; p.T = d->T; p.per = d->T / d->groups; p.E = d->E; p.rms = d->rms != 0;
-  p.rows = rows_of(d->T, p.per); p.nblk = smx_cdiv(p.per, p.rows); p.rs = d->res_scale; p.eps = d->eps;
+  p.rows = rows_of(d->T, p.per, d->E); p.nblk = smx_cdiv(p.per, p.rows); p.rs = d->res_scale; p.eps = d->eps;
+  p.want = (d->dpre_gamma ? 1 : 0) | (d->dpre_beta ? 2 : 0) | (d->dpost_gamma ? 4 : 0) | (d->dpost_beta ? 8 : 0) | (d->dgate ? 16 : 0);
   return p;
 }
 
-template <typename TS>
-int forward(const NRP& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.T), block(256);
-  if (p.E <= 256) SMX_LAUNCH((norm_residual_kernel<TS, 1>), grid, block, 0, st, p);
-  else if (p.E <= 1024) SMX_LAUNCH((norm_residual_kernel<TS, 4>), grid, block, 0, st, p);
-  else if (p.E <= 4096) SMX_LAUNCH((norm_residual_kernel<TS, 16>), grid, block, 0, st, p);
-  else SMX_LAUNCH((norm_residual_kernel<TS, 64>), grid, block, 0, st, p);
-  return smx_launch_status();
+// do all rows of these tensors start on 16 bytes?
+bool wide(int E, int size, std::initializer_list<const void*> ps) {
+  uintptr_t a = (uintptr_t)E * size;
+  for (const void* p : ps) a |= (uintptr_t)p;
+  return (a & 15) == 0;
 }
 
 }  // namespace
@@ -208,30 +382,34 @@ extern "C" int smx_norm_residual(const smx_norm_residual_desc* d, void* stream) 
   const int rc = check(d, false);
   if (rc != SMX_OK) return rc;
   const NRP p = params(d);
-  return d->bf16 ? forward<bf16_t>(p, (hipStream_t)stream) : forward<float>(p, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  const bool w = wide(p.E, d->bf16 ? 2 : 4, {p.x, p.h, p.xo, p.y, p.pg, p.pb, p.ng, p.nb, p.gate});
+  if (d->bf16) return w ? by_width<bf16_t, 8, Fwd>(p, st) : by_width<bf16_t, 1, Fwd>(p, st);
+  return w ? by_width<float, 4, Fwd>(p, st) : by_width<float, 1, Fwd>(p, st);
 }
 
 extern "C" int64_t smx_norm_residual_bwd_ws_floats(int64_t T, int64_t groups, int E) {
   if (T <= 0 || groups <= 0 || T % groups || E <= 0 || E > 16384 || T > 0x7fffffffLL) return -1;
-  return groups * smx_cdiv(T / groups, rows_of(T, T / groups)) * 5 * E;
+  return groups * smx_cdiv(T / groups, rows_of(T, T / groups, E)) * 5 * E;
 }
 
 extern "C" int smx_norm_residual_bwd_f32(const smx_norm_residual_desc* d, void* stream) {
-  const int rc = check(d, true);
+  int rc = check(d, true);
   if (rc != SMX_OK) return rc;
-  if (d->bf16 || (!d->gx && !d->gy) || (d->gy && !d->pre_gamma) || (d->dgate && !d->gate) || (d->groups > 65531 && d->dgate)) return SMX_EINVAL;
+  if (d->bf16 || (!d->gx && !d->gy) || (d->gy && !d->pre_gamma) || (d->dgate && !d->gate)) return SMX_EINVAL;
   if (((d->dpost_gamma || d->dpost_beta) && !d->post_gamma) || ((d->dpre_gamma || d->dpre_beta) && !d->pre_gamma)) return SMX_EINVAL;
   if (!d->ws || ((uintptr_t)d->ws & 15) || d->ws_floats < smx_norm_residual_bwd_ws_floats(d->T, d->groups, d->E)) return SMX_EINVAL;
   const NRP p = params(d);
-  const long long nall = d->groups * p.nblk;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)nall), block(256);
-  if (p.E <= 256) SMX_LAUNCH(norm_residual_bwd_kernel<1>, grid, block, 0, st, p);
-  else if (p.E <= 1024) SMX_LAUNCH(norm_residual_bwd_kernel<4>, grid, block, 0, st, p);
-  else if (p.E <= 4096) SMX_LAUNCH(norm_residual_bwd_kernel<16>, grid, block, 0, st, p);
-  else SMX_LAUNCH(norm_residual_bwd_kernel<64>, grid, block, 0, st, p);
+  rc = wide(p.E, 4, {p.h, p.xo, p.gx, p.gy, p.dx, p.dh, p.pg, p.pb, p.ng, p.nb, p.gate}) ? by_width<float, 4, Bwd>(p, st) : by_width<float, 1, Bwd>(p, st);
+  if (rc != SMX_OK || !p.want) return rc;
   const Outs o = {{d->dpre_gamma, d->dpre_beta, d->dpost_gamma, d->dpost_beta, d->dgate}};
-  SMX_LAUNCH(norm_residual_sum_kernel, dim3(smx_cdiv(p.E, 256), (unsigned)(d->dgate ? 4 + d->groups : 4)), block, 0, st, (const float*)d->ws, o, p.E, nall,
-             p.nblk, (int)d->gate_accumulate);
+  for (long long g0 = 0; g0 == 0 || (d->dgate && g0 < d->groups); g0 += 65000) {      // (a grid's y ends at 65535)
+    Outs now = o;
+    if (g0) now.p[0] = now.p[1] = now.p[2] = now.p[3] = nullptr;
+    const long long left = d->groups - g0;
+    SMX_LAUNCH(norm_residual_sum_kernel, dim3(smx_cdiv(p.E, 32), (unsigned)(d->dgate ? 4 + (left < 65000 ? left : 65000) : 4)), dim3(1024), 0, st, (const float*)d->ws, now,
+               p.E, (long long)d->groups * p.nblk, p.nblk, (int)d->gate_accumulate, g0);
+  }
   return smx_launch_status();
 }
