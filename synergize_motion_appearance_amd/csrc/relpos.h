@@ -19,20 +19,18 @@ constexpr int MAP_MAX = 2049;         // entries of a bucket map
 constexpr int TABLE_PAD = 96;         // entries a 64-key x 32-query tile can reach beyond the map's ends while it touches the map
 
 // ---- fp32 operands on the half-precision matrix pipe ("f16x3") ----------------------------------------------------------------
-// x = (h1 + h2) 2^-k with two IEEE halves: 22 significand bits; a product is h1 g1 + h1 g2 + h2 g1, the dropped h2 g2 is 2^-22 of it.  k is one number per
-// (sample, kv head) that brings the largest |x| of the heads on it to [2^14, 2^15): values down to 2^-16 of the largest keep all 22 bits, smaller ones are off by at most
-// 2^-40 of the largest.  A first pass finds the largest values, a second writes the halves: planes [B][heads][rows rounded up to 64][DHP] of h1 and of h2,
-// rows that nobody may see and the columns from dh on as zeros.  That is read by every tile of the other side, so splitting here once costs less than
-// splitting in the kernels (a 128-query block would split every key of its head again).
+// x = (h1 + h2) 2^-k with two IEEE halves: 22 significand bits; a product is h1 g1 + h1 g2 + h2 g1, the dropped h2 g2 is 2^-22 of it.  k brings the largest |x|
+// that shares it to [2^14, 2^15): values down to 2^-16 of that keep all 22 bits, smaller ones are off by at most 2^-40 of it.  Rows that a wave keeps in
+// registers are split there, each with a k of its own (own_rows).  Rows that are staged -- read by every block of the other side -- are split once, by a
+// pass before: planes [B][heads][rows rounded up to 64][dh rounded up to 32] of h1 and of h2 with one k per 64 rows; rows that nobody may see and the
+// columns from dh on are zeros.  Where a product sums over staged rows, the k of the tile joins the factor of the other operand (Unit).
 struct Split {
-  const float* src; long long bs; int ld, heads, group, rows, kv, flip;  // group: heads of a kv head; kv: rows of keys (masks and lengths apply); flip: odd rows negated
+  const float* src; long long bs; int ld, heads, rows, kv, flip;  // kv: rows of keys (masks and lengths apply); flip: odd rows negated
   _Float16* hi; _Float16* lo;                                   // planes
-  float* pow2;                                                  // [B][heads / group][2]: 2^k, 2^-k
-  float* top;                                                   // [B][heads][nch] largest |x| of each chunk of CH rows
+  float* inv;                                                   // [B][heads][tiles of 64] 2^-k
   const float* o;                                               // gradient rows: the output, for D_i = dO_i . o_i (dense, as src)
   float* dd;                                                    // [B][heads][rows rounded up to 64]
 };
-constexpr int CH = 512;
 
 struct RP {
   const void* q; const void* k; const void* v; void* o;
@@ -48,13 +46,13 @@ struct RP {
 };
 
 static inline int up64(int n) { return (n + 63) & ~63; }
-static inline int dhp(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : 128; }
+static inline int dhp(int dh) { return (dh + 31) / 32 * 32; }
 static inline bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 // the launchers of relpos_attn.hip
 int check(const smx_relpos_desc* d, RP& p, bool bwd);
-int64_t split_bytes(int B, int heads, int rows, int dh);        // planes, scales, chunk maxima
-char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int group, int rows, int dh, bool kv);
+int64_t split_bytes(int B, int heads, int rows, int dh);        // planes and scales
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dh, bool kv);
 int split_launch(const RP& p, const Split* s, int n, hipStream_t st);
 
 // ---- matrix operands -----------------------------------------------------------------------------------------------------------
@@ -81,7 +79,7 @@ __device__ __forceinline__ void to_levels(const float* v, u32x4 (&f)[NL]) {
     if constexpr (NL == 1) h[i] = cvt2_bf16(v[2 * i], v[2 * i + 1]);
     else {
       h[i] = cvt2_f16(v[2 * i], v[2 * i + 1]);
-      l[i] = cvt2_f16(v[2 * i] - f16lo(h[i]), v[2 * i + 1] - f16hi(h[i]));
+      l[i] = cvt2_f16(fmaf(f16lo(h[i]), -1.f, v[2 * i]), fmaf(f16hi(h[i]), -1.f, v[2 * i + 1]));     // (as an fma: one v_fma_mix_f32 each)
     }
   }
   f[0] = u32x4{h[0], h[1], h[2], h[3]};
@@ -127,6 +125,61 @@ __device__ __forceinline__ float other_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// 2^k and 2^-k for values up to m
+__device__ __forceinline__ float pow2_of(float m, float& inv) {
+  const int e = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;     // floor(log2 m); 2^(14 - e) stays a normal number
+  inv = __uint_as_float((unsigned)(e - 14 + 127) << 23);
+  return __uint_as_float((unsigned)(14 - e + 127) << 23);
+}
+
+// 32 fp32 rows as fragments in registers: lane & 31 the row at x, columns 16 kk + 8 (lane >> 5) + 0..7; -> the row's 2^-k
+template <int DHP>
+__device__ __forceinline__ float own_rows(u32x4 (&f)[DHP / 16][2], const float* x, bool in, int dh) {
+  float v[DHP / 16][8], m = 0.f, inv;
+  const int hh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int kk = 0; kk < DHP / 16; ++kk)
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const int d = kk * 16 + hh * 8 + i;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && d < dh) y = *reinterpret_cast<const float4*>(x + d);
+      v[kk][i] = y.x; v[kk][i + 1] = y.y; v[kk][i + 2] = y.z; v[kk][i + 3] = y.w;
+      m = fmaxf(m, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+    }
+  const float sc = pow2_of(other_max(m), inv);
+#pragma unroll
+  for (int kk = 0; kk < DHP / 16; ++kk) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[kk][i] *= sc;
+    to_levels<2>(v[kk], f[kk]);
+  }
+  return inv;
+}
+
+// An accumulator that sums over staged rows is kept in units of the largest 2^-k so far: a tile of larger values first brings it there (exactly: powers
+// of two), a tile of smaller ones enters with the factor 2^log2w <= 1 on its other operand.  (Below 2^-100 what a half holds of it is zero.)
+struct Unit {
+  float inv = 0.f;
+  template <int N> __device__ __forceinline__ int enter(float t, f32x16 (&acc)[N]) {
+    if (t > inv) {
+      const float r = inv / t;
+      inv = t;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] *= r;
+      return 0;
+    }
+    return max((int)(__float_as_uint(t) >> 23) - (int)(__float_as_uint(inv) >> 23), -100);
+  }
+};
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// keys (queries) a step and the block's waves: 64 rows where four waves stage them, 32 for two waves or where two operands of 128 columns in two halves each
+// would not leave room for a second block on a CU
+template <int DHP, int NL, int NW> constexpr int STEP = NL == 1 ? 64 : NW == 2 || DHP == 128 ? 32 : 64;
 
 // Work order: consecutive block ids go to the 8 XCDs in turn; this gives each XCD a run of consecutive work items, so that the blocks that read the
 // same keys share an L2.

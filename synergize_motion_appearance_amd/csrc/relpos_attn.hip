@@ -4,7 +4,7 @@
 //   relpos_tile_kernel   queries in tiles of 32 a wave on the matrix cores (bf16 storage: bf16 products; fp32 storage: f16x3, relpos.h)
 //   relpos_token_kernel  a few queries per sample (decoding): bound by reading the cache, plain fp32 products on the vector units
 //   relpos_join_kernel   joins the parts where the keys were split over blocks
-//   relpos_top / split   the fp32 operands as two halves each
+//   relpos_split_kernel  the staged fp32 operands as two halves each
 #include "relpos.h"
 
 namespace relpos {
@@ -12,36 +12,7 @@ namespace relpos {
 // ---- fp32 operands as halves (relpos.h: Split) ---------------------------------------------------------------------------------
 struct Splits { Split s[4]; int end[4]; };                       // end: running sum of blocks
 
-__device__ __forceinline__ bool row_seen(const RP& p, const Split& s, int b, int r) {
-  if (r >= s.rows) return false;
-  return !s.kv || (r < p.keys(b) && !(p.mask && p.mask[(long long)b * p.S + r]));
-}
-
-// largest |x| of CH rows of one head; NaN and rows nobody sees do not count
-__global__ __launch_bounds__(256) void relpos_top_kernel(RP p, Splits a) {
-  __shared__ float red[4];
-  int t = 0, id = blockIdx.x;
-  while (id >= a.end[t]) ++t;
-  const Split& s = a.s[t];
-  id -= t ? a.end[t - 1] : 0;
-  const int nch = (s.rows + CH - 1) / CH, c = id % nch, h = id / nch % s.heads, b = id / nch / s.heads;
-  const int q4 = p.dh >> 2, n = min(CH, s.rows - c * CH) * q4;
-  const float* src = s.src + b * s.bs + (long long)c * CH * s.ld + h * p.dh;
-  float m = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int r = i / q4;
-    if (!row_seen(p, s, b, c * CH + r)) continue;
-    const float4 x = *reinterpret_cast<const float4*>(src + (long long)r * s.ld + (i - r * q4) * 4);
-    m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) s.top[((long long)b * s.heads + h) * nch + c] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
-// 64 rows of one head -> both planes; gradient rows: D_i = dO_i . o_i too
+// 64 rows of one head -> both planes and their 2^-k; gradient rows: D_i = dO_i . o_i too
 template <int DHP>
 __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
   __shared__ float red[4];
@@ -49,69 +20,75 @@ __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
   while (id >= a.end[t]) ++t;
   const Split& s = a.s[t];
   id -= t ? a.end[t - 1] : 0;
-  const int nch = (s.rows + CH - 1) / CH, nt = (s.rows + 63) / 64, c = id % nt, h = id / nt % s.heads, b = id / nt / s.heads;
-  const float* top = s.top + ((long long)b * s.heads + h / s.group * s.group) * nch;
-  float m = 0.f;
-  for (int i = threadIdx.x; i < s.group * nch; i += 256) m = fmaxf(m, top[i]);
+  const int nt = (s.rows + 63) / 64, c = id % nt, h = id / nt % s.heads, b = id / nt / s.heads;
+  const int n = s.kv ? min(p.keys(b), s.rows) : s.rows;
+  constexpr int NI = DHP / 16;                                   // four threads a row, NI float4 each
+  const int r = threadIdx.x >> 2, q = threadIdx.x & 3, row = c * 64 + r;
+  const bool in = row < n && !(s.kv && p.mask && p.mask[(long long)b * p.S + row]);
+  const long long at = b * s.bs + (long long)row * s.ld + h * p.dh, tile = ((long long)b * s.heads + h) * nt + c;
+  float4 x[NI];
+  float m = 0.f, D = 0.f;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int d = (i * 4 + q) * 4;
+    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in && d < p.dh) {
+      x[i] = *reinterpret_cast<const float4*>(s.src + at + d);
+      if (s.dd) { const float4 y = *reinterpret_cast<const float4*>(s.o + at + d); D += (x[i].x * y.x + x[i].y * y.y) + (x[i].z * y.z + x[i].w * y.w); }
+    }
+    m = fmaxf(m, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+  }
+  if (s.dd) {
+    D += __shfl_xor(D, 1, 64);
+    D += __shfl_xor(D, 2, 64);
+    if (q == 0) s.dd[tile * 64 + r] = D;
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;    // floor(log2 m); 2^(14 - ex) stays a normal number
-  const float sc = __uint_as_float((unsigned)(14 - ex + 127) << 23);
-  if (threadIdx.x == 0 && c == 0 && h % s.group == 0)
-    *reinterpret_cast<float2*>(s.pow2 + ((long long)b * (s.heads / s.group) + h / s.group) * 2) = make_float2(sc, __uint_as_float((unsigned)(ex - 14 + 127) << 23));
-  constexpr int Q4 = DHP / 4;
-  const long long out = (((long long)b * s.heads + h) * nt + c) * 64 * DHP;
+  float inv;
+  float sc = pow2_of(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), inv);
+  if (threadIdx.x == 0) s.inv[tile] = inv;
+  if (s.flip && (r & 1)) sc = -sc;
+  const long long out = (tile * 64 + r) * DHP;
 #pragma unroll
-  for (int it = 0; it < 64 * Q4 / 256; ++it) {
-    const int i = it * 256 + threadIdx.x, r = i / Q4, d = i % Q4 * 4, row = c * 64 + r;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    const long long at = b * s.bs + (long long)row * s.ld + h * p.dh + d;
-    const bool in = d < p.dh && row_seen(p, s, b, row);
-    if (in) x = *reinterpret_cast<const float4*>(s.src + at);
-    if (s.dd) {
-      float D = 0.f;
-      if (in) { const float4 y = *reinterpret_cast<const float4*>(s.o + at); D = (x.x * y.x + x.y * y.y) + (x.z * y.z + x.w * y.w); }
-#pragma unroll
-      for (int o = 1; o < Q4; o <<= 1) D += __shfl_xor(D, o, 64);
-      if (d == 0) s.dd[((long long)b * s.heads + h) * nt * 64 + row] = D;
-    }
-    const float w = s.flip && (r & 1) ? -sc : sc;
-    x.x *= w; x.y *= w; x.z *= w; x.w *= w;
-    const uint2 h2 = make_uint2(cvt2_f16(x.x, x.y), cvt2_f16(x.z, x.w));
-    const uint2 l2 = make_uint2(cvt2_f16(x.x - f16lo(h2.x), x.y - f16hi(h2.x)), cvt2_f16(x.z - f16lo(h2.y), x.w - f16hi(h2.y)));
-    *reinterpret_cast<uint2*>(s.hi + out + i * 4) = h2;
-    *reinterpret_cast<uint2*>(s.lo + out + i * 4) = l2;
+  for (int i = 0; i < NI; ++i) {
+    const float4 y = make_float4(x[i].x * sc, x[i].y * sc, x[i].z * sc, x[i].w * sc);
+    const uint2 h2 = make_uint2(cvt2_f16(y.x, y.y), cvt2_f16(y.z, y.w));
+    const uint2 l2 = make_uint2(cvt2_f16(y.x - f16lo(h2.x), y.y - f16hi(h2.x)), cvt2_f16(y.z - f16lo(h2.y), y.w - f16hi(h2.y)));
+    *reinterpret_cast<uint2*>(s.hi + out + (i * 4 + q) * 4) = h2;
+    *reinterpret_cast<uint2*>(s.lo + out + (i * 4 + q) * 4) = l2;
   }
 }
 
 int64_t split_bytes(int B, int heads, int rows, int dh) {
-  return (int64_t)B * heads * ((int64_t)up64(rows) * dhp(dh) * 4 + 16 + ((rows + CH - 1) / CH + 3) / 4 * 16);
+  return (int64_t)B * heads * ((int64_t)up64(rows) * dhp(dh) * 4 + (up64(rows) / 64 + 3) / 4 * 16);
 }
 
-char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int group, int rows, int dh, bool kv) {
+char* split_setup(Split& s, char* ws, const float* src, long long bs, int ld, int B, int heads, int rows, int dh, bool kv) {
   const int64_t plane = (int64_t)B * heads * up64(rows) * dhp(dh);
-  s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.group = group; s.rows = rows; s.kv = kv;
-  s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.pow2 = (float*)(s.lo + plane); s.top = s.pow2 + 4 * (int64_t)B * heads;
-  s.o = nullptr; s.dd = nullptr; s.flip = 0;
+  s.src = src; s.bs = bs; s.ld = ld; s.heads = heads; s.rows = rows; s.kv = kv; s.flip = 0;
+  s.hi = (_Float16*)ws; s.lo = s.hi + plane; s.inv = (float*)(s.lo + plane);
+  s.o = nullptr; s.dd = nullptr;
   return ws + split_bytes(B, heads, rows, dh);
 }
 
 int split_launch(const RP& p, const Split* s, int n, hipStream_t st) {
-  Splits a, c;
-  long long na = 0, nc = 0;
+  Splits a;
+  long long nb = 0;
   for (int i = 0; i < 4; ++i) {
-    if (i < n) { a.s[i] = c.s[i] = s[i]; na += (long long)p.B * s[i].heads * ((s[i].rows + CH - 1) / CH); nc += (long long)p.B * s[i].heads * (up64(s[i].rows) / 64); }
-    if (na > 0x7fffffffLL || nc > 0x7fffffffLL) return SMX_EINVAL;
-    a.end[i] = (int)na; c.end[i] = (int)nc;
+    if (i < n) { a.s[i] = s[i]; nb += (long long)p.B * s[i].heads * (up64(s[i].rows) / 64); }
+    if (nb > 0x7fffffffLL) return SMX_EINVAL;
+    a.end[i] = (int)nb;
   }
-  SMX_LAUNCH(relpos_top_kernel, dim3((unsigned)na), dim3(256), 0, st, p, a);
-  const int w = dhp(p.dh);
-  if (w == 32) SMX_LAUNCH(relpos_split_kernel<32>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
-  else if (w == 64) SMX_LAUNCH(relpos_split_kernel<64>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
-  else SMX_LAUNCH(relpos_split_kernel<128>, dim3((unsigned)nc), dim3(256), 0, st, p, c);
+  const dim3 grid((unsigned)nb), block(256);
+  switch (dhp(p.dh)) {
+    case 32: SMX_LAUNCH(relpos_split_kernel<32>, grid, block, 0, st, p, a); break;
+    case 64: SMX_LAUNCH(relpos_split_kernel<64>, grid, block, 0, st, p, a); break;
+    case 96: SMX_LAUNCH(relpos_split_kernel<96>, grid, block, 0, st, p, a); break;
+    default: SMX_LAUNCH(relpos_split_kernel<128>, grid, block, 0, st, p, a);
+  }
   return smx_launch_status();
 }
 
@@ -144,30 +121,32 @@ namespace {
 using namespace relpos;
 
 // ---- queries in tiles ----------------------------------------------------------------------------------------------------------
-// where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage the planes; parts: m, l [row][part], o [row][part][dh] when the keys are split
+// where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage q and the planes of k and v; parts: m, l [row][part], o
+// [row][part][dh] when the keys are split
 struct Src {
-  Split q, k, v;
+  Split k, v;
   int nparts, per;                    // parts of the keys, keys of a part (a multiple of 64)
   float* part_ml; float* part_o;
 };
 
 // A wave owns 32 queries as the columns of swapped products: S^T = K Q^T (a lane: one query, 16 of 32 keys), O^T += V^T P^T with P taken from the score
 // registers as they are -- the transposing LDS reads fetch V's columns in the order of an accumulator's rows.  The statistics are lane-local but for one
-// exchange between the two half waves.  Four waves share the staged keys: 64 (32 for DHP = 128) a step, double buffered, the next tile's loads in flight
-// during the products.  The running maximum follows only when a row outgrows it by 2^8: P stays below 2^8 (with fp32 storage P carries 2^6 more, below
-// the largest half by 2^1, its second half then off by at most 2^-31 of the row's largest weight).
+// exchange between the two half waves.  The block's waves share the staged keys, the next tile's loads are in flight during the products.
+// Weights are 2^(s - mo), mo finite and followed only when a row outgrows it by 2^8 (and at its first key): the scores leave the products through one fma,
+// and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
-template <int DHP, int NL>
-__global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
-  constexpr int TK = DHP == 128 ? 32 : 64, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>;
+template <int DHP, int NL, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void relpos_tile_kernel(RP p, Src a) {
+  constexpr int TK = STEP<DHP, NL, NW>, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>, NT = 64 * NW;
   constexpr int PLANE = TK * RB, STAGE = 2 * NL * PLANE;         // K levels, V levels
-  constexpr int CPR = DHP / 8, NCH = TK * CPR / 256;             // 16-byte chunks of a row; of a plane, a thread
+  constexpr int CPR = DHP / 8, NCH = TK * CPR / NT;              // 16-byte chunks of a row; of a plane, a thread
   constexpr float PSH = NL == 2 ? 6.f : 0.f;
   extern __shared__ __attribute__((aligned(16))) char sm[];      // two stages, bias, masks
   float* lut = reinterpret_cast<float*>(sm + 2 * STAGE);
   unsigned long long* seen = reinterpret_cast<unsigned long long*>(sm + 2 * STAGE + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
-  const int nq = (p.L + 127) / 128;
+  constexpr int QB = 32 * NW;
+  const int nq = (p.L + QB - 1) / QB;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
   const int qb = nq - 1 - id % nq;                               // causal: the longest rows first
   id /= nq;
@@ -175,28 +154,19 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   id /= a.nparts;
   const int h = id % p.H, b = id / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);
-  const int q0 = qb * 128 + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
+  const int q0 = qb * QB + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
   const int wlast = pos0 + min(q0 + 31, p.L - 1);                // the wave's last position; none if q0 >= L
-  int kend = p.causal ? min(n, pos0 + min(qb * 128 + 127, p.L - 1) + 1) : n;
+  int kend = p.causal ? min(n, pos0 + min(qb * QB + QB - 1, p.L - 1) + 1) : n;
   const int kbeg = a.nparts > 1 ? part * a.per : 0;
   if (a.nparts > 1) kend = min(kend, kbeg + a.per);
   const int ntiles = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
 
   fill_bias(lut, p, h);
   const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
-  float sc = p.scale * LOG2E, inv_v = 1.f;
+  float sq = p.scale * LOG2E;
   u32x4 qf[KS][NL];
   if constexpr (NL == 2) {
-    const int at2 = (b * p.Hkv + hk) * 2 + 1;
-    sc = sc * a.q.pow2[at2] * a.k.pow2[at2];
-    inv_v = a.v.pow2[at2];
-    const int up = (p.L + 63) & ~63;
-    const long long at = (((long long)b * p.H + h) * up + qi) * DHP + hh * 8;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      qf[kk][0] = qi < up ? *reinterpret_cast<const u32x4*>(a.q.hi + at + kk * 16) : u32x4{0, 0, 0, 0};
-      qf[kk][1] = qi < up ? *reinterpret_cast<const u32x4*>(a.q.lo + at + kk * 16) : u32x4{0, 0, 0, 0};
-    }
+    sq *= own_rows<DHP>(qf, (const float*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh, qi < p.L, p.dh);
   } else {
     const bf16_t* Q = (const bf16_t*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh;
 #pragma unroll
@@ -211,19 +181,21 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
 
   u32x4 kreg[NL][NCH], vreg[NL][NCH];
   unsigned long long sreg = 0;
+  const int tiles = (p.S + 63) >> 6;
+  const long long tile0 = ((long long)b * p.Hkv + hk) * tiles;
   auto load_tile = [&](int key0) {
     if constexpr (NL == 2) {
-      const long long at = (((long long)b * p.Hkv + hk) * ((p.S + 63) & ~63) + key0) * DHP;
+      const long long at = (tile0 * 64 + key0) * DHP;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const int e = (c * 256 + threadIdx.x) * 8;
+        const int e = (c * NT + threadIdx.x) * 8;
         kreg[0][c] = *reinterpret_cast<const u32x4*>(a.k.hi + at + e); kreg[1][c] = *reinterpret_cast<const u32x4*>(a.k.lo + at + e);
         vreg[0][c] = *reinterpret_cast<const u32x4*>(a.v.hi + at + e); vreg[1][c] = *reinterpret_cast<const u32x4*>(a.v.lo + at + e);
       }
     } else {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const int e = c * 256 + threadIdx.x, key = key0 + e / CPR, d = e % CPR * 8;
+        const int e = c * NT + threadIdx.x, key = key0 + e / CPR, d = e % CPR * 8;
         const bf16_t* K = (const bf16_t*)p.k + b * p.k_bs + (long long)key * p.ldk + hk * p.dh + d;
         const bf16_t* V = (const bf16_t*)p.v + b * p.v_bs + (long long)key * p.ldv + hk * p.dh + d;
         uint2 x = make_uint2(0, 0), y = x, z = x, w = x;
@@ -244,7 +216,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
     char* st = sm + buf * STAGE;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int e = c * 256 + threadIdx.x, off = e / CPR * RB + e % CPR * 16;
+      const int e = c * NT + threadIdx.x, off = e / CPR * RB + e % CPR * 16;
 #pragma unroll
       for (int l = 0; l < NL; ++l) {
         *reinterpret_cast<u32x4*>(st + l * PLANE + off) = kreg[l][c];
@@ -257,7 +229,9 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   f32x16 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) o[t] = zero16();
-  float m = -INFINITY, l = 0.f;
+  float mo = 0.f, l = 0.f;
+  bool begun = false;                                            // the row has met a key
+  Unit vu;
   const unsigned long long ALL = TK == 64 ? ~0ull : 0xffffffffull;
   if (ntiles > 0) { load_tile(kbeg); store_tile(0); }
   __syncthreads();
@@ -267,6 +241,11 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
     char* st = sm + buf * STAGE;
     const unsigned long long left = seen[buf];
     if (left && q0 < p.L && !(p.causal && key0 > wlast)) {
+      float sc = sq, lw = 0.f;
+      if constexpr (NL == 2) {
+        sc = sq * a.k.inv[tile0 + (key0 >> 6)];
+        lw = (float)vu.enter(a.v.inv[tile0 + (key0 >> 6)], o);
+      }
       f32x16 s[NU];
 #pragma unroll
       for (int u = 0; u < NU; ++u) s[u] = zero16();
@@ -279,9 +258,10 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
           for (int x = 0; x < NL; ++x) kf[x] = row_frag<DHP>(st + x * PLANE, u * 32, kk);
           s[u] = mfma_levels<NL>(kf, qf[kk], s[u]);
         }
+      const float kc = lw - mo;
       const int e0 = key0 - (pos0 + q0) - p.map_lo;              // entry of the tile's first key and first query; the others: + key - query
       if (e0 + TK - 1 <= 0 || e0 - 31 >= p.map_n - 1) {
-        const float c = e0 + TK - 1 <= 0 ? first_bias : last_bias;
+        const float c = (e0 + TK - 1 <= 0 ? first_bias : last_bias) + kc;
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -291,7 +271,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], sc, lp[u * 32 + crow(r)]);
+          for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], sc, lp[u * 32 + crow(r)]) + kc;
       }
       if (left != ALL) {
         const unsigned long long mine = left >> (4 * hh);
@@ -314,21 +294,27 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-      top = other_max(top);
-      if (__ballot(top > m + 8.f)) {
-        const float mn = fmaxf(m, top), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn; l *= al;
+      top = other_max(top) - lw;                                 // s - mo of the row's largest score
+      const bool first = !begun && top > -INFINITY;
+      if (__ballot(first || top > PSH + 8.f)) {
+        const float d = first ? top - PSH : top > PSH ? top - PSH : 0.f, al = begun ? __builtin_amdgcn_exp2f(-d) : 0.f;
+        begun |= first;
+        mo += d; l *= al;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] *= al;
+          for (int r = 0; r < 16; ++r) s[u][r] -= d;
+#pragma unroll
+        for (int x = 0; x < DT; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[x][r] *= al;
       }
-      const float mo = m == -INFINITY ? 0.f : m - PSH;
+      float lt = 0.f;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         float e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { e[r] = __builtin_amdgcn_exp2f(s[u][r] - mo); l += e[r]; }
+        for (int r = 0; r < 16; ++r) { e[r] = __builtin_amdgcn_exp2f(s[u][r]); lt += e[r]; }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           u32x4 pf[NL];
@@ -342,12 +328,14 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
           }
         }
       }
+      l = fmaf(lt, exp2i(-(int)lw), l);
     }
     if (t + 1 < ntiles) store_tile(buf ^ 1);
     __syncthreads();
   }
   if (qi >= p.L) return;
   l = other_sum(l);
+  const float inv_v = NL == 2 ? vu.inv : 1.f;
   const long long row = ((long long)b * p.H + h) * p.L + qi;
   if (a.nparts > 1) {
     float* O = a.part_o + (row * a.nparts + part) * p.dh;
@@ -358,7 +346,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
         const int c = d * 32 + 8 * g + 4 * hh;
         if (c < p.dh) *reinterpret_cast<float4*>(O + c) = make_float4(o[d][4 * g] * inv_v, o[d][4 * g + 1] * inv_v, o[d][4 * g + 2] * inv_v, o[d][4 * g + 3] * inv_v);
       }
-    if (hh == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.nparts + part) * 2) = make_float2(m == -INFINITY ? m : m - PSH, l);
+    if (hh == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.nparts + part) * 2) = make_float2(begun ? mo : -INFINITY, l);
     return;
   }
   const float il = l > 0.f ? inv_v / l : 0.f;
@@ -373,22 +361,25 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
         else St<bf16_t>::st4((bf16_t*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);
       }
     }
-  if (p.lse && hh == 0) p.lse[row] = l > 0.f ? m - PSH + __log2f(l) : INFINITY;
+  if (p.lse && hh == 0) p.lse[row] = l > 0.f ? mo + __log2f(l) : INFINITY;
 }
 
 // ---- a few queries per sample ---------------------------------------------------------------------------------------------------
 // A block takes a part of one (sample, kv head)'s keys for RT of its G * L query rows.  LPK lanes hold a key's row, EPL values each, and the same columns of the
 // RT queries and running outputs; every group of LPK lanes walks keys of its own, four a step, with a running maximum and sum of its own: the only
 // exchanges are the LPK-lane sums of the scores.  The groups are joined through LDS at the end, the parts by relpos_join_kernel.
-template <typename T, int EPL> struct Row;
+template <typename T, int EPL> struct Row;                       // EPL values as they lie in memory
 template <> struct Row<float, 4> {
-  static __device__ __forceinline__ void ld(const float* p, float (&f)[4]) { const float4 v = *reinterpret_cast<const float4*>(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  typedef float Raw __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ void wide(Raw v, float (&f)[4]) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
 };
 template <> struct Row<bf16_t, 4> {
-  static __device__ __forceinline__ void ld(const bf16_t* p, float (&f)[4]) { const float4 v = St<bf16_t>::ld4(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  typedef unsigned Raw __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void wide(Raw v, float (&f)[4]) { const float4 x = unpack4(make_uint2(v.x, v.y)); f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; }
 };
 template <> struct Row<bf16_t, 8> {
-  static __device__ __forceinline__ void ld(const bf16_t* p, float (&f)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), f); }
+  typedef unsigned Raw __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ void wide(Raw v, float (&f)[8]) { unpack8(make_uint4(v.x, v.y, v.z, v.w), f); }
 };
 
 template <int CTRL> __device__ __forceinline__ float dpp_add(float x) {
@@ -406,9 +397,11 @@ template <int LPK> __device__ __forceinline__ float lanes_sum(float x) {
 
 template <typename T, int EPL, int LPK, int RT>
 __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
-  constexpr int GPB = 256 / LPK, U = 4;                          // groups of a block
+  using R = Row<T, EPL>;
+  using Raw = typename R::Raw;
+  constexpr int GPB = 256 / LPK, U = 4;                          // groups of a block, keys a step
   extern __shared__ __attribute__((aligned(16))) char sm[];
-  float* red = reinterpret_cast<float*>(sm);                     // [GPB][RT][2 + LPK * EPL]
+  float* red = reinterpret_cast<float*>(sm);                     // [4 waves][RT][2 + LPK * EPL]
   const int sub = threadIdx.x % LPK, grp = threadIdx.x / LPK, c0 = sub * EPL;
   const int rows = p.G * p.L, nr = (rows + RT - 1) / RT;
   unsigned id = blockIdx.x;
@@ -430,7 +423,7 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
     m[r] = -INFINITY; l[r] = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) { q[r][e] = 0.f; o[r][e] = 0.f; }
-    if (in) Row<T, EPL>::ld((const T*)p.q + b * p.q_bs + (long long)i * p.ldq + hd[r] * p.dh + c0, q[r]);
+    if (in) R::wide(*reinterpret_cast<const Raw*>((const T*)p.q + b * p.q_bs + (long long)i * p.ldq + hd[r] * p.dh + c0), q[r]);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) q[r][e] *= p.scale * LOG2E;
     fb[r] = p.table[(long long)p.map[0] * p.H + hd[r]] * LOG2E;
@@ -439,49 +432,67 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
   const int k0 = part * a.per, k1 = min(min(k0 + a.per, n), p.causal ? pmax + 1 : n);
   const T* K = (const T*)p.k + b * p.k_bs + hk * p.dh + c0;
   const T* V = (const T*)p.v + b * p.v_bs + hk * p.dh + c0;
-  for (int j0 = k0; j0 < k1; j0 += GPB * U) {
-    float kf[U][EPL], vf[U][EPL];
-    bool ok[U];
+  Raw kn[U], vn[U];                                              // the next step's keys and values, in flight during this one's sums
+  unsigned okn = 0;
+  auto load = [&](int j0) {
+    okn = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * GPB + grp;
-      ok[u] = j < k1 && !(p.mask && p.mask[(long long)b * p.S + j]);
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) { kf[u][e] = 0.f; vf[u][e] = 0.f; }
-      if (ok[u] && in) {
-        Row<T, EPL>::ld(K + (long long)j * p.ldk, kf[u]);
-        Row<T, EPL>::ld(V + (long long)j * p.ldv, vf[u]);
+      kn[u] = Raw(0); vn[u] = Raw(0);
+      if (j < k1 && !(p.mask && p.mask[(long long)b * p.S + j])) {
+        okn |= 1u << u;
+        if (in) {
+          kn[u] = *reinterpret_cast<const Raw*>(K + (long long)j * p.ldk);
+          vn[u] = *reinterpret_cast<const Raw*>(V + (long long)j * p.ldv);
+        }
       }
     }
+  };
+  if (k0 < k1) load(k0);
+  for (int j0 = k0; j0 < k1; j0 += GPB * U) {
+    Raw kr[U], vr[U];
+    const unsigned ok = okn;
+#pragma unroll
+    for (int u = 0; u < U; ++u) { kr[u] = kn[u]; vr[u] = vn[u]; }
+    if (j0 + GPB * U < k1) load(j0 + GPB * U);
     // the step's keys all beyond one end of the map for all rows: the bias is one number a row
     const bool far_lo = j0 + GPB * U - 1 - pmin - p.map_lo <= 0, far_hi = j0 - pmax - p.map_lo >= p.map_n - 1;
+    float s[RT][U];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float s[U], top = -INFINITY;
+    for (int u = 0; u < U; ++u) {
+      float kf[EPL];
+      R::wide(kr[u], kf);
+      const int j = j0 + u * GPB + grp;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int r = 0; r < RT; ++r) {
         float x = 0.f;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) x = fmaf(q[r][e], kf[u][e], x);
+        for (int e = 0; e < EPL; ++e) x = fmaf(q[r][e], kf[e], x);
         x = lanes_sum<LPK>(x);
-        const int delta = j0 + u * GPB + grp - pos[r];
+        const int delta = j - pos[r];
         x += far_lo ? fb[r] : far_hi ? lb[r] : p.table[(long long)p.map[p.entry(delta)] * p.H + hd[r]] * LOG2E;
-        s[u] = ok[u] && !(p.causal && delta > 0) ? x : -INFINITY;
-        top = fmaxf(top, s[u]);
+        s[r][u] = (ok >> u & 1) && !(p.causal && delta > 0) ? x : -INFINITY;
       }
-      const float mn = fmaxf(m[r], top);
-      if (mn == -INFINITY) continue;
-      const float al = __builtin_amdgcn_exp2f(m[r] - mn);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float mn = fmaxf(m[r], fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3])));
+      const float mf = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m[r] - mf);
       m[r] = mn; l[r] *= al;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) o[r][e] *= al;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float w = __builtin_amdgcn_exp2f(s[u] - mn);
-        l[r] += w;
+      for (int u = 0; u < U; ++u) { s[r][u] = __builtin_amdgcn_exp2f(s[r][u] - mf); l[r] += s[r][u]; }
+    }
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(w, vf[u][e], o[r][e]);
-      }
+    for (int u = 0; u < U; ++u) {
+      float vf[EPL];
+      R::wide(vr[u], vf);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(s[r][u], vf[e], o[r][e]);
     }
   }
   // join the groups: first those of a wave, lane by lane, then the waves through LDS
@@ -530,33 +541,42 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
   }
 }
 
-// o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts; a thread four columns of a row
+// o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts: a wave a row, its lanes the parts for the weights, then columns by runs of parts
 template <typename T>
 __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
-  const int q4 = p.dh >> 2;
-  const long long t = blockIdx.x * 256LL + threadIdx.x, row = t / q4;
+  const int lane = threadIdx.x & 63;
+  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
   if (row >= (long long)p.B * p.H * p.L) return;
-  const int c = (int)(t - row * q4) * 4;
-  const float* ml = a.part_ml + row * a.nparts * 2;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nparts;
   float m = -INFINITY;
-  for (int s = 0; s < a.nparts; ++s) m = fmaxf(m, ml[2 * s]);
+  for (int s = lane; s < a.nparts; s += 64) m = fmaxf(m, ml[s].x);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float mf = m == -INFINITY ? 0.f : m;
+  const int lanes = p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32, run = lane / lanes, runs = 64 / lanes, c = lane % lanes * 4;
   float l = 0.f, x = 0.f, y = 0.f, z = 0.f, w = 0.f;
-  if (m != -INFINITY)
-    for (int s = 0; s < a.nparts; ++s) {
-      const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-      if (f == 0.f) continue;
+  for (int s = run; s < a.nparts; s += runs) {
+    const float2 t = ml[s];
+    const float f = __builtin_amdgcn_exp2f(t.x - mf);
+    l += f * t.y;
+    if (c < p.dh && f > 0.f) {
       const float4 v = *reinterpret_cast<const float4*>(a.part_o + (row * a.nparts + s) * p.dh + c);
-      l += f * ml[2 * s + 1]; x += f * v.x; y += f * v.y; z += f * v.z; w += f * v.w;
+      x += f * v.x; y += f * v.y; z += f * v.z; w += f * v.w;
     }
+  }
+  for (int o = lanes; o < 64; o <<= 1) {
+    l += __shfl_xor(l, o, 64); x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); z += __shfl_xor(z, o, 64); w += __shfl_xor(w, o, 64);
+  }
+  if (run) return;
   const float il = l > 0.f ? 1.f / l : 0.f;
   const int i = (int)(row % p.L), h = (int)(row / p.L % p.H);
   const long long b = row / p.L / p.H;
-  St<T>::st4((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, make_float4(x * il, y * il, z * il, w * il));
+  if (c < p.dh) St<T>::st4((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, make_float4(x * il, y * il, z * il, w * il));
   if (p.lse && c == 0) p.lse[row] = l > 0.f ? m + __log2f(l) : INFINITY;
 }
 
 // ---- which kernel, in how many parts ---------------------------------------------------------------------------------------------
-struct Plan { bool token; int nparts, per; long long blocks; int rt; int64_t split_ws, part_ws; };
+struct Plan { bool token; int nparts, per, rt, waves; long long blocks; int64_t split_ws, part_ws; };
 
 Plan plan(const smx_relpos_desc* d, const RP& p) {
   Plan w;
@@ -564,26 +584,37 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
   w.split_ws = 0;
   const int rows = p.G * p.L;
   w.rt = rows >= 8 ? 8 : rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
-  const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
-  // parts until the chip's 256 CUs have two blocks each, a part no shorter than 256 keys
-  long long np = (512 + base - 1) / base, most = (p.S + 255) / 256;
-  if (base >= 256) np = 1;
+  // two waves a block where four would leave CUs without a second block
+  // (fp32 storage, 65 to 96 columns: 64 keys a step for four waves would fill the LDS with one block)
+  w.waves = p.dh > 96 ? 4 : !d->bf16 && p.dh > 64 ? 2 : (long long)p.B * p.H * ((p.L + 127) / 128) >= 512 ? 4 : 2;
+  const int qb = 32 * w.waves;
+  const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + qb - 1) / qb);
+  // parts of the keys, none shorter than 256 keys, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four)
+  long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = (p.S + 255) / 256;
+  if (!w.token && base >= 256) np = 1;
   if (np > most) np = most;
   w.per = (int)(((p.S + np - 1) / np + 63) / 64 * 64);
   w.nparts = (p.S + w.per - 1) / w.per;
   w.blocks = base * w.nparts;
-  if (!w.token && !d->bf16) w.split_ws = split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh);
+  if (!w.token && !d->bf16) w.split_ws = 2 * split_bytes(p.B, p.Hkv, p.S, p.dh);
   w.part_ws = w.nparts > 1 ? (int64_t)p.B * p.H * p.L * w.nparts * (p.dh + 4) * 4 : 0;
   return w;
 }
 
-template <int DHP, int NL>
+template <int DHP, int NL, int NW>
 int tile_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
-  constexpr int TK = DHP == 128 ? 32 : 64;
-  const int fixed = 2 * 2 * NL * TK * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
-  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
-  SMX_LAUNCH((relpos_tile_kernel<DHP, NL>), dim3((unsigned)w.blocks), dim3(256), lds, st, p, a);
+  const int fixed = 2 * 2 * NL * STEP<DHP, NL, NW> * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
+  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL, NW>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
+  SMX_LAUNCH((relpos_tile_kernel<DHP, NL, NW>), dim3((unsigned)w.blocks), dim3(64 * NW), lds, st, p, a);
   return smx_launch_status();
+}
+template <int DHP>
+int tile_width(bool bf16, const RP& p, const Src& a, const Plan& w, hipStream_t st) {
+  if constexpr (DHP < 128)
+    if (w.waves == 2) return bf16 ? tile_launch<DHP, 1, 2>(p, a, w, st) : tile_launch<DHP, 2, 2>(p, a, w, st);
+  if (bf16) return tile_launch<DHP, 1, 4>(p, a, w, st);
+  if constexpr (DHP != 96) return tile_launch<DHP, 2, 4>(p, a, w, st);
+  return SMX_EINVAL;
 }
 
 template <typename T, int EPL, int LPK>
@@ -635,21 +666,21 @@ extern "C" int smx_attention_relpos(const smx_relpos_desc* d, void* stream) {
     else rc = token_width<bf16_t, 4>(p, a, w, st);
   } else {
     if (!d->bf16) {
-      ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.G, p.L, p.dh, false);
-      ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, 1, p.S, p.dh, true);
-      ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, 1, p.S, p.dh, true);
-      const Split all[3] = {a.q, a.k, a.v};
-      rc = split_launch(p, all, 3, st);
+      ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, p.S, p.dh, true);
+      ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, p.S, p.dh, true);
+      const Split both[2] = {a.k, a.v};
+      rc = split_launch(p, both, 2, st);
       if (rc != SMX_OK) return rc;
     }
     switch (dhp(p.dh)) {
-      case 32: rc = d->bf16 ? tile_launch<32, 1>(p, a, w, st) : tile_launch<32, 2>(p, a, w, st); break;
-      case 64: rc = d->bf16 ? tile_launch<64, 1>(p, a, w, st) : tile_launch<64, 2>(p, a, w, st); break;
-      default: rc = d->bf16 ? tile_launch<128, 1>(p, a, w, st) : tile_launch<128, 2>(p, a, w, st); break;
+      case 32: rc = tile_width<32>(d->bf16, p, a, w, st); break;
+      case 64: rc = tile_width<64>(d->bf16, p, a, w, st); break;
+      case 96: rc = tile_width<96>(d->bf16, p, a, w, st); break;
+      default: rc = tile_width<128>(d->bf16, p, a, w, st);
     }
   }
   if (rc != SMX_OK || w.nparts == 1) return rc;
-  const long long nj = ((long long)p.B * p.H * p.L * (p.dh / 4) + 255) / 256;
+  const long long nj = ((long long)p.B * p.H * p.L + 3) / 4;
   if (nj > 0x7fffffffLL) return SMX_EINVAL;
   if (d->bf16) SMX_LAUNCH(relpos_join_kernel<bf16_t>, dim3((unsigned)nj), dim3(256), 0, st, p, a);
   else SMX_LAUNCH(relpos_join_kernel<float>, dim3((unsigned)nj), dim3(256), 0, st, p, a);

@@ -15,6 +15,8 @@ using namespace relpos;
 struct Bwd {
   Split q, k, v, g;
   float* part;                                                   // [B][H][query blocks][map_n + 2 DPAD] sums of dS by distance
+  float* dkv;                                                    // [nparts][2][B][S][Hkv * dh]: dk and dv where the queries of a key block are split over blocks
+  int nparts;
 };
 constexpr int DPAD = 64;                                         // entries a 32 x 32 tile reaches beyond the map's ends while it touches the map
 
@@ -37,9 +39,9 @@ __device__ __forceinline__ void follow(float top, float& f, f32x16 (&acc)[N]) {
 constexpr float F0 = 1.2676506002282294e30f;                     // 2^100: before the first dS that is not zero
 
 // stage TK rows of four planes (h1, h2 of two operands) through registers
-template <int DHP, int NT>
+template <int DHP, int NW>
 struct Stage {
-  static constexpr int TK = DHP == 128 ? 32 : 64, RB = ROWB<DHP>, PLANE = TK * RB, CPR = DHP / 8, NCH = TK * CPR / NT;
+  static constexpr int NT = 64 * NW, TK = STEP<DHP, 2, NW>, RB = ROWB<DHP>, PLANE = TK * RB, CPR = DHP / 8, NCH = TK * CPR / NT;
   u32x4 reg[4][NCH];
   __device__ __forceinline__ void load(const Split& x, const Split& y, long long at) {
 #pragma unroll
@@ -59,17 +61,6 @@ struct Stage {
   }
 };
 
-// fragments of 32 rows of an operand that stays in registers
-template <int DHP>
-__device__ __forceinline__ void own_rows(u32x4 (&f)[DHP / 16][2], const Split& s, long long row, bool in) {
-  const long long at = row * DHP + ((threadIdx.x & 63) >> 5) * 8;
-#pragma unroll
-  for (int kk = 0; kk < DHP / 16; ++kk) {
-    f[kk][0] = in ? *reinterpret_cast<const u32x4*>(s.hi + at + kk * 16) : u32x4{0, 0, 0, 0};
-    f[kk][1] = in ? *reinterpret_cast<const u32x4*>(s.lo + at + kk * 16) : u32x4{0, 0, 0, 0};
-  }
-}
-
 // 32 x 32 product of staged rows (planes at t, t + PLANE) with owned rows
 template <int DHP>
 __device__ __forceinline__ f32x16 rows_times(const char* t, int plane, int r0, const u32x4 (&own)[DHP / 16][2]) {
@@ -82,54 +73,52 @@ __device__ __forceinline__ f32x16 rows_times(const char* t, int plane, int r0, c
   return a;
 }
 
-// dq and the sums of dS by distance.  A wave: 32 queries as columns, K and V staged 64 keys at a time (32 for DHP = 128); S^T = K Q^T, dP^T = V dO^T, then
+// dq and the sums of dS by distance.  A wave: 32 queries as columns, K and V staged 64 or 32 keys at a time; S^T = K Q^T, dP^T = V dO^T, then
 // dQ^T += K^T dS^T with dS^T from the registers.  dS by distance: in a tile that lies beyond the map's ends all pairs are of one entry, a
 // lane adds its own; elsewhere lane t collects the tile's diagonal key - query = t - 31 through lane permutes, register by register, and adds it to the
 // wave's table in LDS -- one lane an entry, tile after tile: a fixed order without atomics.
-template <int DHP>
-__global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(RP p, Bwd a) {
-  using ST = Stage<DHP, 256>;
-  constexpr int TK = ST::TK, NU = TK / 32, KS = DHP / 16, DT = DHP / 32;
+template <int DHP, int NW>
+__global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP p, Bwd a) {
+  using ST = Stage<DHP, NW>;
+  constexpr int TK = ST::TK, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, NT = 64 * NW, QB = 32 * NW;
   extern __shared__ __attribute__((aligned(16))) char sm[];
   const int nent = p.map_n + 2 * DPAD;
   float* lut = reinterpret_cast<float*>(sm + 4 * ST::PLANE);
-  float* dacc = lut + p.map_n + 2 * TABLE_PAD;                   // [4 waves][nent]
+  float* dacc = lut + p.map_n + 2 * TABLE_PAD;                   // [NW][nent]
   __shared__ unsigned long long seen;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
-  const int nq = (p.L + 127) / 128, up = (p.L + 63) & ~63;
+  const int nq = (p.L + QB - 1) / QB;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
   const int qb = nq - 1 - id % nq;
   id /= nq;
   const int h = id % p.H, b = id / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);
-  const int q0 = qb * 128 + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
+  const int q0 = qb * QB + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
   const int wlast = pos0 + min(q0 + 31, p.L - 1);
-  const int kend = p.causal ? min(n, pos0 + min(qb * 128 + 127, p.L - 1) + 1) : n;
+  const int kend = p.causal ? min(n, pos0 + min(qb * QB + QB - 1, p.L - 1) + 1) : n;
   const int ntiles = kend > 0 ? (kend + TK - 1) / TK : 0;
-  const long long row = ((long long)b * p.H + h) * p.L + qi, prow = ((long long)b * p.H + h) * up + qi;
+  const bool live = qi < p.L;
 
   fill_bias(lut, p, h);
-  for (int t = threadIdx.x; t < 4 * nent; t += 256) dacc[t] = 0.f;
+  for (int t = threadIdx.x; t < NW * nent; t += NT) dacc[t] = 0.f;
   dacc += wave * nent;
   const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
-  const int at2 = (b * p.Hkv + hk) * 2;
-  const float inv_k = a.k.pow2[at2 + 1], inv_v = a.v.pow2[at2 + 1], inv_g = a.g.pow2[at2 + 1];
-  const float sc = p.scale * LOG2E * a.q.pow2[at2 + 1] * inv_k;
-  const float lse = qi < p.L ? p.lse[row] : INFINITY;
-  const float D = qi < p.L ? a.g.dd[prow] * a.g.pow2[at2] * a.v.pow2[at2] : 0.f;       // in the units of dP's accumulators
+  const float lse = live ? p.lse[((long long)b * p.H + h) * p.L + qi] : INFINITY;
+  const float D = live ? a.g.dd[((long long)b * p.H + h) * ((p.L + 63) & ~63) + qi] : 0.f;
   u32x4 qf[KS][2], gf[KS][2];
-  own_rows<DHP>(qf, a.q, prow, qi < up);
-  own_rows<DHP>(gf, a.g, prow, qi < up);
+  const float sq = p.scale * LOG2E * own_rows<DHP>(qf, (const float*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh, live, p.dh);
+  const float sg = own_rows<DHP>(gf, p.d_o + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh, live, p.dh);
   f32x16 dq[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dq[t] = zero16();
   float f = F0, below = 0.f, above = 0.f;
+  Unit ku;
 
   ST st;
   unsigned long long sreg = 0;
-  const long long kv0 = ((long long)b * p.Hkv + hk) * ((p.S + 63) & ~63);
+  const long long tile0 = ((long long)b * p.Hkv + hk) * ((p.S + 63) >> 6);
   auto load_tile = [&](int key0) {
-    st.load(a.k, a.v, (kv0 + key0) * DHP);
+    st.load(a.k, a.v, (tile0 * 64 + key0) * DHP);
     if (wave == 0) {
       const int key = key0 + lane;
       sreg = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
@@ -146,6 +135,8 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
     if (t + 1 < ntiles) load_tile(key0 + TK);
     const unsigned long long left = seen;
     if (!left || q0 >= p.L || (p.causal && key0 > wlast)) continue;
+    const float inv_k = a.k.inv[tile0 + (key0 >> 6)], sc = sq * inv_k, sp = sg * a.v.inv[tile0 + (key0 >> 6)];
+    const float wk = exp2i(ku.enter(inv_k, dq));
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = rows_times<DHP>(sm, ST::PLANE, u * 32, qf);
@@ -175,7 +166,7 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
       }
       float ds[16], top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * ((r & 1 ? -dp[r] : dp[r]) - D); top = fmaxf(top, fabsf(ds[r])); }
+      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * fmaf(dp[r], r & 1 ? -sp : sp, -D); top = fmaxf(top, fabsf(ds[r])); }
       if (lo || hi) {
         float sum = 0.f;
 #pragma unroll
@@ -197,8 +188,9 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
         dacc[DPAD + e0 + lane - 31] += sum;                      // (lane 63: no diagonal of its own, adds 0)
       }
       follow(top, f, dq);
+      const float fk = f * wk;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= f;
+      for (int r = 0; r < 16; ++r) ds[r] *= fk;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2];
@@ -218,9 +210,14 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
   __syncthreads();
   dacc -= wave * nent;
   float* part = a.part + (((long long)b * p.H + h) * nq + qb) * nent;
-  for (int t = threadIdx.x; t < nent; t += 256) part[t] = ((dacc[t] + dacc[nent + t]) + (dacc[2 * nent + t] + dacc[3 * nent + t])) * inv_g * inv_v;
-  if (qi >= p.L) return;
-  const float w1 = inv_g * inv_k, w2 = inv_v * p.scale, fi = 1.f / f;
+  for (int t = threadIdx.x; t < nent; t += NT) {
+    float x = dacc[t];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) x += dacc[w * nent + t];
+    part[t] = x;
+  }
+  if (!live) return;
+  const float w = ku.inv * p.scale, fi = 1.f / f;
   float* DQ = p.dq + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -229,71 +226,75 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_q_kernel(R
       const int c = d * 32 + 8 * g + 4 * hh;
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * g + e] * fi * w1 * w2;
+      for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * g + e] * fi * w;
       if (c < p.dh) *reinterpret_cast<float4*>(DQ + c) = make_float4(x[0], x[1], x[2], x[3]);
     }
 }
 
-// dk and dv.  A wave: 32 keys as columns; Q and dO of the heads that share them staged 64 queries at a time (32 for DHP = 128); S = Q K^T, dP = dO V^T,
-// dV^T += dO^T P, dK^T += Q^T dS.  P carries 2^14.
-template <int DHP>
-__global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
-  using ST = Stage<DHP, 256>;
-  constexpr int TQ = ST::TK, NU = TQ / 32, KS = DHP / 16, DT = DHP / 32;
+// dk and dv.  A wave: 32 keys as columns; Q and dO of the heads that share them staged 64 or 32 queries at a time; S = Q K^T, dP = dO V^T, dV^T += dO^T P,
+// dK^T += Q^T dS.  P carries 2^14.  Few key blocks: a part of their queries (tiles of all the heads) a block, joined by relpos_bwd_sum_kernel.
+template <int DHP, int NW>
+__global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
+  using ST = Stage<DHP, NW>;
+  constexpr int TQ = ST::TK, NU = TQ / 32, KS = DHP / 16, DT = DHP / 32, KB = 32 * NW;
   extern __shared__ __attribute__((aligned(16))) char sm[];
-  float* rl = reinterpret_cast<float*>(sm + 4 * ST::PLANE);      // the tile's lse - 14
+  float* rl = reinterpret_cast<float*>(sm + 4 * ST::PLANE);      // the tile's lse
   float* rd = rl + 64;                                           // and D
   float* lut = rd + 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
-  const int nk = (p.S + 127) / 128, up = (p.L + 63) & ~63;
+  const int nk = (p.S + KB - 1) / KB, qt = (p.L + 63) >> 6;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
+  const int part = id % a.nparts;
+  id /= a.nparts;
   const int kb = id % nk;
   id /= nk;
   const int hk = id % p.Hkv, b = id / p.Hkv;
   const int n = p.keys(b), pos0 = p.pos0(n);
-  const int k0 = kb * 128 + wave * 32, key = k0 + (lane & 31);
-  const int ups = (p.S + 63) & ~63;
-  const long long krow = ((long long)b * p.Hkv + hk) * ups + key;
-  const int at2 = (b * p.Hkv + hk) * 2;
-  const float inv_q = a.q.pow2[at2 + 1], inv_v = a.v.pow2[at2 + 1], inv_g = a.g.pow2[at2 + 1], pg = a.g.pow2[at2], pv = a.v.pow2[at2];
-  const float sc = p.scale * LOG2E * inv_q * a.k.pow2[at2 + 1];
+  const int k0 = kb * KB + wave * 32, key = k0 + (lane & 31);
+  const bool in = key < n && !(p.mask && p.mask[(long long)b * p.S + key]);
   u32x4 kf[KS][2], vf[KS][2];
-  own_rows<DHP>(kf, a.k, krow, key < ups);
-  own_rows<DHP>(vf, a.v, krow, key < ups);
+  const float sk = p.scale * LOG2E * own_rows<DHP>(kf, (const float*)p.k + b * p.k_bs + (long long)key * p.ldk + hk * p.dh, in, p.dh);
+  const float sv = own_rows<DHP>(vf, (const float*)p.v + b * p.v_bs + (long long)key * p.ldv + hk * p.dh, in, p.dh);
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = zero16();
   float f = F0;
-  const float sign = key & 1 ? -1.f : 1.f;                       // V's odd rows are negated
+  Unit qu, gu;
   // causal: the first query that stands at this block's first key or behind it
-  const int t0 = p.causal ? max(0, kb * 128 - pos0) / TQ : 0, t1 = kb * 128 < n ? (p.L + TQ - 1) / TQ : 0;
-  const int per = max(0, t1 - t0), ntiles = per * p.G;
+  const int t0 = p.causal ? max(0, kb * KB - pos0) / TQ : 0, t1 = kb * KB < n ? (p.L + TQ - 1) / TQ : 0;
+  const int per = max(0, t1 - t0);
+  const long long all = (long long)per * p.G;
+  const int first = (int)(all * part / a.nparts), last = (int)(all * (part + 1) / a.nparts);
   ST st;
   float lreg = 0.f, dreg = 0.f;
   auto load_tile = [&](int t) {
-    const int h = hk * p.G + t / per, i0 = (t0 + t % per) * TQ, i = i0 + threadIdx.x;
-    const long long r = (long long)b * p.H + h;
-    st.load(a.q, a.g, (r * up + i0) * DHP);
+    const int i0 = (t0 + t % per) * TQ, i = i0 + threadIdx.x;
+    const long long r = (long long)b * p.H + hk * p.G + t / per;
+    st.load(a.q, a.g, (r * qt * 64 + i0) * DHP);
     if (threadIdx.x < TQ) {
-      lreg = i < p.L ? p.lse[r * p.L + i] - 14.f : INFINITY;
-      dreg = i < p.L ? a.g.dd[r * up + i] * pg * pv : 0.f;
+      lreg = i < p.L ? p.lse[r * p.L + i] : INFINITY;
+      dreg = i < p.L ? a.g.dd[r * qt * 64 + i] : 0.f;
     }
   };
-  if (ntiles > 0) load_tile(0);
+  if (first < last) load_tile(first);
   float first_bias = 0.f, last_bias = 0.f;
-  for (int t = 0; t < ntiles; ++t) {
+  for (int t = first; t < last; ++t) {
     const int h = hk * p.G + t / per, i0 = (t0 + t % per) * TQ;
     __syncthreads();
     st.store(sm);
     if (threadIdx.x < TQ) { rl[threadIdx.x] = lreg; rd[threadIdx.x] = dreg; }
-    if (t % per == 0) {
+    if (t == first || t % per == 0) {
       fill_bias(lut, p, h);
       first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E;
       last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
     }
     __syncthreads();
-    if (t + 1 < ntiles) load_tile(t + 1);
+    if (t + 1 < last) load_tile(t + 1);
     if (k0 >= n || (p.causal && pos0 + i0 + TQ - 1 < k0)) continue;
+    const long long tile = ((long long)b * p.H + h) * qt + (i0 >> 6);
+    const float inv_q = a.q.inv[tile], inv_g = a.g.inv[tile], sc = sk * inv_q, sp = sv * inv_g;
+    const int lg = 14 + gu.enter(inv_g, dv);                     // P carries 2^lg
+    const float ig = exp2i(-lg), wq = exp2i(qu.enter(inv_q, dk)) * ig;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = rows_times<DHP>(sm, ST::PLANE, u * 32, kf);
@@ -307,13 +308,13 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(
       }
       const int q0 = pos0 + i0 + u * 32, e0 = k0 - q0 - p.map_lo;  // entry of the first key and the tile's first query; the others: + key - query
       if (e0 + 31 <= 0 || e0 - 31 >= p.map_n - 1) {
-        const float c = e0 + 31 <= 0 ? first_bias : last_bias;
+        const float c = (e0 + 31 <= 0 ? first_bias : last_bias) + lg;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, c - lv[r]));
       } else {
         const float* lp = lut + TABLE_PAD + e0 + (lane & 31) - 4 * hh;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, lp[-crow(r)] - lv[r]));
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, lp[-crow(r)] - (lv[r] - lg)));
       }
       if (p.causal && k0 + 31 > q0) {
         const int d = key - q0 - 4 * hh;
@@ -323,10 +324,11 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(
       }
       float ds[16], top = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * fmaf(dp[r], sign, -dd[r]); top = fmaxf(top, fabsf(ds[r])); }
-      follow(top, f, dk);
+      for (int r = 0; r < 16; ++r) { ds[r] = s[r] * fmaf(dp[r], sp, -dd[r]); top = fmaxf(top, fabsf(ds[r])); }
+      follow(top * ig, f, dk);
+      const float fq = f * wq;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= f;
+      for (int r = 0; r < 16; ++r) ds[r] *= fq;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2], sf[2];
@@ -337,96 +339,161 @@ __global__ __launch_bounds__(256, DHP == 128 ? 1 : 2) void relpos_bwd_kv_kernel(
         for (int d = 0; d < DT; ++d) {
           const u32x4 gt[2] = {col_frag<DHP>(sm + 2 * ST::PLANE, u * 32 + g * 16, d), col_frag<DHP>(sm + 3 * ST::PLANE, u * 32 + g * 16, d)};
           dv[d] = mfma_levels<2>(gt, pf, dv[d]);
-          const u32x4 qt[2] = {col_frag<DHP>(sm, u * 32 + g * 16, d), col_frag<DHP>(sm + ST::PLANE, u * 32 + g * 16, d)};
-          dk[d] = mfma_levels<2>(qt, sf, dk[d]);
+          const u32x4 qt2[2] = {col_frag<DHP>(sm, u * 32 + g * 16, d), col_frag<DHP>(sm + ST::PLANE, u * 32 + g * 16, d)};
+          dk[d] = mfma_levels<2>(qt2, sf, dk[d]);
         }
       }
     }
   }
   if (key >= p.S) return;
-  const bool out = key >= n || (p.mask && p.mask[(long long)b * p.S + key]);       // nobody sees it: what its column holds is dropped
-  const float w1 = inv_g * inv_q, w2 = inv_v * p.scale, fi = 0x1p-14f / f, wv = inv_g * 0x1p-14f;
-  const long long at = ((long long)b * p.S + key) * p.Hkv * p.dh + hk * p.dh;
+  const float w = qu.inv * p.scale, fi = 1.f / f, wv = gu.inv * 0x1p-14f;
+  const long long at = ((long long)b * p.S + key) * p.Hkv * p.dh + hk * p.dh, size = (long long)p.B * p.S * p.Hkv * p.dh;
+  float* DK = a.nparts > 1 ? a.dkv + part * 2 * size : p.dk;
+  float* DV = a.nparts > 1 ? a.dkv + (part * 2 + 1) * size : p.dv;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = d * 32 + 8 * g + 4 * hh;
-      float x[4], y[4];
+      float x[4], y[4];                                          // a key that nobody sees: what its column holds is dropped
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { x[e] = out ? 0.f : dk[d][4 * g + e] * fi * w1 * w2; y[e] = out ? 0.f : dv[d][4 * g + e] * wv; }
+      for (int e = 0; e < 4; ++e) { x[e] = in ? dk[d][4 * g + e] * fi * w : 0.f; y[e] = in ? dv[d][4 * g + e] * wv : 0.f; }
       if (c < p.dh) {
-        *reinterpret_cast<float4*>(p.dk + at + c) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(p.dv + at + c) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(DK + at + c) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(DV + at + c) = make_float4(y[0], y[1], y[2], y[3]);
       }
     }
 }
 
-// dtable[bucket][h] += the distances of that bucket: a block a head, the query blocks' sums in four fixed runs, then bucket by bucket
+// dk and dv from their parts, in order
+__global__ __launch_bounds__(256) void relpos_bwd_sum_kernel(const float* __restrict__ dkv, float* __restrict__ dk, float* __restrict__ dv, long long size, int nparts) {
+  const long long i = (blockIdx.x * 256LL + threadIdx.x) * 4;
+  if (i >= size) return;
+  const int which = blockIdx.y;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int t = 0; t < nparts; ++t) {
+    const float4 x = *reinterpret_cast<const float4*>(dkv + (t * 2 + which) * size + i);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  *reinterpret_cast<float4*>((which ? dv : dk) + i) = s;
+}
+
+// dtable[bucket][h] += the distances of that bucket: a block a head, the query blocks' sums in four fixed runs, then a wave a bucket
 __global__ __launch_bounds__(1024) void relpos_bwd_table_kernel(RP p, const float* __restrict__ part, int nq) {
   __shared__ float ent[4][MAP_MAX + 2 * DPAD];
-  const int h = blockIdx.x, nent = p.map_n + 2 * DPAD, run = threadIdx.x >> 8;
-  const long long rows = (long long)p.B * nq, r0 = rows * run / 4, r1 = rows * (run + 1) / 4;
+  __shared__ unsigned short of[MAP_MAX + 2 * DPAD];
+  const int h = blockIdx.x, nent = p.map_n + 2 * DPAD, run = threadIdx.x >> 8, lane = threadIdx.x & 63;
+  const int rows = p.B * nq, r0 = (int)((long long)rows * run / 4), r1 = (int)((long long)rows * (run + 1) / 4);
+  for (int e = threadIdx.x; e < nent; e += 1024) of[e] = (unsigned short)p.map[p.entry(e - DPAD + p.map_lo)];
   for (int e = threadIdx.x & 255; e < nent; e += 256) {
     float s = 0.f;
-    for (long long r = r0; r < r1; ++r) s += part[((r / nq * p.H + h) * nq + r % nq) * nent + e];
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) s += part[(((long long)(r / nq) * p.H + h) * nq + r % nq) * nent + e];
     ent[run][e] = s;
   }
   __syncthreads();
-  for (int bucket = threadIdx.x; bucket < p.nb; bucket += 1024) {
+  for (int bucket = threadIdx.x >> 6; bucket < p.nb; bucket += 16) {
     float s = 0.f;
-    for (int e = 0; e < nent; ++e)
-      if (p.map[p.entry(e - DPAD + p.map_lo)] == bucket) s += (ent[0][e] + ent[1][e]) + (ent[2][e] + ent[3][e]);
-    p.dtable[(long long)bucket * p.H + h] += s;
+    for (int e = lane; e < nent; e += 64)
+      if (of[e] == bucket) s += (ent[0][e] + ent[1][e]) + (ent[2][e] + ent[3][e]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) p.dtable[(long long)bucket * p.H + h] += s;
   }
 }
 
-template <int DHP>
-int launch(const RP& p, const Bwd& a, hipStream_t st) {
-  const int nq = (p.L + 127) / 128, nk = (p.S + 127) / 128;
-  const long long qb = (long long)p.B * p.H * nq, kb = (long long)p.B * p.Hkv * nk;
-  if (qb > 0x7fffffffLL || kb > 0x7fffffffLL) return SMX_EINVAL;
-  const int planes = 4 * Stage<DHP, 256>::PLANE, lq = 4 * (p.map_n + 2 * TABLE_PAD + 4 * (p.map_n + 2 * DPAD)), lk = 4 * (128 + p.map_n + 2 * TABLE_PAD);
-  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_q_kernel<DHP>, planes + 4 * (MAP_MAX + 2 * TABLE_PAD + 4 * (MAP_MAX + 2 * DPAD))));
-  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_kv_kernel<DHP>, planes + 4 * (128 + MAP_MAX + 2 * TABLE_PAD)));
-  SMX_LAUNCH(relpos_bwd_q_kernel<DHP>, dim3((unsigned)qb), dim3(256), planes + lq, st, p, a);
-  SMX_LAUNCH(relpos_bwd_kv_kernel<DHP>, dim3((unsigned)kb), dim3(256), planes + lk, st, p, a);
-  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(p.H), dim3(1024), 0, st, p, (const float*)a.part, nq);
+// Four waves a block where that still gives the chip's 256 CUs two blocks each, else two.  Key blocks: with a causal rule they differ (the first key meets all
+// queries, the last one), and few kv heads give few of them: parts of the queries until there are about four blocks a CU, none shorter than four tiles;
+// the parts' dk and dv are written and read once more.
+struct Plan { int qw, kw, nparts; long long qblocks, kblocks; int64_t part, dd, dkv, total; };
+
+Plan plan(const RP& p) {
+  Plan w;
+  const bool wide = p.dh > 96;
+  w.qw = wide || (long long)p.B * p.H * ((p.L + 127) / 128) >= 512 ? 4 : 2;
+  w.qblocks = (long long)p.B * p.H * ((p.L + 32 * w.qw - 1) / (32 * w.qw));
+  w.kw = wide || (long long)p.B * p.Hkv * ((p.S + 127) / 128) >= 256 ? 4 : 2;
+  const long long base = (long long)p.B * p.Hkv * ((p.S + 32 * w.kw - 1) / (32 * w.kw));
+  const long long tiles = (long long)p.G * ((p.L + 63) / 64);
+  long long np = (1024 + base - 1) / base, most = tiles / 4;
+  if (base >= 1024 || (!p.causal && base >= 512)) np = 1;
+  if (np > most) np = most;
+  if (np > 8) np = 8;
+  w.nparts = np < 1 ? 1 : (int)np;
+  w.kblocks = base * w.nparts;
+  w.part = ((int64_t)p.B * p.H * ((p.L + 32 * w.qw - 1) / (32 * w.qw)) * (p.map_n + 2 * DPAD) * 4 + 15) / 16 * 16;
+  w.dd = (int64_t)p.B * p.H * up64(p.L) * 4;
+  w.dkv = w.nparts > 1 ? (int64_t)w.nparts * 2 * p.B * p.S * p.Hkv * p.dh * 4 : 0;
+  w.total = 2 * split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh) + w.part + w.dd + w.dkv;
+  return w;
+}
+
+template <int DHP, int NW>
+int launch_q(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
+  const int planes = 4 * Stage<DHP, NW>::PLANE, lds = planes + 4 * (p.map_n + 2 * TABLE_PAD + NW * (p.map_n + 2 * DPAD));
+  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_bwd_q_kernel<DHP, NW>), planes + 4 * (MAP_MAX + 2 * TABLE_PAD + NW * (MAP_MAX + 2 * DPAD))));
+  SMX_LAUNCH((relpos_bwd_q_kernel<DHP, NW>), dim3((unsigned)w.qblocks), dim3(64 * NW), lds, st, p, a);
+  return smx_launch_status();
+}
+template <int DHP, int NW>
+int launch_kv(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
+  const int planes = 4 * Stage<DHP, NW>::PLANE, lds = planes + 4 * (128 + p.map_n + 2 * TABLE_PAD);
+  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_bwd_kv_kernel<DHP, NW>), planes + 4 * (128 + MAP_MAX + 2 * TABLE_PAD)));
+  SMX_LAUNCH((relpos_bwd_kv_kernel<DHP, NW>), dim3((unsigned)w.kblocks), dim3(64 * NW), lds, st, p, a);
   return smx_launch_status();
 }
 
-int64_t part_bytes(const RP& p) { return ((int64_t)p.B * p.H * ((p.L + 127) / 128) * (p.map_n + 2 * DPAD) * 4 + 15) / 16 * 16; }
+template <int DHP>
+int launch(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
+  int rc;
+  if constexpr (DHP < 128) {
+    rc = w.qw == 4 ? launch_q<DHP, 4>(p, a, w, st) : launch_q<DHP, 2>(p, a, w, st);
+    if (rc == SMX_OK) rc = w.kw == 4 ? launch_kv<DHP, 4>(p, a, w, st) : launch_kv<DHP, 2>(p, a, w, st);
+  } else {
+    rc = launch_q<DHP, 4>(p, a, w, st);
+    if (rc == SMX_OK) rc = launch_kv<DHP, 4>(p, a, w, st);
+  }
+  return rc;
+}
 
 }  // namespace
 
 extern "C" int64_t smx_attention_relpos_bwd_ws_bytes(const smx_relpos_desc* d) {
   RP p;
-  if (check(d, p, true) != SMX_OK) return -1;
-  return 2 * split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh) + part_bytes(p) + (int64_t)p.B * p.H * up64(p.L) * 4;
+  return check(d, p, true) == SMX_OK ? plan(p).total : -1;
 }
 
 extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stream) {
   RP p;
   int rc = check(d, p, true);
   if (rc != SMX_OK) return rc;
-  if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < smx_attention_relpos_bwd_ws_bytes(d) || p.H > 65535) return SMX_EINVAL;
+  const Plan w = plan(p);
+  const long long size = (long long)p.B * p.S * p.Hkv * p.dh, sums = (size / 4 + 255) / 256;
+  if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < w.total || w.qblocks > 0x7fffffffLL || w.kblocks > 0x7fffffffLL || sums > 0x7fffffffLL) return SMX_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   Bwd a;
   char* ws = (char*)d->ws;
-  ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.G, p.L, p.dh, false);
-  ws = split_setup(a.g, ws, p.d_o, (long long)p.L * p.H * p.dh, p.H * p.dh, p.B, p.H, p.G, p.L, p.dh, false);
-  ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, 1, p.S, p.dh, true);
-  ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, 1, p.S, p.dh, true);
+  ws = split_setup(a.q, ws, (const float*)p.q, p.q_bs, p.ldq, p.B, p.H, p.L, p.dh, false);
+  ws = split_setup(a.g, ws, p.d_o, (long long)p.L * p.H * p.dh, p.H * p.dh, p.B, p.H, p.L, p.dh, false);
+  ws = split_setup(a.k, ws, (const float*)p.k, p.k_bs, p.ldk, p.B, p.Hkv, p.S, p.dh, true);
+  ws = split_setup(a.v, ws, (const float*)p.v, p.v_bs, p.ldv, p.B, p.Hkv, p.S, p.dh, true);
   a.v.flip = 1;
   a.part = (float*)ws;
   a.g.o = (const float*)p.o;
-  a.g.dd = (float*)(ws + part_bytes(p));
+  a.g.dd = (float*)(ws + w.part);
+  a.dkv = (float*)(ws + w.part + w.dd);
+  a.nparts = w.nparts;
   const Split all[4] = {a.q, a.g, a.k, a.v};
   rc = split_launch(p, all, 4, st);
   if (rc != SMX_OK) return rc;
   switch (dhp(p.dh)) {
-    case 32: return launch<32>(p, a, st);
-    case 64: return launch<64>(p, a, st);
-    default: return launch<128>(p, a, st);
+    case 32: rc = launch<32>(p, a, w, st); break;
+    case 64: rc = launch<64>(p, a, w, st); break;
+    case 96: rc = launch<96>(p, a, w, st); break;
+    default: rc = launch<128>(p, a, w, st);
   }
+  if (rc != SMX_OK) return rc;
+  if (w.nparts > 1) SMX_LAUNCH(relpos_bwd_sum_kernel, dim3((unsigned)sums, 2), dim3(256), 0, st, (const float*)a.dkv, p.dk, p.dv, size, w.nparts);
+  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(p.H), dim3(1024), 0, st, p, (const float*)a.part, (p.L + 32 * w.qw - 1) / (32 * w.qw));
+  return smx_launch_status();
 }
