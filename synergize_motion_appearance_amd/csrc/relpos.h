@@ -177,9 +177,8 @@ struct Unit {
 };
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// keys (queries) a step and the block's waves: 64 rows where four waves stage them, 32 for two waves or where two operands of 128 columns in two halves each
-// would not leave room for a second block on a CU
-template <int DHP, int NL, int NW> constexpr int STEP = NL == 1 ? 64 : NW == 2 || DHP == 128 ? 32 : 64;
+// keys (queries) a step: 64, or 32 where two operands of 128 columns in two halves each would not leave room for a second block on a CU
+template <int DHP, int NL> constexpr int STEP = NL == 2 && DHP == 128 ? 32 : 64;
 
 // Work order: consecutive block ids go to the 8 XCDs in turn; this gives each XCD a run of consecutive work items, so that the blocks that read the
 // same keys share an L2.

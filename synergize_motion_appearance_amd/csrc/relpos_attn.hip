@@ -121,6 +121,9 @@ namespace {
 using namespace relpos;
 
 // ---- queries in tiles ----------------------------------------------------------------------------------------------------------
+// two stages of keys in turn, one barrier a step; one where two would leave a CU with one block (fp32 storage, 65 to 96 columns: 106 KB)
+template <int DHP, int NL> constexpr int BUFFERS = NL == 2 && DHP == 96 ? 1 : 2;
+
 // where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage q and the planes of k and v; parts: m, l [row][part], o
 // [row][part][dh] when the keys are split
 struct Src {
@@ -135,17 +138,18 @@ struct Src {
 // Weights are 2^(s - mo), mo finite and followed only when a row outgrows it by 2^8 (and at its first key): the scores leave the products through one fma,
 // and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
-template <int DHP, int NL, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void relpos_tile_kernel(RP p, Src a) {
-  constexpr int TK = STEP<DHP, NL, NW>, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>, NT = 64 * NW;
+template <int DHP, int NL>
+__global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
+  constexpr int TK = STEP<DHP, NL>, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>, NT = 256;
   constexpr int PLANE = TK * RB, STAGE = 2 * NL * PLANE;         // K levels, V levels
+  constexpr int NBUF = BUFFERS<DHP, NL>;
   constexpr int CPR = DHP / 8, NCH = TK * CPR / NT;              // 16-byte chunks of a row; of a plane, a thread
   constexpr float PSH = NL == 2 ? 6.f : 0.f;
-  extern __shared__ __attribute__((aligned(16))) char sm[];      // two stages, bias, masks
-  float* lut = reinterpret_cast<float*>(sm + 2 * STAGE);
-  unsigned long long* seen = reinterpret_cast<unsigned long long*>(sm + 2 * STAGE + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16);
+  extern __shared__ __attribute__((aligned(16))) char sm[];      // stages, bias, masks
+  float* lut = reinterpret_cast<float*>(sm + NBUF * STAGE);
+  unsigned long long* seen = reinterpret_cast<unsigned long long*>(sm + NBUF * STAGE + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
-  constexpr int QB = 32 * NW;
+  constexpr int QB = 128;
   const int nq = (p.L + QB - 1) / QB;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
   const int qb = nq - 1 - id % nq;                               // causal: the longest rows first
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(64 * NW, 2) void relpos_tile_kernel(RP p, Src a) {
   if (ntiles > 0) { load_tile(kbeg); store_tile(0); }
   __syncthreads();
   for (int t = 0; t < ntiles; ++t) {
-    const int buf = t & 1, key0 = kbeg + t * TK;
+    const int buf = NBUF == 2 ? t & 1 : 0, key0 = kbeg + t * TK;
     if (t + 1 < ntiles) load_tile(key0 + TK);
     char* st = sm + buf * STAGE;
     const unsigned long long left = seen[buf];
@@ -330,7 +334,8 @@ __global__ __launch_bounds__(64 * NW, 2) void relpos_tile_kernel(RP p, Src a) {
       }
       l = fmaf(lt, exp2i(-(int)lw), l);
     }
-    if (t + 1 < ntiles) store_tile(buf ^ 1);
+    if (NBUF == 1) __syncthreads();
+    if (t + 1 < ntiles) store_tile(NBUF == 2 ? buf ^ 1 : 0);
     __syncthreads();
   }
   if (qi >= p.L) return;
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
 }
 
 // ---- which kernel, in how many parts ---------------------------------------------------------------------------------------------
-struct Plan { bool token; int nparts, per, rt, waves; long long blocks; int64_t split_ws, part_ws; };
+struct Plan { bool token; int nparts, per, rt; long long blocks; int64_t split_ws, part_ws; };
 
 Plan plan(const smx_relpos_desc* d, const RP& p) {
   Plan w;
@@ -584,14 +589,9 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
   w.split_ws = 0;
   const int rows = p.G * p.L;
   w.rt = rows >= 8 ? 8 : rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
-  // two waves a block where four would leave CUs without a second block
-  // (fp32 storage, 65 to 96 columns: 64 keys a step for four waves would fill the LDS with one block)
-  w.waves = p.dh > 96 ? 4 : !d->bf16 && p.dh > 64 ? 2 : (long long)p.B * p.H * ((p.L + 127) / 128) >= 512 ? 4 : 2;
-  const int qb = 32 * w.waves;
-  const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + qb - 1) / qb);
+  const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
   // parts of the keys, none shorter than 256 keys, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four)
   long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = (p.S + 255) / 256;
-  if (!w.token && base >= 256) np = 1;
   if (np > most) np = most;
   w.per = (int)(((p.S + np - 1) / np + 63) / 64 * 64);
   w.nparts = (p.S + w.per - 1) / w.per;
@@ -601,20 +601,12 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
   return w;
 }
 
-template <int DHP, int NL, int NW>
+template <int DHP, int NL>
 int tile_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
-  const int fixed = 2 * 2 * NL * STEP<DHP, NL, NW> * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
-  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL, NW>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
-  SMX_LAUNCH((relpos_tile_kernel<DHP, NL, NW>), dim3((unsigned)w.blocks), dim3(64 * NW), lds, st, p, a);
+  const int fixed = BUFFERS<DHP, NL> * 2 * NL * STEP<DHP, NL> * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
+  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
+  SMX_LAUNCH((relpos_tile_kernel<DHP, NL>), dim3((unsigned)w.blocks), dim3(256), lds, st, p, a);
   return smx_launch_status();
-}
-template <int DHP>
-int tile_width(bool bf16, const RP& p, const Src& a, const Plan& w, hipStream_t st) {
-  if constexpr (DHP < 128)
-    if (w.waves == 2) return bf16 ? tile_launch<DHP, 1, 2>(p, a, w, st) : tile_launch<DHP, 2, 2>(p, a, w, st);
-  if (bf16) return tile_launch<DHP, 1, 4>(p, a, w, st);
-  if constexpr (DHP != 96) return tile_launch<DHP, 2, 4>(p, a, w, st);
-  return SMX_EINVAL;
 }
 
 template <typename T, int EPL, int LPK>
@@ -673,10 +665,10 @@ extern "C" int smx_attention_relpos(const smx_relpos_desc* d, void* stream) {
       if (rc != SMX_OK) return rc;
     }
     switch (dhp(p.dh)) {
-      case 32: rc = tile_width<32>(d->bf16, p, a, w, st); break;
-      case 64: rc = tile_width<64>(d->bf16, p, a, w, st); break;
-      case 96: rc = tile_width<96>(d->bf16, p, a, w, st); break;
-      default: rc = tile_width<128>(d->bf16, p, a, w, st);
+      case 32: rc = d->bf16 ? tile_launch<32, 1>(p, a, w, st) : tile_launch<32, 2>(p, a, w, st); break;
+      case 64: rc = d->bf16 ? tile_launch<64, 1>(p, a, w, st) : tile_launch<64, 2>(p, a, w, st); break;
+      case 96: rc = d->bf16 ? tile_launch<96, 1>(p, a, w, st) : tile_launch<96, 2>(p, a, w, st); break;
+      default: rc = d->bf16 ? tile_launch<128, 1>(p, a, w, st) : tile_launch<128, 2>(p, a, w, st);
     }
   }
   if (rc != SMX_OK || w.nparts == 1) return rc;

@@ -14,9 +14,9 @@ using namespace relpos;
 
 struct Bwd {
   Split q, k, v, g;
-  float* part;                                                   // [B][H][query blocks][map_n + 2 DPAD] sums of dS by distance
-  float* dkv;                                                    // [nparts][2][B][S][Hkv * dh]: dk and dv where the queries of a key block are split over blocks
-  int nparts;
+  float* part;                                                   // [B][H][query blocks * qparts][map_n + 2 DPAD] sums of dS by distance
+  float* dqp; float* dkv;                                        // [qparts][B][L][H * dh] dq, [kparts][2][B][S][Hkv * dh] dk and dv, where the other side is split
+  int qparts, kparts;
 };
 constexpr int DPAD = 64;                                         // entries a 32 x 32 tile reaches beyond the map's ends while it touches the map
 
@@ -39,9 +39,9 @@ __device__ __forceinline__ void follow(float top, float& f, f32x16 (&acc)[N]) {
 constexpr float F0 = 1.2676506002282294e30f;                     // 2^100: before the first dS that is not zero
 
 // stage TK rows of four planes (h1, h2 of two operands) through registers
-template <int DHP, int NW>
+template <int DHP>
 struct Stage {
-  static constexpr int NT = 64 * NW, TK = STEP<DHP, 2, NW>, RB = ROWB<DHP>, PLANE = TK * RB, CPR = DHP / 8, NCH = TK * CPR / NT;
+  static constexpr int NT = 256, TK = STEP<DHP, 2>, RB = ROWB<DHP>, PLANE = TK * RB, CPR = DHP / 8, NCH = TK * CPR / NT;
   u32x4 reg[4][NCH];
   __device__ __forceinline__ void load(const Split& x, const Split& y, long long at) {
 #pragma unroll
@@ -77,10 +77,10 @@ __device__ __forceinline__ f32x16 rows_times(const char* t, int plane, int r0, c
 // dQ^T += K^T dS^T with dS^T from the registers.  dS by distance: in a tile that lies beyond the map's ends all pairs are of one entry, a
 // lane adds its own; elsewhere lane t collects the tile's diagonal key - query = t - 31 through lane permutes, register by register, and adds it to the
 // wave's table in LDS -- one lane an entry, tile after tile: a fixed order without atomics.
-template <int DHP, int NW>
-__global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP p, Bwd a) {
-  using ST = Stage<DHP, NW>;
-  constexpr int TK = ST::TK, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, NT = 64 * NW, QB = 32 * NW;
+template <int DHP>
+__global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP p, Bwd a) {
+  using ST = Stage<DHP>;
+  constexpr int TK = ST::TK, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, NW = 4, NT = 256, QB = 128;
   extern __shared__ __attribute__((aligned(16))) char sm[];
   const int nent = p.map_n + 2 * DPAD;
   float* lut = reinterpret_cast<float*>(sm + 4 * ST::PLANE);
@@ -89,6 +89,8 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kerne
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nq = (p.L + QB - 1) / QB;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
+  const int part = id % a.qparts;
+  id /= a.qparts;
   const int qb = nq - 1 - id % nq;
   id /= nq;
   const int h = id % p.H, b = id / p.H, hk = h / p.G;
@@ -96,7 +98,8 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kerne
   const int q0 = qb * QB + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
   const int wlast = pos0 + min(q0 + 31, p.L - 1);
   const int kend = p.causal ? min(n, pos0 + min(qb * QB + QB - 1, p.L - 1) + 1) : n;
-  const int ntiles = kend > 0 ? (kend + TK - 1) / TK : 0;
+  const int all = kend > 0 ? (kend + TK - 1) / TK : 0;
+  const int first = (int)((long long)all * part / a.qparts), last = (int)((long long)all * (part + 1) / a.qparts);
   const bool live = qi < p.L;
 
   fill_bias(lut, p, h);
@@ -124,15 +127,15 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kerne
       sreg = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
     }
   };
-  if (ntiles > 0) load_tile(0);
+  if (first < last) load_tile(first * TK);
   const unsigned long long ALL = TK == 64 ? ~0ull : 0xffffffffull;
-  for (int t = 0; t < ntiles; ++t) {
+  for (int t = first; t < last; ++t) {
     const int key0 = t * TK;
     __syncthreads();                                             // the tile before has been read
     st.store(sm);
     if (threadIdx.x == 0) seen = sreg;
     __syncthreads();
-    if (t + 1 < ntiles) load_tile(key0 + TK);
+    if (t + 1 < last) load_tile(key0 + TK);
     const unsigned long long left = seen;
     if (!left || q0 >= p.L || (p.causal && key0 > wlast)) continue;
     const float inv_k = a.k.inv[tile0 + (key0 >> 6)], sc = sq * inv_k, sp = sg * a.v.inv[tile0 + (key0 >> 6)];
@@ -209,16 +212,16 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kerne
   if (lane == 0) { dacc[DPAD] += below; dacc[DPAD + p.map_n - 1] += above; }
   __syncthreads();
   dacc -= wave * nent;
-  float* part = a.part + (((long long)b * p.H + h) * nq + qb) * nent;
+  float* sums = a.part + ((((long long)b * p.H + h) * nq + qb) * a.qparts + part) * nent;
   for (int t = threadIdx.x; t < nent; t += NT) {
     float x = dacc[t];
 #pragma unroll
     for (int w = 1; w < NW; ++w) x += dacc[w * nent + t];
-    part[t] = x;
+    sums[t] = x;
   }
   if (!live) return;
   const float w = ku.inv * p.scale, fi = 1.f / f;
-  float* DQ = p.dq + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh;
+  float* DQ = (a.qparts > 1 ? a.dqp + (long long)part * p.B * p.L * p.H * p.dh : p.dq) + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -233,10 +236,10 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kerne
 
 // dk and dv.  A wave: 32 keys as columns; Q and dO of the heads that share them staged 64 or 32 queries at a time; S = Q K^T, dP = dO V^T, dV^T += dO^T P,
 // dK^T += Q^T dS.  P carries 2^14.  Few key blocks: a part of their queries (tiles of all the heads) a block, joined by relpos_bwd_sum_kernel.
-template <int DHP, int NW>
-__global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
-  using ST = Stage<DHP, NW>;
-  constexpr int TQ = ST::TK, NU = TQ / 32, KS = DHP / 16, DT = DHP / 32, KB = 32 * NW;
+template <int DHP>
+__global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
+  using ST = Stage<DHP>;
+  constexpr int TQ = ST::TK, NU = TQ / 32, KS = DHP / 16, DT = DHP / 32, KB = 128;
   extern __shared__ __attribute__((aligned(16))) char sm[];
   float* rl = reinterpret_cast<float*>(sm + 4 * ST::PLANE);      // the tile's lse
   float* rd = rl + 64;                                           // and D
@@ -244,8 +247,8 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kern
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nk = (p.S + KB - 1) / KB, qt = (p.L + 63) >> 6;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int part = id % a.nparts;
-  id /= a.nparts;
+  const int part = id % a.kparts;
+  id /= a.kparts;
   const int kb = id % nk;
   id /= nk;
   const int hk = id % p.Hkv, b = id / p.Hkv;
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kern
   const int t0 = p.causal ? max(0, kb * KB - pos0) / TQ : 0, t1 = kb * KB < n ? (p.L + TQ - 1) / TQ : 0;
   const int per = max(0, t1 - t0);
   const long long all = (long long)per * p.G;
-  const int first = (int)(all * part / a.nparts), last = (int)(all * (part + 1) / a.nparts);
+  const int first = (int)(all * part / a.kparts), last = (int)(all * (part + 1) / a.kparts);
   ST st;
   float lreg = 0.f, dreg = 0.f;
   auto load_tile = [&](int t) {
@@ -348,8 +351,8 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kern
   if (key >= p.S) return;
   const float w = qu.inv * p.scale, fi = 1.f / f, wv = gu.inv * 0x1p-14f;
   const long long at = ((long long)b * p.S + key) * p.Hkv * p.dh + hk * p.dh, size = (long long)p.B * p.S * p.Hkv * p.dh;
-  float* DK = a.nparts > 1 ? a.dkv + part * 2 * size : p.dk;
-  float* DV = a.nparts > 1 ? a.dkv + (part * 2 + 1) * size : p.dv;
+  float* DK = a.kparts > 1 ? a.dkv + part * 2 * size : p.dk;
+  float* DV = a.kparts > 1 ? a.dkv + (part * 2 + 1) * size : p.dv;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -365,17 +368,20 @@ __global__ __launch_bounds__(64 * NW, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kern
     }
 }
 
-// dk and dv from their parts, in order
-__global__ __launch_bounds__(256) void relpos_bwd_sum_kernel(const float* __restrict__ dkv, float* __restrict__ dk, float* __restrict__ dv, long long size, int nparts) {
+// gradients from their parts, in order: dq by grid.y = 0, dk and dv by 1 and 2
+struct Sum { const float* src; float* dst; long long size, step; int nparts; };
+struct Sums { Sum s[3]; };
+__global__ __launch_bounds__(256) void relpos_bwd_sum_kernel(Sums a) {
+  const Sum& s = a.s[blockIdx.y];
   const long long i = (blockIdx.x * 256LL + threadIdx.x) * 4;
-  if (i >= size) return;
-  const int which = blockIdx.y;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int t = 0; t < nparts; ++t) {
-    const float4 x = *reinterpret_cast<const float4*>(dkv + (t * 2 + which) * size + i);
-    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  if (i >= s.size) return;
+  float4 x = *reinterpret_cast<const float4*>(s.src + i);
+#pragma unroll 4
+  for (int t = 1; t < s.nparts; ++t) {
+    const float4 y = *reinterpret_cast<const float4*>(s.src + t * s.step + i);
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
   }
-  *reinterpret_cast<float4*>((which ? dv : dk) + i) = s;
+  *reinterpret_cast<float4*>(s.dst + i) = x;
 }
 
 // dtable[bucket][h] += the distances of that bucket: a block a head, the query blocks' sums in four fixed runs, then a wave a bucket
@@ -402,58 +408,41 @@ __global__ __launch_bounds__(1024) void relpos_bwd_table_kernel(RP p, const floa
   }
 }
 
-// Four waves a block where that still gives the chip's 256 CUs two blocks each, else two.  Key blocks: with a causal rule they differ (the first key meets all
-// queries, the last one), and few kv heads give few of them: parts of the queries until there are about four blocks a CU, none shorter than four tiles;
-// the parts' dk and dv are written and read once more.
-struct Plan { int qw, kw, nparts; long long qblocks, kblocks; int64_t part, dd, dkv, total; };
+// Parts: 256 CUs hold two blocks each at a time, and a wave alone on its SIMD waits through its own latencies, so fewer blocks than two a CU walk parts of
+// the other side (none shorter than four tiles; their gradients are written and read once more).  With a causal rule blocks differ in length -- a first key meets all
+// queries, a last one itself -- and four a CU are wanted.
+struct Plan { int qparts, kparts; long long qblocks, kblocks; int64_t part, dd, dqp, dkv, total; };
+
+int parts(long long base, long long tiles, bool causal) {
+  const long long want = causal ? 1024 : 512;
+  long long n = base >= want ? 1 : (want + base - 1) / base;
+  if (n > tiles / 4) n = tiles / 4;
+  return n < 1 ? 1 : n > 8 ? 8 : (int)n;
+}
 
 Plan plan(const RP& p) {
   Plan w;
-  const bool wide = p.dh > 96;
-  w.qw = wide || (long long)p.B * p.H * ((p.L + 127) / 128) >= 512 ? 4 : 2;
-  w.qblocks = (long long)p.B * p.H * ((p.L + 32 * w.qw - 1) / (32 * w.qw));
-  w.kw = wide || (long long)p.B * p.Hkv * ((p.S + 127) / 128) >= 256 ? 4 : 2;
-  const long long base = (long long)p.B * p.Hkv * ((p.S + 32 * w.kw - 1) / (32 * w.kw));
-  const long long tiles = (long long)p.G * ((p.L + 63) / 64);
-  long long np = (1024 + base - 1) / base, most = tiles / 4;
-  if (base >= 1024 || (!p.causal && base >= 512)) np = 1;
-  if (np > most) np = most;
-  if (np > 8) np = 8;
-  w.nparts = np < 1 ? 1 : (int)np;
-  w.kblocks = base * w.nparts;
-  w.part = ((int64_t)p.B * p.H * ((p.L + 32 * w.qw - 1) / (32 * w.qw)) * (p.map_n + 2 * DPAD) * 4 + 15) / 16 * 16;
+  const long long nq = (p.L + 127) / 128, nk = (p.S + 127) / 128;
+  w.qparts = parts(p.B * p.H * nq, (p.S + 63) / 64, p.causal);
+  w.kparts = parts(p.B * p.Hkv * nk, (long long)p.G * ((p.L + 63) / 64), p.causal);
+  w.qblocks = p.B * p.H * nq * w.qparts;
+  w.kblocks = p.B * p.Hkv * nk * w.kparts;
+  w.part = ((int64_t)w.qblocks * (p.map_n + 2 * DPAD) * 4 + 15) / 16 * 16;
   w.dd = (int64_t)p.B * p.H * up64(p.L) * 4;
-  w.dkv = w.nparts > 1 ? (int64_t)w.nparts * 2 * p.B * p.S * p.Hkv * p.dh * 4 : 0;
-  w.total = 2 * split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh) + w.part + w.dd + w.dkv;
+  w.dqp = w.qparts > 1 ? (int64_t)w.qparts * p.B * p.L * p.H * p.dh * 4 : 0;
+  w.dkv = w.kparts > 1 ? (int64_t)w.kparts * 2 * p.B * p.S * p.Hkv * p.dh * 4 : 0;
+  w.total = 2 * split_bytes(p.B, p.H, p.L, p.dh) + 2 * split_bytes(p.B, p.Hkv, p.S, p.dh) + w.part + w.dd + w.dqp + w.dkv;
   return w;
-}
-
-template <int DHP, int NW>
-int launch_q(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
-  const int planes = 4 * Stage<DHP, NW>::PLANE, lds = planes + 4 * (p.map_n + 2 * TABLE_PAD + NW * (p.map_n + 2 * DPAD));
-  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_bwd_q_kernel<DHP, NW>), planes + 4 * (MAP_MAX + 2 * TABLE_PAD + NW * (MAP_MAX + 2 * DPAD))));
-  SMX_LAUNCH((relpos_bwd_q_kernel<DHP, NW>), dim3((unsigned)w.qblocks), dim3(64 * NW), lds, st, p, a);
-  return smx_launch_status();
-}
-template <int DHP, int NW>
-int launch_kv(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
-  const int planes = 4 * Stage<DHP, NW>::PLANE, lds = planes + 4 * (128 + p.map_n + 2 * TABLE_PAD);
-  SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_bwd_kv_kernel<DHP, NW>), planes + 4 * (128 + MAP_MAX + 2 * TABLE_PAD)));
-  SMX_LAUNCH((relpos_bwd_kv_kernel<DHP, NW>), dim3((unsigned)w.kblocks), dim3(64 * NW), lds, st, p, a);
-  return smx_launch_status();
 }
 
 template <int DHP>
 int launch(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
-  int rc;
-  if constexpr (DHP < 128) {
-    rc = w.qw == 4 ? launch_q<DHP, 4>(p, a, w, st) : launch_q<DHP, 2>(p, a, w, st);
-    if (rc == SMX_OK) rc = w.kw == 4 ? launch_kv<DHP, 4>(p, a, w, st) : launch_kv<DHP, 2>(p, a, w, st);
-  } else {
-    rc = launch_q<DHP, 4>(p, a, w, st);
-    if (rc == SMX_OK) rc = launch_kv<DHP, 4>(p, a, w, st);
-  }
-  return rc;
+  const int planes = 4 * Stage<DHP>::PLANE, lq = 4 * (p.map_n + 2 * TABLE_PAD + 4 * (p.map_n + 2 * DPAD)), lk = 4 * (128 + p.map_n + 2 * TABLE_PAD);
+  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_q_kernel<DHP>, planes + 4 * (MAP_MAX + 2 * TABLE_PAD + 4 * (MAP_MAX + 2 * DPAD))));
+  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_kv_kernel<DHP>, planes + 4 * (128 + MAP_MAX + 2 * TABLE_PAD)));
+  SMX_LAUNCH(relpos_bwd_q_kernel<DHP>, dim3((unsigned)w.qblocks), dim3(256), planes + lq, st, p, a);
+  SMX_LAUNCH(relpos_bwd_kv_kernel<DHP>, dim3((unsigned)w.kblocks), dim3(256), planes + lk, st, p, a);
+  return smx_launch_status();
 }
 
 }  // namespace
@@ -468,7 +457,7 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
   int rc = check(d, p, true);
   if (rc != SMX_OK) return rc;
   const Plan w = plan(p);
-  const long long size = (long long)p.B * p.S * p.Hkv * p.dh, sums = (size / 4 + 255) / 256;
+  const long long sq = (long long)p.B * p.L * p.H * p.dh, sk = (long long)p.B * p.S * p.Hkv * p.dh, sums = ((sq > sk ? sq : sk) / 4 + 255) / 256;
   if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < w.total || w.qblocks > 0x7fffffffLL || w.kblocks > 0x7fffffffLL || sums > 0x7fffffffLL) return SMX_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   Bwd a;
@@ -481,8 +470,9 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
   a.part = (float*)ws;
   a.g.o = (const float*)p.o;
   a.g.dd = (float*)(ws + w.part);
-  a.dkv = (float*)(ws + w.part + w.dd);
-  a.nparts = w.nparts;
+  a.dqp = (float*)(ws + w.part + w.dd);
+  a.dkv = (float*)(ws + w.part + w.dd + w.dqp);
+  a.qparts = w.qparts; a.kparts = w.kparts;
   const Split all[4] = {a.q, a.g, a.k, a.v};
   rc = split_launch(p, all, 4, st);
   if (rc != SMX_OK) return rc;
@@ -493,7 +483,11 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
     default: rc = launch<128>(p, a, w, st);
   }
   if (rc != SMX_OK) return rc;
-  if (w.nparts > 1) SMX_LAUNCH(relpos_bwd_sum_kernel, dim3((unsigned)sums, 2), dim3(256), 0, st, (const float*)a.dkv, p.dk, p.dv, size, w.nparts);
-  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(p.H), dim3(1024), 0, st, p, (const float*)a.part, (p.L + 32 * w.qw - 1) / (32 * w.qw));
+  if (w.qparts > 1 || w.kparts > 1) {
+    const Sums u = {{{a.dqp, p.dq, w.qparts > 1 ? sq : 0, sq, w.qparts}, {a.dkv, p.dk, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts},
+                     {a.dkv + sk, p.dv, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts}}};
+    SMX_LAUNCH(relpos_bwd_sum_kernel, dim3((unsigned)sums, 3), dim3(256), 0, st, u);
+  }
+  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(p.H), dim3(1024), 0, st, p, (const float*)a.part, (p.L + 127) / 128 * w.qparts);
   return smx_launch_status();
 }
