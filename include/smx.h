@@ -694,7 +694,7 @@ int smx_chan_affine_f32(const float* x, int ldx, const float* scale, const float
  *   not masked, delta <= 0 if causal);  o_i = sum_j P_ij v_j.  A query with no key left: o = 0 and no gradient.
  * What the places of masked keys and of keys behind n_b hold is never used (NaN and infinities too); their dk / dv are written as 0.
  * q [B][L] rows of H*dh, k / v [B][S] rows of Hkv*dh (head h reads kv head h / (H / Hkv)), row strides ld*, sample strides *_bs in
- * elements (k / v sample stride 0: one context for all samples).  dh % 4 == 0, dh <= 128; strides % 4 == 0, pointers aligned to four
+ * elements (k / v sample stride 0: one context for all samples), ld* <= 2^24.  dh % 4 == 0, dh <= 128; strides % 4 == 0, pointers aligned to four
  * elements.  table [num_buckets][H] fp32, map [map_n] int32 device array with values in 0..num_buckets-1, map_n <= 2049,
  * map_lo <= 0 <= map_lo + map_n - 1; mask [B][S] bytes (1 = masked) or NULL; kv_len [B] int32 device or NULL.
  * lse: [B][H][L] floats or NULL: log2 of the row's softmax sum (+inf for a row with no key), what the backward reads.

@@ -12,6 +12,7 @@ namespace relpos {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));        // (HIP's own uint4 is a struct: its copies kept staging registers in scratch memory)
+typedef u32x4 u32x4a8 __attribute__((aligned(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -70,20 +71,48 @@ __device__ __forceinline__ f32x16 mfma_levels(const u32x4 (&a)[NL], const u32x4 
   }
   return mfma<NL>(a[0], b[0], c);
 }
-// eight fp32 -> the levels' fragments (bf16: one, rounded to nearest; halves: two)
+// eight fp32, times w, -> the levels' fragments (bf16: one, rounded to nearest; halves: two).  The second half is one v_fma_mix_f32 a value (v w - h1)
+// and the rounding in pairs; a caller without a factor passes one(), a 1 that the compiler does not see as such: it would fall back to a conversion
+// and a subtraction.
+__device__ __forceinline__ float one() {
+  float x = 1.f;
+  asm volatile("" : "+s"(x));
+  return x;
+}
 template <int NL>
-__device__ __forceinline__ void to_levels(const float* v, u32x4 (&f)[NL]) {
+__device__ __forceinline__ void to_levels(const float* v, float w, u32x4 (&f)[NL]) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (NL == 1) h[i] = cvt2_bf16(v[2 * i], v[2 * i + 1]);
+    const float a = v[2 * i], b = v[2 * i + 1];
+    if constexpr (NL == 1) h[i] = cvt2_bf16(a, b);
     else {
-      h[i] = cvt2_f16(v[2 * i], v[2 * i + 1]);
-      l[i] = cvt2_f16(fmaf(f16lo(h[i]), -1.f, v[2 * i]), fmaf(f16hi(h[i]), -1.f, v[2 * i + 1]));     // (as an fma: one v_fma_mix_f32 each)
+      h[i] = cvt2_f16(a * w, b * w);
+      l[i] = cvt2_f16(fmaf(a, w, -f16lo(h[i])), fmaf(b, w, -f16hi(h[i])));
     }
   }
   f[0] = u32x4{h[0], h[1], h[2], h[3]};
   if constexpr (NL == 2) f[1] = u32x4{l[0], l[1], l[2], l[3]};
+}
+// the same for weights, whose first half is taken of v itself
+__device__ __forceinline__ void to_halves(const float* v, float w1, u32x4 (&f)[2]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = cvt2_f16(v[2 * i], v[2 * i + 1]);
+    l[i] = cvt2_f16(fmaf(v[2 * i], w1, -f16lo(h[i])), fmaf(v[2 * i + 1], w1, -f16hi(h[i])));
+  }
+  f[0] = u32x4{h[0], h[1], h[2], h[3]};
+  f[1] = u32x4{l[0], l[1], l[2], l[3]};
+}
+
+// lanes 0..31: bit k of a wave-uniform word, lanes 32..63: bit k + 4, as a select's lane mask (scalar work, one select a value)
+__device__ __forceinline__ bool row_bit(unsigned long long word, int k) {
+  const unsigned a = -(unsigned)((word >> k) & 1), b = -(unsigned)((word >> (k + 4)) & 1);
+  return __builtin_amdgcn_inverse_ballot_w64((unsigned long long)b << 32 | a);
+}
+__device__ __forceinline__ unsigned long long uniform64(unsigned long long x) {
+  return (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)x);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -151,9 +180,7 @@ __device__ __forceinline__ float own_rows(u32x4 (&f)[DHP / 16][2], const float* 
   const float sc = pow2_of(other_max(m), inv);
 #pragma unroll
   for (int kk = 0; kk < DHP / 16; ++kk) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[kk][i] *= sc;
-    to_levels<2>(v[kk], f[kk]);
+    to_levels<2>(v[kk], sc, f[kk]);
   }
   return inv;
 }

@@ -100,6 +100,7 @@ int check(const smx_relpos_desc* d, RP& p, bool bwd) {
   if (d->has_q_start && (d->q_start > (1 << 30) || d->q_start < -(1 << 30))) return SMX_EINVAL;
   if (!(d->scale == d->scale) || (d->bf16 != 0 && d->bf16 != 1) || (bwd && d->bf16)) return SMX_EINVAL;
   if (d->ldq < d->H * d->dh || d->ldk < d->Hkv * d->dh || d->ldv < d->Hkv * d->dh || d->ldo < d->H * d->dh) return SMX_EINVAL;
+  if (d->ldq > (1 << 24) || d->ldk > (1 << 24) || d->ldv > (1 << 24) || d->ldo > (1 << 24)) return SMX_EINVAL;
   if ((d->ldq | d->ldk | d->ldv | d->ldo) % 4 || d->q_bs < 0 || d->k_bs < 0 || d->v_bs < 0 || d->o_bs < 0) return SMX_EINVAL;
   if (d->q_bs % 4 || d->k_bs % 4 || d->v_bs % 4 || d->o_bs % 4) return SMX_EINVAL;
   const int el = 4 * (d->bf16 ? 2 : 4);
@@ -187,28 +188,47 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   unsigned long long sreg = 0;
   const int tiles = (p.S + 63) >> 6;
   const long long tile0 = ((long long)b * p.Hkv + hk) * tiles;
+  // a step's rows: a wave-uniform start and 32-bit places behind it (bf16: rows of at most 2^24 elements)
+  unsigned ko[NCH], vo[NCH];
+  bool cin[NCH];
+  if constexpr (NL == 1) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const unsigned e = c * NT + threadIdx.x, d = e % CPR * 8;
+      ko[c] = (e / CPR * p.ldk + d) * 2; vo[c] = (e / CPR * p.ldv + d) * 2;
+      cin[c] = (int)d < p.dh;
+    }
+  }
   auto load_tile = [&](int key0) {
     if constexpr (NL == 2) {
       const long long at = (tile0 * 64 + key0) * DHP;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const int e = (c * NT + threadIdx.x) * 8;
+        const unsigned e = (c * NT + threadIdx.x) * 8;
         kreg[0][c] = *reinterpret_cast<const u32x4*>(a.k.hi + at + e); kreg[1][c] = *reinterpret_cast<const u32x4*>(a.k.lo + at + e);
         vreg[0][c] = *reinterpret_cast<const u32x4*>(a.v.hi + at + e); vreg[1][c] = *reinterpret_cast<const u32x4*>(a.v.lo + at + e);
       }
     } else {
+      const char* K = reinterpret_cast<const char*>((const bf16_t*)p.k + b * p.k_bs + (long long)key0 * p.ldk + hk * p.dh);
+      const char* V = reinterpret_cast<const char*>((const bf16_t*)p.v + b * p.v_bs + (long long)key0 * p.ldv + hk * p.dh);
+      if (key0 + TK <= n && !p.mask && p.dh % 8 == 0) {          // the usual step: nothing to look at
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const int e = c * NT + threadIdx.x, key = key0 + e / CPR, d = e % CPR * 8;
-        const bf16_t* K = (const bf16_t*)p.k + b * p.k_bs + (long long)key * p.ldk + hk * p.dh + d;
-        const bf16_t* V = (const bf16_t*)p.v + b * p.v_bs + (long long)key * p.ldv + hk * p.dh + d;
-        uint2 x = make_uint2(0, 0), y = x, z = x, w = x;
-        if (key < n && !(p.mask && p.mask[(long long)b * p.S + key])) {        // what a left-out place holds must not meet a zero weight: zeros instead
-          if (d < p.dh) { x = *reinterpret_cast<const uint2*>(K); z = *reinterpret_cast<const uint2*>(V); }
-          if (d + 4 < p.dh) { y = *reinterpret_cast<const uint2*>(K + 4); w = *reinterpret_cast<const uint2*>(V + 4); }
+        for (int c = 0; c < NCH; ++c) {
+          kreg[0][c] = vreg[0][c] = u32x4{0, 0, 0, 0};
+          if (cin[c]) { kreg[0][c] = *reinterpret_cast<const u32x4a8*>(K + ko[c]); vreg[0][c] = *reinterpret_cast<const u32x4a8*>(V + vo[c]); }
         }
-        kreg[0][c] = u32x4{x.x, x.y, y.x, y.y};
-        vreg[0][c] = u32x4{z.x, z.y, w.x, w.y};
+      } else {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          const int e = c * NT + threadIdx.x, key = key0 + e / CPR, d = e % CPR * 8;
+          uint2 x = make_uint2(0, 0), y = x, z = x, w = x;
+          if (key < n && !(p.mask && p.mask[(long long)b * p.S + key])) {      // what a left-out place holds must not meet a zero weight: zeros instead
+            if (d < p.dh) { x = *reinterpret_cast<const uint2*>(K + ko[c]); z = *reinterpret_cast<const uint2*>(V + vo[c]); }
+            if (d + 4 < p.dh) { y = *reinterpret_cast<const uint2*>(K + ko[c] + 8); w = *reinterpret_cast<const uint2*>(V + vo[c] + 8); }
+          }
+          kreg[0][c] = u32x4{x.x, x.y, y.x, y.y};
+          vreg[0][c] = u32x4{z.x, z.y, w.x, w.y};
+        }
       }
     }
     if (wave == 0) {
@@ -236,6 +256,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   float mo = 0.f, l = 0.f;
   bool begun = false;                                            // the row has met a key
   Unit vu;
+  const float w1 = one();
   const unsigned long long ALL = TK == 64 ? ~0ull : 0xffffffffull;
   if (ntiles > 0) { load_tile(kbeg); store_tile(0); }
   __syncthreads();
@@ -243,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
     const int buf = NBUF == 2 ? t & 1 : 0, key0 = kbeg + t * TK;
     if (t + 1 < ntiles) load_tile(key0 + TK);
     char* st = sm + buf * STAGE;
-    const unsigned long long left = seen[buf];
+    const unsigned long long left = uniform64(seen[buf]);
     if (left && q0 < p.L && !(p.causal && key0 > wlast)) {
       float sc = sq, lw = 0.f;
       if constexpr (NL == 2) {
@@ -278,20 +299,18 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
           for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], sc, lp[u * 32 + crow(r)]) + kc;
       }
       if (left != ALL) {
-        const unsigned long long mine = left >> (4 * hh);
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!((mine >> (u * 32 + crow(r))) & 1)) s[u][r] = -INFINITY;
+          for (int r = 0; r < 16; ++r) s[u][r] = row_bit(left, u * 32 + crow(r)) ? s[u][r] : -INFINITY;
       }
       if (p.causal && key0 + TK - 1 > pos0 + q0) {
-        const int d = key0 + 4 * hh - pos;
+        const int d = pos - key0 - 4 * hh;
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (d + u * 32 + crow(r) > 0) s[u][r] = -INFINITY;
+            if (d < u * 32 + crow(r)) s[u][r] = -INFINITY;
       }
       float top = s[0][0];
 #pragma unroll
@@ -322,7 +341,8 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           u32x4 pf[NL];
-          to_levels<NL>(e + 8 * g, pf);
+          if constexpr (NL == 2) to_halves(e + 8 * g, w1, pf);
+          else to_levels<1>(e + 8 * g, 1.f, pf);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
             u32x4 vf[NL];

@@ -46,9 +46,9 @@ struct Stage {
   __device__ __forceinline__ void load(const Split& x, const Split& y, long long at) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const long long e = at + (c * NT + threadIdx.x) * 8;
-      reg[0][c] = *reinterpret_cast<const u32x4*>(x.hi + e); reg[1][c] = *reinterpret_cast<const u32x4*>(x.lo + e);
-      reg[2][c] = *reinterpret_cast<const u32x4*>(y.hi + e); reg[3][c] = *reinterpret_cast<const u32x4*>(y.lo + e);
+      const unsigned e = (c * NT + threadIdx.x) * 8;
+      reg[0][c] = *reinterpret_cast<const u32x4*>(x.hi + at + e); reg[1][c] = *reinterpret_cast<const u32x4*>(x.lo + at + e);
+      reg[2][c] = *reinterpret_cast<const u32x4*>(y.hi + at + e); reg[3][c] = *reinterpret_cast<const u32x4*>(y.lo + at + e);
     }
   }
   __device__ __forceinline__ void store(char* sm) const {
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
     if (threadIdx.x == 0) seen = sreg;
     __syncthreads();
     if (t + 1 < last) load_tile(key0 + TK);
-    const unsigned long long left = seen;
+    const unsigned long long left = uniform64(seen);
     if (!left || q0 >= p.L || (p.causal && key0 > wlast)) continue;
     const float inv_k = a.k.inv[tile0 + (key0 >> 6)], sc = sq * inv_k, sp = sg * a.v.inv[tile0 + (key0 >> 6)];
     const float wk = exp2i(ku.enter(inv_k, dq));
@@ -156,16 +156,14 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, lp[crow(r)]) - lse);
       }
       if (left != ALL) {
-        const unsigned long long mine = left >> (4 * hh + u * 32);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((mine >> crow(r)) & 1)) s[r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = row_bit(left, u * 32 + crow(r)) ? s[r] : 0.f;
       }
       if (p.causal && key0 + u * 32 + 31 > pos0 + q0) {
-        const int d = key0 + u * 32 + 4 * hh - pos;
+        const int d = pos - (key0 + u * 32 + 4 * hh);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (d + crow(r) > 0) s[r] = 0.f;
+          if (d < crow(r)) s[r] = 0.f;
       }
       float ds[16], top = 0.f;
 #pragma unroll
@@ -193,11 +191,9 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
       follow(top, f, dq);
       const float fk = f * wk;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= fk;
-#pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2];
-        to_levels<2>(ds + 8 * g, pf);
+        to_levels<2>(ds + 8 * g, fk, pf);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const u32x4 kf[2] = {col_frag<DHP>(sm, u * 32 + g * 16, d), col_frag<DHP>(sm + ST::PLANE, u * 32 + g * 16, d)};
@@ -263,6 +259,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = zero16();
   float f = F0;
   Unit qu, gu;
+  const float w1 = one();
   // causal: the first query that stands at this block's first key or behind it
   const int t0 = p.causal ? max(0, kb * KB - pos0) / TQ : 0, t1 = kb * KB < n ? (p.L + TQ - 1) / TQ : 0;
   const int per = max(0, t1 - t0);
@@ -323,7 +320,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
         const int d = key - q0 - 4 * hh;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (d - crow(r) > 0) s[r] = 0.f;
+          if (d > crow(r)) s[r] = 0.f;
       }
       float ds[16], top = 0.f;
 #pragma unroll
@@ -331,13 +328,11 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       follow(top * ig, f, dk);
       const float fq = f * wq;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= fq;
-#pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2], sf[2];
         const float e[8] = {s[8 * g], s[8 * g + 1], s[8 * g + 2], s[8 * g + 3], s[8 * g + 4], s[8 * g + 5], s[8 * g + 6], s[8 * g + 7]};
-        to_levels<2>(e, pf);
-        to_levels<2>(ds + 8 * g, sf);
+        to_halves(e, w1, pf);
+        to_levels<2>(ds + 8 * g, fq, sf);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const u32x4 gt[2] = {col_frag<DHP>(sm + 2 * ST::PLANE, u * 32 + g * 16, d), col_frag<DHP>(sm + 3 * ST::PLANE, u * 32 + g * 16, d)};

@@ -1306,7 +1306,7 @@ def _rows3(t, what, B, width, like):
     bs, ld, one = t.stride()
     ld = ld if t.shape[1] > 1 else width
     bs = bs if B > 1 else 0
-    if (one != 1 and width > 1) or ld < width or ld % 4 or bs % 4 or t.data_ptr() % (4 * t.element_size()) or ld > 0x7fffffff:
+    if (one != 1 and width > 1) or ld < width or ld % 4 or bs % 4 or t.data_ptr() % (4 * t.element_size()) or ld > 1 << 24:
         raise L.SmxError(f"{what}: dense channels, row and sample strides in multiples of four elements and rows that start on one are needed, "
                          f"got strides {t.stride()} at {t.data_ptr():#x}")
     return t.data_ptr(), ld, bs

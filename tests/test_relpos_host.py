@@ -88,7 +88,7 @@ def relpos_desc(**kw):
 
 BAD = [dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(table=None), dict(map=None), dict(B=0), dict(H=0), dict(Hkv=0), dict(Hkv=3), dict(L=0), dict(S=0),
        dict(dh=0), dict(dh=30), dict(dh=132, H=1, Hkv=1, ldq=132, ldo=132, ldk=132, ldv=132), dict(map_n=0), dict(map_n=2050), dict(map_lo=1), dict(map_lo=-8),
-       dict(num_buckets=0), dict(num_buckets=4097), dict(ldq=124), dict(ldk=60), dict(ldv=66), dict(ldo=130), dict(q_bs=642), dict(k_bs=-4), dict(v_bs=2), dict(o_bs=1),
+       dict(num_buckets=0), dict(num_buckets=4097), dict(ldq=124), dict(ldk=60), dict(ldv=66), dict(ldo=130), dict(ldk=(1 << 24) + 4), dict(q_bs=642), dict(k_bs=-4), dict(v_bs=2), dict(o_bs=1),
        dict(q=FAKE + 4), dict(k=FAKE + 8), dict(v=FAKE + 2), dict(o=FAKE + 12), dict(bf16=2), dict(bf16=1, k=FAKE + 4), dict(scale=math.nan),
        dict(has_q_start=1, q_start=2 ** 30 + 1), dict(has_q_start=1, q_start=-2 ** 30 - 1), dict(L=2 ** 29 + 1), dict(S=2 ** 29 + 1)]
 
