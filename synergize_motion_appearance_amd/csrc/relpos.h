@@ -111,10 +111,6 @@ __device__ __forceinline__ bool row_bit(unsigned long long word, int k) {
   const unsigned a = -(unsigned)((word >> k) & 1), b = -(unsigned)((word >> (k + 4)) & 1);
   return __builtin_amdgcn_inverse_ballot_w64((unsigned long long)b << 32 | a);
 }
-__device__ __forceinline__ unsigned long long uniform64(unsigned long long x) {
-  return (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)x);
-}
-
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll

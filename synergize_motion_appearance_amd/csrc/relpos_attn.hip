@@ -140,15 +140,14 @@ struct Src {
 // and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
 template <int DHP, int NL>
-__global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
+__global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile_kernel(RP p, Src a) {
   constexpr int TK = STEP<DHP, NL>, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>, NT = 256;
   constexpr int PLANE = TK * RB, STAGE = 2 * NL * PLANE;         // K levels, V levels
   constexpr int NBUF = BUFFERS<DHP, NL>;
   constexpr int CPR = DHP / 8, NCH = TK * CPR / NT;              // 16-byte chunks of a row; of a plane, a thread
   constexpr float PSH = NL == 2 ? 6.f : 0.f;
-  extern __shared__ __attribute__((aligned(16))) char sm[];      // stages, bias, masks
+  extern __shared__ __attribute__((aligned(16))) char sm[];      // stages, bias
   float* lut = reinterpret_cast<float*>(sm + NBUF * STAGE);
-  unsigned long long* seen = reinterpret_cast<unsigned long long*>(sm + NBUF * STAGE + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   constexpr int QB = 128;
   const int nq = (p.L + QB - 1) / QB;
@@ -185,7 +184,8 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   }
 
   u32x4 kreg[NL][NCH], vreg[NL][NCH];
-  unsigned long long sreg = 0;
+  unsigned long long nleft = 0;                                  // the next step's keys that are left, and the 2^-k of its tile
+  float nik = 1.f, niv = 1.f;
   const int tiles = (p.S + 63) >> 6;
   const long long tile0 = ((long long)b * p.Hkv + hk) * tiles;
   // a step's rows: a wave-uniform start and 32-bit places behind it (bf16: rows of at most 2^24 elements)
@@ -231,10 +231,9 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
         }
       }
     }
-    if (wave == 0) {
-      const int key = key0 + lane;
-      sreg = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
-    }
+    const int key = key0 + lane;
+    nleft = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
+    if constexpr (NL == 2) { nik = a.k.inv[tile0 + (key0 >> 6)]; niv = a.v.inv[tile0 + (key0 >> 6)]; }
   };
   auto store_tile = [&](int buf) {
     char* st = sm + buf * STAGE;
@@ -247,7 +246,6 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
         *reinterpret_cast<u32x4*>(st + (NL + l) * PLANE + off) = vreg[l][c];
       }
     }
-    if (threadIdx.x == 0) seen[buf] = sreg;
   };
 
   f32x16 o[DT];
@@ -262,14 +260,15 @@ __global__ __launch_bounds__(256, 2) void relpos_tile_kernel(RP p, Src a) {
   __syncthreads();
   for (int t = 0; t < ntiles; ++t) {
     const int buf = NBUF == 2 ? t & 1 : 0, key0 = kbeg + t * TK;
+    const unsigned long long left = nleft;
+    const float ik = nik, iv = niv;
     if (t + 1 < ntiles) load_tile(key0 + TK);
     char* st = sm + buf * STAGE;
-    const unsigned long long left = uniform64(seen[buf]);
     if (left && q0 < p.L && !(p.causal && key0 > wlast)) {
       float sc = sq, lw = 0.f;
       if constexpr (NL == 2) {
-        sc = sq * a.k.inv[tile0 + (key0 >> 6)];
-        lw = (float)vu.enter(a.v.inv[tile0 + (key0 >> 6)], o);
+        sc = sq * ik;
+        lw = (float)vu.enter(iv, o);
       }
       f32x16 s[NU];
 #pragma unroll
@@ -623,7 +622,7 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
 
 template <int DHP, int NL>
 int tile_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
-  const int fixed = BUFFERS<DHP, NL> * 2 * NL * STEP<DHP, NL> * ROWB<DHP> + 16, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
+  const int fixed = BUFFERS<DHP, NL> * 2 * NL * STEP<DHP, NL> * ROWB<DHP>, lds = fixed + ((p.map_n + 2 * TABLE_PAD) * 4 + 15) / 16 * 16;
   SMX_HIP(smx_max_dynamic_lds((const void*)(relpos_tile_kernel<DHP, NL>), fixed + ((MAP_MAX + 2 * TABLE_PAD) * 4 + 15) / 16 * 16));
   SMX_LAUNCH((relpos_tile_kernel<DHP, NL>), dim3((unsigned)w.blocks), dim3(256), lds, st, p, a);
   return smx_launch_status();

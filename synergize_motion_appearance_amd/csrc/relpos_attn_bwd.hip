@@ -85,7 +85,6 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   const int nent = p.map_n + 2 * DPAD;
   float* lut = reinterpret_cast<float*>(sm + 4 * ST::PLANE);
   float* dacc = lut + p.map_n + 2 * TABLE_PAD;                   // [NW][nent]
-  __shared__ unsigned long long seen;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nq = (p.L + QB - 1) / QB;
   unsigned id = xcd_order(blockIdx.x, gridDim.x);
@@ -118,14 +117,14 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   Unit ku;
 
   ST st;
-  unsigned long long sreg = 0;
+  unsigned long long nleft = 0;                                  // the next step's keys that are left, and the 2^-k of its tile
+  float nik = 1.f, niv = 1.f;
   const long long tile0 = ((long long)b * p.Hkv + hk) * ((p.S + 63) >> 6);
   auto load_tile = [&](int key0) {
     st.load(a.k, a.v, (tile0 * 64 + key0) * DHP);
-    if (wave == 0) {
-      const int key = key0 + lane;
-      sreg = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
-    }
+    const int key = key0 + lane;
+    nleft = __ballot(lane < TK && key < n && !(p.mask && p.mask[(long long)b * p.S + key]));
+    nik = a.k.inv[tile0 + (key0 >> 6)]; niv = a.v.inv[tile0 + (key0 >> 6)];
   };
   if (first < last) load_tile(first * TK);
   const unsigned long long ALL = TK == 64 ? ~0ull : 0xffffffffull;
@@ -133,12 +132,11 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
     const int key0 = t * TK;
     __syncthreads();                                             // the tile before has been read
     st.store(sm);
-    if (threadIdx.x == 0) seen = sreg;
+    const unsigned long long left = nleft;
+    const float inv_k = nik, sc = sq * inv_k, sp = sg * niv;
     __syncthreads();
     if (t + 1 < last) load_tile(key0 + TK);
-    const unsigned long long left = uniform64(seen);
     if (!left || q0 >= p.L || (p.causal && key0 > wlast)) continue;
-    const float inv_k = a.k.inv[tile0 + (key0 >> 6)], sc = sq * inv_k, sp = sg * a.v.inv[tile0 + (key0 >> 6)];
     const float wk = exp2i(ku.enter(inv_k, dq));
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -266,7 +264,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
   const long long all = (long long)per * p.G;
   const int first = (int)(all * part / a.kparts), last = (int)(all * (part + 1) / a.kparts);
   ST st;
-  float lreg = 0.f, dreg = 0.f;
+  float lreg = 0.f, dreg = 0.f, niq = 1.f, nig = 1.f;            // the next tile's lse and D; its 2^-k
   auto load_tile = [&](int t) {
     const int i0 = (t0 + t % per) * TQ, i = i0 + threadIdx.x;
     const long long r = (long long)b * p.H + hk * p.G + t / per;
@@ -275,6 +273,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       lreg = i < p.L ? p.lse[r * p.L + i] : INFINITY;
       dreg = i < p.L ? a.g.dd[r * qt * 64 + i] : 0.f;
     }
+    niq = a.q.inv[r * qt + (i0 >> 6)]; nig = a.g.inv[r * qt + (i0 >> 6)];
   };
   if (first < last) load_tile(first);
   float first_bias = 0.f, last_bias = 0.f;
@@ -289,10 +288,9 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
     }
     __syncthreads();
+    const float inv_q = niq, inv_g = nig, sc = sk * inv_q, sp = sv * inv_g;
     if (t + 1 < last) load_tile(t + 1);
     if (k0 >= n || (p.causal && pos0 + i0 + TQ - 1 < k0)) continue;
-    const long long tile = ((long long)b * p.H + h) * qt + (i0 >> 6);
-    const float inv_q = a.q.inv[tile], inv_g = a.g.inv[tile], sc = sk * inv_q, sp = sv * inv_g;
     const int lg = 14 + gu.enter(inv_g, dv);                     // P carries 2^lg
     const float ig = exp2i(-lg), wq = exp2i(qu.enter(inv_q, dk)) * ig;
 #pragma unroll
