@@ -184,20 +184,24 @@ __device__ __forceinline__ float own_rows(u32x4 (&f)[DHP / 16][2], const float* 
 // An accumulator that sums over staged rows is kept in units of the largest 2^-k so far: a tile of larger values first brings it there (exactly: powers
 // of two), a tile of smaller ones enters with the factor 2^log2w <= 1 on its other operand.  (Below 2^-100 what a half holds of it is zero.)
 struct Unit {
-  float inv = 0.f;
-  template <int N> __device__ __forceinline__ int enter(float t, f32x16 (&acc)[N]) {
-    if (t > inv) {
-      const float r = inv / t;
-      inv = t;
+  int e = 0;                                                    // 2^-k's exponent bits, wave-uniform; 0: none yet
+  template <int N> __device__ __forceinline__ int enter(int t, f32x16 (&acc)[N]) {
+    if (t > e) {
+      const float r = __uint_as_float((unsigned)max(127 + e - t, 0) << 23);        // (the first tile: the accumulators are zeros)
+      e = t;
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[n][i] *= r;
       return 0;
     }
-    return max((int)(__float_as_uint(t) >> 23) - (int)(__float_as_uint(inv) >> 23), -100);
+    return max(t - e, -100);
   }
+  __device__ __forceinline__ float inv() const { return __uint_as_float((unsigned)e << 23); }     // (0: no tile came)
 };
+// the exponent bits of a power of two that all lanes hold, and back
+__device__ __forceinline__ int bits_of(float pow2) { return __builtin_amdgcn_readfirstlane(__float_as_uint(pow2) >> 23); }
+__device__ __forceinline__ float pow2_bits(int e) { return __uint_as_float((unsigned)e << 23); }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
 // keys (queries) a step: 64, or 32 where two operands of 128 columns in two halves each would not leave room for a second block on a CU

@@ -261,14 +261,15 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
   for (int t = 0; t < ntiles; ++t) {
     const int buf = NBUF == 2 ? t & 1 : 0, key0 = kbeg + t * TK;
     const unsigned long long left = nleft;
-    const float ik = nik, iv = niv;
+    const int ek = bits_of(nik), ev = bits_of(niv);
     if (t + 1 < ntiles) load_tile(key0 + TK);
     char* st = sm + buf * STAGE;
     if (left && q0 < p.L && !(p.causal && key0 > wlast)) {
-      float sc = sq, lw = 0.f;
+      float sc = sq;
+      int lw = 0;
       if constexpr (NL == 2) {
-        sc = sq * ik;
-        lw = (float)vu.enter(iv, o);
+        sc = sq * pow2_bits(ek);
+        lw = vu.enter(ev, o);
       }
       f32x16 s[NU];
 #pragma unroll
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
           for (int x = 0; x < NL; ++x) kf[x] = row_frag<DHP>(st + x * PLANE, u * 32, kk);
           s[u] = mfma_levels<NL>(kf, qf[kk], s[u]);
         }
-      const float kc = lw - mo;
+      const float kc = (float)lw - mo;
       const int e0 = key0 - (pos0 + q0) - p.map_lo;              // entry of the tile's first key and first query; the others: + key - query
       if (e0 + TK - 1 <= 0 || e0 - 31 >= p.map_n - 1) {
         const float c = (e0 + TK - 1 <= 0 ? first_bias : last_bias) + kc;
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-      top = other_max(top) - lw;                                 // s - mo of the row's largest score
+      top = other_max(top) - (float)lw;                                 // s - mo of the row's largest score
       const bool first = !begun && top > -INFINITY;
       if (__ballot(first || top > PSH + 8.f)) {
         const float d = first ? top - PSH : top > PSH ? top - PSH : 0.f, al = begun ? __builtin_amdgcn_exp2f(-d) : 0.f;
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
           }
         }
       }
-      l = fmaf(lt, exp2i(-(int)lw), l);
+      l = fmaf(lt, exp2i(-lw), l);
     }
     if (NBUF == 1) __syncthreads();
     if (t + 1 < ntiles) store_tile(NBUF == 2 ? buf ^ 1 : 0);
@@ -359,7 +360,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
   }
   if (qi >= p.L) return;
   l = other_sum(l);
-  const float inv_v = NL == 2 ? vu.inv : 1.f;
+  const float inv_v = NL == 2 ? vu.inv() : 1.f;
   const long long row = ((long long)b * p.H + h) * p.L + qi;
   if (a.nparts > 1) {
     float* O = a.part_o + (row * a.nparts + part) * p.dh;

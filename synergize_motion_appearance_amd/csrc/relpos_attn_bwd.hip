@@ -133,11 +133,12 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
     __syncthreads();                                             // the tile before has been read
     st.store(sm);
     const unsigned long long left = nleft;
-    const float inv_k = nik, sc = sq * inv_k, sp = sg * niv;
+    const int ek = bits_of(nik);
+    const float sc = sq * pow2_bits(ek), sp = sg * pow2_bits(bits_of(niv));
     __syncthreads();
     if (t + 1 < last) load_tile(key0 + TK);
     if (!left || q0 >= p.L || (p.causal && key0 > wlast)) continue;
-    const float wk = exp2i(ku.enter(inv_k, dq));
+    const float wk = exp2i(ku.enter(ek, dq));
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = rows_times<DHP>(sm, ST::PLANE, u * 32, qf);
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
     sums[t] = x;
   }
   if (!live) return;
-  const float w = ku.inv * p.scale, fi = 1.f / f;
+  const float w = ku.inv() * p.scale, fi = 1.f / f;
   float* DQ = (a.qparts > 1 ? a.dqp + (long long)part * p.B * p.L * p.H * p.dh : p.dq) + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -288,11 +289,12 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
     }
     __syncthreads();
-    const float inv_q = niq, inv_g = nig, sc = sk * inv_q, sp = sv * inv_g;
+    const int eq = bits_of(niq), eg = bits_of(nig);
+    const float sc = sk * pow2_bits(eq), sp = sv * pow2_bits(eg);
     if (t + 1 < last) load_tile(t + 1);
     if (k0 >= n || (p.causal && pos0 + i0 + TQ - 1 < k0)) continue;
-    const int lg = 14 + gu.enter(inv_g, dv);                     // P carries 2^lg
-    const float ig = exp2i(-lg), wq = exp2i(qu.enter(inv_q, dk)) * ig;
+    const int lg = 14 + gu.enter(eg, dv);                     // P carries 2^lg
+    const float ig = exp2i(-lg), wq = exp2i(qu.enter(eq, dk)) * ig;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = rows_times<DHP>(sm, ST::PLANE, u * 32, kf);
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     }
   }
   if (key >= p.S) return;
-  const float w = qu.inv * p.scale, fi = 1.f / f, wv = gu.inv * 0x1p-14f;
+  const float w = qu.inv() * p.scale, fi = 1.f / f, wv = gu.inv() * 0x1p-14f;
   const long long at = ((long long)b * p.S + key) * p.Hkv * p.dh + hk * p.dh, size = (long long)p.B * p.S * p.Hkv * p.dh;
   float* DK = a.kparts > 1 ? a.dkv + part * 2 * size : p.dk;
   float* DV = a.kparts > 1 ? a.dkv + (part * 2 + 1) * size : p.dv;
