@@ -179,20 +179,39 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
   for (int k = 0; k < NV; ++k) in[k] = (ln.sub + LPR * (k / V)) * V < p.E;
   const long long t1 = g * p.per + min(p.per, (blk + 1) * (long long)p.rows);
   const float iE = 1.f / p.E;
-  for (long long t = g * p.per + blk * p.rows + ln.row; t < t1; t += RPB) {
+  constexpr bool AHEAD = NV <= 8;                    // the next row is on its way during this one's sums
+  float row[2][4][NV];
+  auto load = [&](float (&w)[4][NV], long long t) {
     const long long at = t * p.E;
-    float x[NV], h[NV], c[NV], gy[NV];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int col = (ln.sub + LPR * k) * V;
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[k * V + e] = h[k * V + e] = c[k * V + e] = gy[k * V + e] = 0.f;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[i][k * V + e] = 0.f;
       if (col < p.E) {
-        ldv<float, V>((const float*)p.h + at + col, h + k * V);
-        if (p.gx) ldv<float, V>(p.gx + at + col, c + k * V);
-        if (p.gy) { ldv<float, V>((const float*)p.xo + at + col, x + k * V); ldv<float, V>(p.gy + at + col, gy + k * V); }
+        ldv<float, V>((const float*)p.h + at + col, w[1] + k * V);
+        if (p.gx) ldv<float, V>(p.gx + at + col, w[2] + k * V);
+        if (p.gy) { ldv<float, V>((const float*)p.xo + at + col, w[0] + k * V); ldv<float, V>(p.gy + at + col, w[3] + k * V); }
       }
     }
+  };
+  long long t = g * p.per + blk * p.rows + ln.row;
+  if (AHEAD && t < t1) load(row[1], t);
+  for (; t < t1; t += RPB) {
+    const long long at = t * p.E;
+    float (&x)[NV] = row[0][0];
+    float (&h)[NV] = row[0][1];
+    float (&c)[NV] = row[0][2];
+    float (&gy)[NV] = row[0][3];
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) row[0][i][k] = row[1][i][k];
+      if (t + RPB < t1) load(row[1], t + RPB);
+    } else load(row[0], t);
     float mx, rx, mh, rh, s1 = 0.f, s2 = 0.f;
     stats2<NV, LPR>(ln, x, h, in, p.E, p.rms, p.eps, mx, rx, mh, rh);
     if (p.gy) {

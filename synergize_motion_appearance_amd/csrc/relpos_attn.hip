@@ -610,8 +610,8 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
   const int rows = p.G * p.L;
   w.rt = rows >= 8 ? 8 : rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
   const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
-  // parts of the keys, none shorter than 256 keys, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four)
-  long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = (p.S + 255) / 256;
+  // parts of the keys from 513 keys on, none shorter than 256, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four)
+  long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = p.S <= 512 ? 1 : (p.S + 255) / 256;
   if (np > most) np = most;
   w.per = (int)(((p.S + np - 1) / np + 63) / 64 * 64);
   w.nparts = (p.S + w.per - 1) / w.per;

@@ -4,6 +4,7 @@ There is NO fallback: if the library is missing or was not built, importing this
 `load()` raises -- the product path never routes through a CPU implementation."""
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libsmx.so")
@@ -61,6 +62,11 @@ class Gemm16Desc(C.Structure):
     ]
 
 
+def _packer(fields):
+    """all fields of a struct at once (struct.pack: some ten times as fast as assigning them one by one)"""
+    return struct.Struct("@" + "".join({_p: "P", _i64: "q", C.c_int32: "i", _f: "f"}[t] for _, t in fields)).pack
+
+
 class RelposDesc(C.Structure):
     """mirror of `smx_relpos_desc` (include/smx.h)."""
     _fields_ = ([(n, _p) for n in ("q", "k", "v", "o", "table", "map", "mask", "kv_len", "lse", "ws", "d_o", "dq", "dk", "dv", "dtable")]
@@ -68,6 +74,7 @@ class RelposDesc(C.Structure):
                 + [(n, C.c_int32) for n in ("ldq", "ldk", "ldv", "ldo", "B", "H", "Hkv", "L", "S", "dh", "map_lo", "map_n", "num_buckets",
                                             "causal", "has_q_start", "q_start", "bf16")]
                 + [("scale", _f)])
+    pack = _packer(_fields_)
 
 
 class NormResidualDesc(C.Structure):
@@ -77,6 +84,7 @@ class NormResidualDesc(C.Structure):
                 + [(n, _i64) for n in ("T", "groups", "ws_floats")]
                 + [(n, C.c_int32) for n in ("E", "rms", "bf16", "gate_accumulate")]
                 + [("res_scale", _f), ("eps", _f)])
+    pack = _packer(_fields_)
 
 
 # name -> (restype, argtypes); every symbol include/smx.h declares

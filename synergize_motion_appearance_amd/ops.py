@@ -841,54 +841,64 @@ def layernorm(x, gamma, beta, pos=None, eps=1e-5):
     return y, yp
 
 
-def _call(t, fn, *args):
-    """fn(*args, stream) on the device that holds t and that device's current stream."""
-    if t.device.index == torch.cuda.current_device():
-        return fn(*args, _stream())
-    with torch.cuda.device(t.device):
-        return fn(*args, _stream())
+def _call(fn, d, index):
+    """fn(descriptor, stream) on device `index` and its current stream."""
+    if index == torch._C._cuda_getDevice():
+        return fn(d, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(d, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _vec(t, what, shape, like, dtype=torch.float32):
-    """address of a dense tensor of this shape and type on like's device."""
-    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device or not t.is_contiguous():
+def _vec(t, what, shape, device, dtype=torch.float32):
+    """address of a dense tensor of this shape and type on this device."""
+    if not torch.is_tensor(t) or t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if torch.is_tensor(t) else type(t).__name__
-        raise L.SmxError(f"{what}: a contiguous {dtype} tensor {shape} on {like.device} expected, got {got}")
+        raise L.SmxError(f"{what}: a contiguous {dtype} tensor {shape} on {device} expected, got {got}")
     return t.data_ptr()
 
 
-def _norm_weights(w, what, kind, E, like):
+def _norm_weights(w, what, E, device):
     """(gamma, beta) addresses of a norm given as (gamma, beta) or (gamma,), or None."""
     if w is None:
-        return None, None
+        return 0, 0
     if not isinstance(w, (tuple, list)) or len(w) not in (1, 2):
         raise L.SmxError(f"{what}: (gamma, beta) or (gamma,) expected")
-    beta = w[1] if len(w) == 2 else None
-    return _vec(w[0], f"{what} gamma", (E,), like), None if beta is None else _vec(beta, f"{what} beta", (E,), like)
+    return _vec(w[0], what, (E,), device), _vec(w[1], what, (E,), device) if len(w) == 2 and w[1] is not None else 0
 
 
-def _norm_residual_desc(x, h, post, gate, res_scale, pre, kind, eps):
-    """the fields of smx_norm_residual_desc that forward and backward share."""
+def _norm_residual(x, h, post, gate, res_scale, pre, kind, eps):
+    """ops.norm_residual -> (x', y, descriptor: what the backward completes, None without tokens)"""
     _dev(x, "norm_residual x", _ANY)
     _dev(h, "norm_residual h", _ANY)
-    if kind not in ("layer", "rms"):
+    if kind != "layer" and kind != "rms":
         raise L.SmxError(f"norm_residual: kind 'layer' or 'rms' expected, got {kind!r}")
-    if x.shape != h.shape or x.dtype != h.dtype or x.device != h.device or x.dim() < 2 or not x.is_contiguous() or not h.is_contiguous():
+    dev, dt, shape = x.device, x.dtype, x.shape
+    if shape != h.shape or h.dtype is not dt or h.device != dev or len(shape) < 2 or not x.is_contiguous() or not h.is_contiguous():
         raise L.SmxError(f"norm_residual: x and h must be contiguous tokens of one shape, type and device "
-                         f"({tuple(x.shape)} {x.dtype} {x.device}, {tuple(h.shape)} {h.dtype} {h.device})")
-    E = x.shape[-1]
+                         f"({tuple(shape)} {dt} {dev}, {tuple(h.shape)} {h.dtype} {h.device})")
+    E = shape[-1]
     if not 1 <= E <= 16384:
         raise L.SmxError(f"norm_residual: 1 to 16384 channels expected, got {E}")
-    T = x.numel() // E
-    d = L.NormResidualDesc(h=h.data_ptr(), T=T, groups=1, E=E, rms=int(kind == "rms"), bf16=int(x.dtype == BF16), res_scale=res_scale, eps=eps)
-    d.post_gamma, d.post_beta = _norm_weights(post, "norm_residual post", kind, E, x)
-    d.pre_gamma, d.pre_beta = _norm_weights(pre, "norm_residual pre", kind, E, x)
+    n = x.numel()
+    T = n // E
+    pg, pb = _norm_weights(post, "norm_residual post", E, dev)
+    ng, nb = _norm_weights(pre, "norm_residual pre", E, dev)
+    g, groups = 0, 1
     if gate is not None:
-        d.groups = gate.numel() // E if torch.is_tensor(gate) else 0
-        if d.groups < 1 or T % d.groups:
+        groups = gate.numel() // E if torch.is_tensor(gate) else 0
+        if groups < 1 or T % groups:
             raise L.SmxError(f"norm_residual: the gate's rows must divide the {T} tokens")
-        d.gate = _vec(gate, "norm_residual gate", (E,) if gate.dim() == 1 else (d.groups, E), x)
-    return d
+        g = _vec(gate, "norm_residual gate", (E,) if gate.dim() == 1 else (groups, E), dev)
+    xo = torch.empty_like(x)
+    y = torch.empty_like(x) if pre is not None else None
+    if not n:
+        return xo, y, None
+    d = L.NormResidualDesc.from_buffer_copy(L.NormResidualDesc.pack(
+        x.data_ptr(), h.data_ptr(), xo.data_ptr(), 0 if y is None else y.data_ptr(), pg, pb, ng, nb, g, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+        T, groups, 0, E, kind == "rms", dt is BF16, 0, res_scale, eps))
+    meta = None if _PROFILE is None else {"bytes": x.element_size() * (3.0 + (y is not None)) * n}
+    L.check(_timed("norm_residual", meta, _call, L.load().smx_norm_residual, d, dev.index), "norm_residual")
+    return xo, y, d
 
 
 def norm_residual(x, h, *, post=None, gate=None, res_scale=1.0, pre=None, kind="layer", eps=1e-5):
@@ -897,14 +907,7 @@ def norm_residual(x, h, *, post=None, gate=None, res_scale=1.0, pre=None, kind="
     type (fp32 or bf16), E <= 16384.  post / pre: (gamma, beta) or (gamma,), fp32 [E]; post None: h as it is; pre None: no y.
     gate: fp32 [E], or [G, E] with G dividing the tokens (row g gates the g-th run of T / G tokens: a sample, a frame, a token); None: 1.
     kind: "layer" (mean and variance) or "rms" (root mean square).  -> (x', y or None); y is the norm of x' as it is stored."""
-    d = _norm_residual_desc(x, h, post, gate, res_scale, pre, kind, eps)
-    xo = torch.empty_like(x)
-    y = torch.empty_like(x) if pre is not None else None
-    if x.numel():
-        d.x, d.xo, d.y = x.data_ptr(), xo.data_ptr(), None if y is None else y.data_ptr()
-        L.check(_timed("norm_residual", {"bytes": x.element_size() * (3.0 + (y is not None)) * x.numel()}, _call, x, L.load().smx_norm_residual, C.byref(d)),
-                "norm_residual")
-    return xo, y
+    return _norm_residual(x, h, post, gate, res_scale, pre, kind, eps)[:2]
 
 
 def softmax_rows(s, S, scale=1.0, mask=None, rows_per_mask=0):
@@ -1299,72 +1302,77 @@ def relpos(num_buckets=32, max_distance=128, two_sided=True):
     return RelPos(num_buckets, max_distance, two_sided)
 
 
-def _rows3(t, what, B, width, like):
-    """(address, row stride, sample stride) of [B, N, width] rows: dense channels, any row and sample strides that are multiples of four"""
-    if t.dim() != 3 or t.shape[0] != B or t.shape[2] != width or t.dtype != like.dtype or t.device != like.device:
-        raise L.SmxError(f"{what}: [{B}, N, {width}] {like.dtype} on {like.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _rows3(t, what, B, width, dtype, device):
+    """(address, row stride, sample stride, rows) of [B, N, width] rows: dense channels, any row and sample strides that are multiples of four"""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != width or t.dtype is not dtype or t.device != device:
+        raise L.SmxError(f"{what}: [{B}, N, {width}] {dtype} on {device} expected, got {tuple(shape)} {t.dtype} on {t.device}")
     bs, ld, one = t.stride()
-    ld = ld if t.shape[1] > 1 else width
-    bs = bs if B > 1 else 0
-    if (one != 1 and width > 1) or ld < width or ld % 4 or bs % 4 or t.data_ptr() % (4 * t.element_size()) or ld > 1 << 24:
+    at = t.data_ptr()
+    if shape[1] <= 1:
+        ld = width
+    if B <= 1:
+        bs = 0
+    if one != 1 or not width <= ld <= 1 << 24 or (ld | bs) & 3 or at % (4 * t.element_size()):
         raise L.SmxError(f"{what}: dense channels, row and sample strides in multiples of four elements and rows that start on one are needed, "
-                         f"got strides {t.stride()} at {t.data_ptr():#x}")
-    return t.data_ptr(), ld, bs
+                         f"got strides {t.stride()} at {at:#x}")
+    return at, ld, bs, shape[1]
 
 
-def _relpos_desc(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale):
-    """the fields of smx_relpos_desc that forward and backward share."""
+def _attention_relpos(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale, train):
+    """ops.attention_relpos -> (o, the rows' lse if train, descriptor: what the backward completes, None without queries or keys)"""
     _dev(q, "attention_relpos q", _ANY)
     _dev(k, "attention_relpos k", _ANY)
     _dev(v, "attention_relpos v", _ANY)
-    if not isinstance(rp, RelPos):
+    if type(rp) is not RelPos:
         raise L.SmxError(f"attention_relpos: a RelPos expected, got {type(rp).__name__}")
     nkv = nhead if nkv is None else nkv
-    if q.dim() != 3 or k.dim() != 3 or nhead < 1 or nkv < 1 or nhead % nkv or q.shape[2] % nhead:
-        raise L.SmxError(f"attention_relpos: q [B, L, heads * dh] and k / v [B, S, kv heads * dh] expected, got {tuple(q.shape)} / {tuple(k.shape)} with "
+    qs = q.shape
+    if len(qs) != 3 or nhead < 1 or nkv < 1 or nhead % nkv or qs[2] % nhead:
+        raise L.SmxError(f"attention_relpos: q [B, L, heads * dh] and k / v [B, S, kv heads * dh] expected, got {tuple(qs)} / {tuple(k.shape)} with "
                          f"{nhead} heads on {nkv}")
-    B, Lq, E = q.shape
-    S, dh = k.shape[1], E // nhead
-    if dh % 4 or not 4 <= dh <= 128 or E > 1 << 20 or B * nhead > 1 << 24 or max(Lq, S) > 1 << 29:
+    B, Lq, E = qs
+    dh, dev, dt = E // nhead, q.device, q.dtype
+    qp, ldq, qbs, _ = _rows3(q, "attention_relpos q", B, E, dt, dev)
+    kp, ldk, kbs, S = _rows3(k, "attention_relpos k", B, nkv * dh, dt, dev)
+    vp, ldv, vbs, Sv = _rows3(v, "attention_relpos v", B, nkv * dh, dt, dev)
+    if S != Sv:
+        raise L.SmxError(f"attention_relpos: k and v have {S} and {Sv} rows")
+    if dh & 3 or not 4 <= dh <= 128 or E > 1 << 20 or B * nhead > 1 << 24 or max(Lq, S) > 1 << 29:
         raise L.SmxError(f"attention_relpos: a head size of 4 to 128 in steps of four expected, got {dh} (B {B}, L {Lq}, S {S}, {nhead} heads)")
-    d = L.RelposDesc(B=B, H=nhead, Hkv=nkv, L=Lq, S=S, dh=dh, map_lo=rp.lo, map_n=len(rp.map), num_buckets=rp.num_buckets, causal=int(bool(causal)),
-                     bf16=int(q.dtype == BF16), scale=dh ** -0.5 if scale is None else scale)
-    d.q, d.ldq, d.q_bs = _rows3(q, "attention_relpos q", B, E, q)
-    d.k, d.ldk, d.k_bs = _rows3(k, "attention_relpos k", B, nkv * dh, q)
-    d.v, d.ldv, d.v_bs = _rows3(v, "attention_relpos v", B, nkv * dh, q)
-    if v.shape[1] != S:
-        raise L.SmxError(f"attention_relpos: k and v have {S} and {v.shape[1]} rows")
-    d.table = _vec(table, "attention_relpos table", (rp.num_buckets, nhead), q)
-    d.map = rp.on(q.device).data_ptr()
+    tp = _vec(table, "attention_relpos table", (rp.num_buckets, nhead), dev)
+    mp = np = 0
     if mask is not None:
-        d.mask = _vec(mask.view(torch.uint8) if torch.is_tensor(mask) and mask.dtype == torch.bool else mask, "attention_relpos mask", (B, S), q, torch.uint8)
+        mp = _vec(mask.view(torch.uint8) if torch.is_tensor(mask) and mask.dtype is torch.bool else mask, "attention_relpos mask", (B, S), dev, torch.uint8)
     if kv_len is not None:
-        d.kv_len = _vec(kv_len, "attention_relpos kv_len", (B,), q, torch.int32)
-    if q_start is not None:
-        if abs(q_start) > 1 << 30:
-            raise L.SmxError(f"attention_relpos: q_start {q_start} is out of range")
-        d.has_q_start, d.q_start = 1, q_start
-    return d
+        np = _vec(kv_len, "attention_relpos kv_len", (B,), dev, torch.int32)
+    if q_start is not None and abs(q_start) > 1 << 30:
+        raise L.SmxError(f"attention_relpos: q_start {q_start} is out of range")
+    o = torch.empty(qs, device=dev, dtype=dt)
+    if not S or not o.numel():
+        return o.zero_(), None, None
+    lse = torch.empty((B, nhead, Lq), device=dev) if train else None
+    d = L.RelposDesc.from_buffer_copy(L.RelposDesc.pack(
+        qp, kp, vp, o.data_ptr(), tp, rp.on(dev).data_ptr(), mp, np, 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0, 0,
+        qbs, kbs, vbs, Lq * E, 0, ldq, ldk, ldv, E, B, nhead, nkv, Lq, S, dh, rp.lo, len(rp.map), rp.num_buckets,
+        bool(causal), q_start is not None, q_start or 0, dt is BF16, dh ** -0.5 if scale is None else scale))
+    lib = L.load()
+    n = lib.smx_attention_relpos_ws_bytes(d)
+    if n > 0:
+        ws = torch.empty((n,), device=dev, dtype=torch.uint8)
+        d.ws, d.ws_bytes = ws.data_ptr(), n
+    meta = None if _PROFILE is None else {"flops": 4.0 * B * nhead * Lq * S * dh, "bytes": 2.0 * q.element_size() * (q.numel() + k.numel())}
+    L.check(_timed("attention_relpos", meta, _call, lib.smx_attention_relpos, d, dev.index), "attention_relpos")
+    return o, lse, d
 
 
-def attention_relpos(q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None, _lse=None):
+def attention_relpos(q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None):
     """Attention with a learned relative position bias: o_i = softmax_j(scale q_i . k_j + table[rp.bucket(j - pos_i)][head]) v_j per head.
     q [B, L, nhead * dh], k / v [B, S, nkv * dh] (fp32 or bf16; views of a fused projection are fine; head h reads kv head
     h // (nhead / nkv)), dh a multiple of four up to 128; table fp32 [rp.num_buckets, nhead]; scale: dh^-1/2 by default.
     kv_len int32 [B]: sample b has the first kv_len[b] of the S keys (clamped to 0..S).  Positions: key j is at j, query i at q_start + i,
     by default the queries are the last L of the sample's keys -- all of them in self attention, the newest one with L = 1.
     causal: keys behind the query's position are left out; mask uint8 or bool [B, S], nonzero: key left out.  What left-out keys of `mask` and
-    `kv_len` hold is not used, whatever it is.  A query with no key left answers zeros.  -> o [B, L, nhead * dh]."""
-    d = _relpos_desc(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale)
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    if not d.S or not o.numel():
-        return o.zero_()
-    lib = L.load()
-    d.o, d.ldo, d.o_bs = o.data_ptr(), q.shape[2], q.shape[1] * q.shape[2]
-    d.lse = None if _lse is None else _lse.data_ptr()
-    n = lib.smx_attention_relpos_ws_bytes(C.byref(d))
-    ws = torch.empty((n,), device=q.device, dtype=torch.uint8) if n > 0 else None
-    d.ws, d.ws_bytes = None if ws is None else ws.data_ptr(), n
-    meta = {"flops": 4.0 * d.B * nhead * d.L * d.S * d.dh, "bytes": q.element_size() * 2.0 * (q.numel() + k.numel())}
-    L.check(_timed(f"attention_relpos_d{d.dh}", meta, _call, q, lib.smx_attention_relpos, C.byref(d)), "attention_relpos")
-    return o
+    `kv_len` hold is not used, whatever it is (keys that only the causal rule hides from some queries must hold finite numbers).
+    A query with no key left answers zeros.  -> o [B, L, nhead * dh]."""
+    return _attention_relpos(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale, False)[0]

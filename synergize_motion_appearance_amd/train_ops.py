@@ -485,33 +485,34 @@ def norm_residual(tp, x, h, *, post=None, gate=None, res_scale=1.0, pre=None, ki
     pv, pg = zip(*((_param(tp, r)[:2]) for r in post)) if post is not None else (None, ())
     nv, ng = zip(*((_param(tp, r)[:2]) for r in pre)) if pre is not None else (None, ())
     gv, gg = (gate, None) if gate is None or torch.is_tensor(gate) else _param(tp, gate)[:2]
-    xo, y = ops.norm_residual(xc, hc, post=pv, gate=gv, res_scale=res_scale, pre=nv, kind=kind, eps=eps)
+    xo, y, d = ops._norm_residual(xc, hc, pv, gv, res_scale, nv, kind, eps)
+    held = (xc, hc, pv, nv, gv)                          # what the descriptor points at
 
     def bwd():
         gx, gy = tp.take(xo), (tp.take(y) if y is not None else None)
-        if (gx is None and gy is None) or not xo.numel():
+        if (gx is None and gy is None) or d is None:
             return
         lib = tp.lib
         gx = gx if gx is None or gx.is_contiguous() else _dense(lib, gx)
         gy = gy if gy is None or gy.is_contiguous() else _dense(lib, gy)
-        d = ops._norm_residual_desc(xc, hc, pv, gv, res_scale, nv, kind, eps)
-        dx = _empty(x.shape, x) if tp.needs(x) else None
-        dh = _empty(h.shape, h) if tp.needs(h) else None
-        dgate = gg if gg is not None else _empty(gv.shape, gv) if gv is not None and torch.is_tensor(gate) and tp.needs(gate) else None
-        d.xo, d.gate_accumulate = xo.data_ptr(), int(gg is not None)
-        for n, t in (("gx", gx), ("gy", gy), ("dx", dx), ("dh", dh), ("dgate", dgate)):
-            setattr(d, n, None if t is None else t.data_ptr())
-        for n, t in list(zip(("dpost_gamma", "dpost_beta"), pg)) + (list(zip(("dpre_gamma", "dpre_beta"), ng)) if gy is not None else []):
-            setattr(d, n, None if t is None else t.data_ptr())
-        n = int(lib.smx_norm_residual_bwd_ws_floats(d.T, d.groups, d.E))
+        dx = torch.empty_like(held[0]) if tp.needs(x) else None
+        dh = torch.empty_like(held[1]) if tp.needs(h) else None
+        dgate = gg if gg is not None else torch.empty_like(gv) if gv is not None and torch.is_tensor(gate) and tp.needs(gate) else None
+
+        def at(t):
+            return 0 if t is None else t.data_ptr()
+        d.gx, d.gy, d.dx, d.dh, d.dgate, d.gate_accumulate = at(gx), at(gy), at(dx), at(dh), at(dgate), gg is not None
+        if pg:
+            d.dpost_gamma, d.dpost_beta = at(pg[0]), at(pg[1]) if len(pg) > 1 else 0
+        if ng and gy is not None:
+            d.dpre_gamma, d.dpre_beta = at(ng[0]), at(ng[1]) if len(ng) > 1 else 0
+        n = lib.smx_norm_residual_bwd_ws_floats(d.T, d.groups, d.E)
         ws = torch.empty((n,), device=x.device, dtype=F32)
         d.ws, d.ws_floats = ws.data_ptr(), n
-        L.check(ops._call(x, lib.smx_norm_residual_bwd_f32, C.byref(d)), "norm_residual_bwd")
-        if dx is not None:
-            tp.acc(x, dx)
-        if dh is not None:
-            tp.acc(h, dh)
-        if gg is None and dgate is not None:
+        L.check(ops._call(lib.smx_norm_residual_bwd_f32, d, x.device.index), "norm_residual_bwd")
+        tp.acc(x, dx)
+        tp.acc(h, dh)
+        if gg is None:
             tp.acc(gate, dgate)
     tp.record(bwd)
     return xo, y
@@ -569,28 +570,26 @@ def attention_relpos(tp, q, k, v, table, rp, nhead, *, nkv=None, causal=False, m
     tv, tg, _ = _param(tp, table)
     if q.dtype != F32:
         raise L.SmxError(f"attention_relpos: the training step is fp32, got {q.dtype}")
-    lse = _empty((q.shape[0], nhead, q.shape[1]), q)
-    o = ops.attention_relpos(q, k, v, tv, rp, nhead, nkv=nkv, causal=causal, mask=mask, kv_len=kv_len, q_start=q_start, scale=scale, _lse=lse)
+    o, lse, d = ops._attention_relpos(q, k, v, tv, rp, nhead, nkv, causal, mask, kv_len, q_start, scale, True)
+    held = (q, k, v, tv, mask, kv_len, lse)              # what the descriptor points at
 
     def bwd():
         g = tp.take(o)
         if g is None:
             return
-        if not o.numel() or not k.numel():
-            for t in (q, k, v):
+        if d is None:
+            for t in held[:3]:
                 tp.acc(t, _zeros(t.shape, t))
             return
         lib = tp.lib
         g = g if g.is_contiguous() and g.data_ptr() % 16 == 0 else _dense(lib, g)
-        d = ops._relpos_desc(q, k, v, tv, rp, nhead, nkv, causal, mask, kv_len, q_start, scale)
-        dq, dk, dv = _empty(q.shape, q), _empty(k.shape, k), _empty(v.shape, v)
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=F32) for t in held[:3])
         dt = tg if tg is not None else _zeros(tv.shape, tv)
-        d.o, d.ldo, d.o_bs, d.lse, d.d_o = o.data_ptr(), q.shape[2], q.shape[1] * q.shape[2], lse.data_ptr(), g.data_ptr()
-        d.dq, d.dk, d.dv, d.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
-        n = int(lib.smx_attention_relpos_bwd_ws_bytes(C.byref(d)))
+        d.d_o, d.dq, d.dk, d.dv, d.dtable = g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
+        n = lib.smx_attention_relpos_bwd_ws_bytes(d)
         ws = torch.empty((max(n, 16),), device=q.device, dtype=torch.uint8)
         d.ws, d.ws_bytes = ws.data_ptr(), n
-        L.check(ops._call(q, lib.smx_attention_relpos_bwd_f32, C.byref(d)), "attention_relpos_bwd")
+        L.check(ops._call(lib.smx_attention_relpos_bwd_f32, d, q.device.index), "attention_relpos_bwd")
         tp.acc(q, dq)
         tp.acc(k, dk)
         tp.acc(v, dv)
