@@ -566,19 +566,19 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
   }
 }
 
-// o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts: a wave a row, its lanes the parts for the weights, then columns by runs of parts
+// o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts.  8, 16 or 32 lanes hold a row's columns, four each; up to 8 parts go by one after the other and a
+// wave has several rows, more are dealt to runs of lanes and joined by shuffles.
 template <typename T>
 __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
-  const int lane = threadIdx.x & 63;
-  const long long row = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  const int lanes = p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32, runs = a.nparts <= 8 ? 1 : 64 / lanes, per = lanes * runs;
+  const int lane = threadIdx.x & 63, run = lane % per / lanes, c = lane % lanes * 4;
+  const long long row = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / per) + lane / per;
   if (row >= (long long)p.B * p.H * p.L) return;
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nparts;
   float m = -INFINITY;
-  for (int s = lane; s < a.nparts; s += 64) m = fmaxf(m, ml[s].x);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  for (int s = run; s < a.nparts; s += runs) m = fmaxf(m, ml[s].x);
+  for (int o = lanes; o < per; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float mf = m == -INFINITY ? 0.f : m;
-  const int lanes = p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32, run = lane / lanes, runs = 64 / lanes, c = lane % lanes * 4;
   float l = 0.f, x = 0.f, y = 0.f, z = 0.f, w = 0.f;
   for (int s = run; s < a.nparts; s += runs) {
     const float2 t = ml[s];
@@ -589,7 +589,7 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
       x += f * v.x; y += f * v.y; z += f * v.z; w += f * v.w;
     }
   }
-  for (int o = lanes; o < 64; o <<= 1) {
+  for (int o = lanes; o < per; o <<= 1) {
     l += __shfl_xor(l, o, 64); x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); z += __shfl_xor(z, o, 64); w += __shfl_xor(w, o, 64);
   }
   if (run) return;
@@ -692,7 +692,8 @@ extern "C" int smx_attention_relpos(const smx_relpos_desc* d, void* stream) {
     }
   }
   if (rc != SMX_OK || w.nparts == 1) return rc;
-  const long long nj = ((long long)p.B * p.H * p.L + 3) / 4;
+  const int rows_a_block = 4 * (w.nparts <= 8 ? 64 / (p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32) : 1);
+  const long long nj = ((long long)p.B * p.H * p.L + rows_a_block - 1) / rows_a_block;
   if (nj > 0x7fffffffLL) return SMX_EINVAL;
   if (d->bf16) SMX_LAUNCH(relpos_join_kernel<bf16_t>, dim3((unsigned)nj), dim3(256), 0, st, p, a);
   else SMX_LAUNCH(relpos_join_kernel<float>, dim3((unsigned)nj), dim3(256), 0, st, p, a);

@@ -363,33 +363,35 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     }
 }
 
-// gradients from their parts, in order: dq by grid.y = 0, dk and dv by 1 and 2
-struct Sum { const float* src; float* dst; long long size, step; int nparts; };
-struct Sums { Sum s[3]; };
-__global__ __launch_bounds__(256) void relpos_bwd_sum_kernel(Sums a) {
-  const Sum& s = a.s[blockIdx.y];
-  const long long i = (blockIdx.x * 256LL + threadIdx.x) * 4;
-  if (i >= s.size) return;
-  float4 x = *reinterpret_cast<const float4*>(s.src + i);
-#pragma unroll 4
-  for (int t = 1; t < s.nparts; ++t) {
-    const float4 y = *reinterpret_cast<const float4*>(s.src + t * s.step + i);
-    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-  }
-  *reinterpret_cast<float4*>(s.dst + i) = x;
-}
-
-// dtable[bucket][h] += the distances of that bucket: a block a head, the query blocks' sums in four fixed runs, then a wave a bucket
-__global__ __launch_bounds__(1024) void relpos_bwd_table_kernel(RP p, const float* __restrict__ part, int nq) {
+// What is left once the two passes are done, one launch: the first H blocks dtable, the others gradients from their parts, in order (dq, dk, dv).
+// dtable[bucket][h] += the distances of that bucket: the query blocks' sums in four fixed runs, then a wave a bucket.
+struct Sum { const float* src; float* dst; long long size, step; int nparts, end; };      // end: running sum of blocks
+struct Rest { Sum s[3]; const float* part; int rows; };                                  // rows: query blocks (and their parts) of a head and sample
+__global__ __launch_bounds__(1024) void relpos_bwd_rest_kernel(RP p, Rest a) {
   __shared__ float ent[4][MAP_MAX + 2 * DPAD];
   __shared__ unsigned short of[MAP_MAX + 2 * DPAD];
+  if ((int)blockIdx.x >= p.H) {
+    int id = blockIdx.x - p.H, t = 0;
+    while (id >= a.s[t].end) ++t;
+    const Sum& s = a.s[t];
+    const long long i = ((id - (t ? a.s[t - 1].end : 0)) * 1024LL + threadIdx.x) * 4;
+    if (i >= s.size) return;
+    float4 x = *reinterpret_cast<const float4*>(s.src + i);
+#pragma unroll 4
+    for (int n = 1; n < s.nparts; ++n) {
+      const float4 y = *reinterpret_cast<const float4*>(s.src + n * s.step + i);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    *reinterpret_cast<float4*>(s.dst + i) = x;
+    return;
+  }
   const int h = blockIdx.x, nent = p.map_n + 2 * DPAD, run = threadIdx.x >> 8, lane = threadIdx.x & 63;
-  const int rows = p.B * nq, r0 = (int)((long long)rows * run / 4), r1 = (int)((long long)rows * (run + 1) / 4);
+  const int rows = p.B * a.rows, r0 = (int)((long long)rows * run / 4), r1 = (int)((long long)rows * (run + 1) / 4);
   for (int e = threadIdx.x; e < nent; e += 1024) of[e] = (unsigned short)p.map[p.entry(e - DPAD + p.map_lo)];
   for (int e = threadIdx.x & 255; e < nent; e += 256) {
     float s = 0.f;
-#pragma unroll 4
-    for (int r = r0; r < r1; ++r) s += part[(((long long)(r / nq) * p.H + h) * nq + r % nq) * nent + e];
+#pragma unroll 8
+    for (int r = r0; r < r1; ++r) s += a.part[(((long long)(r / a.rows) * p.H + h) * a.rows + r % a.rows) * nent + e];
     ent[run][e] = s;
   }
   __syncthreads();
@@ -452,8 +454,9 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
   int rc = check(d, p, true);
   if (rc != SMX_OK) return rc;
   const Plan w = plan(p);
-  const long long sq = (long long)p.B * p.L * p.H * p.dh, sk = (long long)p.B * p.S * p.Hkv * p.dh, sums = ((sq > sk ? sq : sk) / 4 + 255) / 256;
-  if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < w.total || w.qblocks > 0x7fffffffLL || w.kblocks > 0x7fffffffLL || sums > 0x7fffffffLL) return SMX_EINVAL;
+  const long long sq = (long long)p.B * p.L * p.H * p.dh, sk = (long long)p.B * p.S * p.Hkv * p.dh;
+  if (!d->ws || !aligned(d->ws, 16) || d->ws_bytes < w.total || w.qblocks > 0x7fffffffLL || w.kblocks > 0x7fffffffLL ||
+      (sq + 2 * sk) / 4096 > 0x7ff00000LL - p.H) return SMX_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   Bwd a;
   char* ws = (char*)d->ws;
@@ -478,11 +481,11 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
     default: rc = launch<128>(p, a, w, st);
   }
   if (rc != SMX_OK) return rc;
-  if (w.qparts > 1 || w.kparts > 1) {
-    const Sums u = {{{a.dqp, p.dq, w.qparts > 1 ? sq : 0, sq, w.qparts}, {a.dkv, p.dk, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts},
-                     {a.dkv + sk, p.dv, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts}}};
-    SMX_LAUNCH(relpos_bwd_sum_kernel, dim3((unsigned)sums, 3), dim3(256), 0, st, u);
-  }
-  SMX_LAUNCH(relpos_bwd_table_kernel, dim3(p.H), dim3(1024), 0, st, p, (const float*)a.part, (p.L + 127) / 128 * w.qparts);
+  Rest u = {{{a.dqp, p.dq, w.qparts > 1 ? sq : 0, sq, w.qparts, 0}, {a.dkv, p.dk, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0},
+             {a.dkv + sk, p.dv, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0}}, a.part, (p.L + 127) / 128 * w.qparts};
+  long long blocks = 0;
+  for (Sum& x : u.s) { blocks += (x.size + 4095) / 4096; x.end = (int)blocks; }
+  if (blocks + p.H > 0x7fffffffLL) return SMX_EINVAL;
+  SMX_LAUNCH(relpos_bwd_rest_kernel, dim3((unsigned)(p.H + blocks)), dim3(1024), 0, st, p, u);
   return smx_launch_status();
 }

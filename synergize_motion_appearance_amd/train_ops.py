@@ -482,8 +482,13 @@ def norm_residual(tp, x, h, *, post=None, gate=None, res_scale=1.0, pre=None, ki
         raise L.SmxError(f"norm_residual: the training step is fp32, got {x.dtype} / {h.dtype}")
     xc = x if x.is_contiguous() else _dense(tp.lib, x)
     hc = h if h.is_contiguous() else _dense(tp.lib, h)
-    pv, pg = zip(*((_param(tp, r)[:2]) for r in post)) if post is not None else (None, ())
-    nv, ng = zip(*((_param(tp, r)[:2]) for r in pre)) if pre is not None else (None, ())
+    pv = pg = nv = ng = None
+    if post is not None:
+        w = [_param(tp, r) for r in post]
+        pv, pg = [t[0] for t in w], [t[1] for t in w]
+    if pre is not None:
+        w = [_param(tp, r) for r in pre]
+        nv, ng = [t[0] for t in w], [t[1] for t in w]
     gv, gg = (gate, None) if gate is None or torch.is_tensor(gate) else _param(tp, gate)[:2]
     xo, y, d = ops._norm_residual(xc, hc, pv, gv, res_scale, nv, kind, eps)
     held = (xc, hc, pv, nv, gv)                          # what the descriptor points at
