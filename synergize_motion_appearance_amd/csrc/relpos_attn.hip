@@ -151,12 +151,9 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   constexpr int QB = 128;
   const int nq = (p.L + QB - 1) / QB;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int qb = nq - 1 - id % nq;                               // causal: the longest rows first
-  id /= nq;
-  const int part = id % a.nparts;
-  id /= a.nparts;
-  const int h = id % p.H, b = id / p.H, hk = h / p.G;
+  const Work w = work_of(blockIdx.x, nq * a.nparts, p.B * p.H, p.causal);
+  const int part = w.i % a.nparts, qb = nq - 1 - w.i / a.nparts;
+  const int h = w.head % p.H, b = w.head / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);
   const int q0 = qb * QB + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
   const int wlast = pos0 + min(q0 + 31, p.L - 1);                // the wave's last position; none if q0 >= L

@@ -87,12 +87,9 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   float* dacc = lut + p.map_n + 2 * TABLE_PAD;                   // [NW][nent]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nq = (p.L + QB - 1) / QB;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int part = id % a.qparts;
-  id /= a.qparts;
-  const int qb = nq - 1 - id % nq;
-  id /= nq;
-  const int h = id % p.H, b = id / p.H, hk = h / p.G;
+  const Work w = work_of(blockIdx.x, nq * a.qparts, p.B * p.H, p.causal);
+  const int part = w.i % a.qparts, qb = nq - 1 - w.i / a.qparts;
+  const int h = w.head % p.H, b = w.head / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);
   const int q0 = qb * QB + wave * 32, qi = q0 + (lane & 31), pos = pos0 + qi;
   const int wlast = pos0 + min(q0 + 31, p.L - 1);
@@ -211,11 +208,11 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   for (int t = threadIdx.x; t < nent; t += NT) {
     float x = dacc[t];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) x += dacc[w * nent + t];
+    for (int y = 1; y < NW; ++y) x += dacc[y * nent + t];
     sums[t] = x;
   }
   if (!live) return;
-  const float w = ku.inv() * p.scale, fi = 1.f / f;
+  const float wq = ku.inv() * p.scale, fi = 1.f / f;
   float* DQ = (a.qparts > 1 ? a.dqp + (long long)part * p.B * p.L * p.H * p.dh : p.dq) + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -224,7 +221,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
       const int c = d * 32 + 8 * g + 4 * hh;
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * g + e] * fi * w;
+      for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * g + e] * fi * wq;
       if (c < p.dh) *reinterpret_cast<float4*>(DQ + c) = make_float4(x[0], x[1], x[2], x[3]);
     }
 }
@@ -241,12 +238,9 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
   float* lut = rd + 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nk = (p.S + KB - 1) / KB, qt = (p.L + 63) >> 6;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int part = id % a.kparts;
-  id /= a.kparts;
-  const int kb = id % nk;
-  id /= nk;
-  const int hk = id % p.Hkv, b = id / p.Hkv;
+  const Work w = work_of(blockIdx.x, nk * a.kparts, p.B * p.Hkv, p.causal);
+  const int part = w.i % a.kparts, kb = w.i / a.kparts;
+  const int hk = w.head % p.Hkv, b = w.head / p.Hkv;
   const int n = p.keys(b), pos0 = p.pos0(n);
   const int k0 = kb * KB + wave * 32, key = k0 + (lane & 31);
   const bool in = key < n && !(p.mask && p.mask[(long long)b * p.S + key]);
@@ -344,7 +338,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     }
   }
   if (key >= p.S) return;
-  const float w = qu.inv() * p.scale, fi = 1.f / f, wv = gu.inv() * 0x1p-14f;
+  const float wk = qu.inv() * p.scale, fi = 1.f / f, wv = gu.inv() * 0x1p-14f;
   const long long at = ((long long)b * p.S + key) * p.Hkv * p.dh + hk * p.dh, size = (long long)p.B * p.S * p.Hkv * p.dh;
   float* DK = a.kparts > 1 ? a.dkv + part * 2 * size : p.dk;
   float* DV = a.kparts > 1 ? a.dkv + (part * 2 + 1) * size : p.dv;
@@ -355,7 +349,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       const int c = d * 32 + 8 * g + 4 * hh;
       float x[4], y[4];                                          // a key that nobody sees: what its column holds is dropped
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { x[e] = in ? dk[d][4 * g + e] * fi * w : 0.f; y[e] = in ? dv[d][4 * g + e] * wv : 0.f; }
+      for (int e = 0; e < 4; ++e) { x[e] = in ? dk[d][4 * g + e] * fi * wk : 0.f; y[e] = in ? dv[d][4 * g + e] * wv : 0.f; }
       if (c < p.dh) {
         *reinterpret_cast<float4*>(DK + at + c) = make_float4(x[0], x[1], x[2], x[3]);
         *reinterpret_cast<float4*>(DV + at + c) = make_float4(y[0], y[1], y[2], y[3]);
