@@ -214,12 +214,13 @@ __device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned n) {
   return x < r ? x * (q + 1) + s : r * (q + 1) + (x - r) * q + s;
 }
 
-// Which of a head's n blocks, and which of the heads, a block works on.  With a causal rule a head's blocks differ in length, 0 the longest: all heads' longest
-// go first (a chip that ends on long blocks waits for them: 1.3 waves a SIMD on average instead of 1.9), the heads of one XCD consecutive ones where they are a multiple of 8.
+// Which of a head's n blocks, and which of the heads, a block works on.  Blocks of one length: runs of heads by XCD.  With a causal rule a head's blocks differ, 0 the
+// longest: all heads' longest go first (a chip that ends on long blocks waits for them: 1.3 waves a SIMD on average instead of 1.9), the heads of one XCD
+// consecutive ones where they are a multiple of 8.  Ragged samples: heads in turn, so that no XCD has only the short ones.
 struct Work { int i, head; };
-__device__ __forceinline__ Work work_of(unsigned id, int n, int heads, int causal) {
-  if (!causal) { id = xcd_order(id, gridDim.x); return {(int)(id % n), (int)(id / n)}; }
-  if (heads & 7) return {(int)(id / heads), (int)(id % heads)};
+__device__ __forceinline__ Work work_of(unsigned id, int n, int heads, int causal, bool ragged) {
+  if (!causal && !ragged) { id = xcd_order(id, gridDim.x); return {(int)(id % n), (int)(id / n)}; }
+  if (ragged || (heads & 7)) return {(int)(id / heads), (int)(id % heads)};
   const unsigned m = heads >> 3, s = id >> 3;
   return {(int)(s / m), (int)((id & 7) * m + s % m)};
 }

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   constexpr int QB = 128;
   const int nq = (p.L + QB - 1) / QB;
-  const Work w = work_of(blockIdx.x, nq * a.nparts, p.B * p.H, p.causal);
+  const Work w = work_of(blockIdx.x, nq * a.nparts, p.B * p.H, p.causal, p.kv_len != nullptr);
   const int part = w.i % a.nparts, qb = nq - 1 - w.i / a.nparts;
   const int h = w.head % p.H, b = w.head / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);

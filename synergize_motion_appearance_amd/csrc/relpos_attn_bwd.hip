@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   float* dacc = lut + p.map_n + 2 * TABLE_PAD;                   // [NW][nent]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nq = (p.L + QB - 1) / QB;
-  const Work w = work_of(blockIdx.x, nq * a.qparts, p.B * p.H, p.causal);
+  const Work w = work_of(blockIdx.x, nq * a.qparts, p.B * p.H, p.causal, p.kv_len != nullptr);
   const int part = w.i % a.qparts, qb = nq - 1 - w.i / a.qparts;
   const int h = w.head % p.H, b = w.head / p.H, hk = h / p.G;
   const int n = p.keys(b), pos0 = p.pos0(n);
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
   float* lut = rd + 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nk = (p.S + KB - 1) / KB, qt = (p.L + 63) >> 6;
-  const Work w = work_of(blockIdx.x, nk * a.kparts, p.B * p.Hkv, p.causal);
+  const Work w = work_of(blockIdx.x, nk * a.kparts, p.B * p.Hkv, p.causal, p.kv_len != nullptr);
   const int part = w.i % a.kparts, kb = w.i / a.kparts;
   const int hk = w.head % p.Hkv, b = w.head / p.Hkv;
   const int n = p.keys(b), pos0 = p.pos0(n);
