@@ -151,10 +151,11 @@ __device__ __forceinline__ float other_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 2^k and 2^-k for values up to m
+// 2^k and 2^-k for values up to m.  Nothing but zeros: 2^-k reads 0.  An infinity: 2^-k reads infinity, so that what its tile enters is no number -- with a
+// finite one the other values of the tile would be lost without a sign.
 __device__ __forceinline__ float pow2_of(float m, float& inv) {
   const int e = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 15) - 127 : 14;     // floor(log2 m); 2^(14 - e) stays a normal number
-  inv = __uint_as_float((unsigned)(e - 14 + 127) << 23);
+  inv = m == 0.f ? 0.f : e == 128 ? INFINITY : __uint_as_float((unsigned)(e - 14 + 127) << 23);
   return __uint_as_float((unsigned)(14 - e + 127) << 23);
 }
 
@@ -181,19 +182,25 @@ __device__ __forceinline__ float own_rows(u32x4 (&f)[DHP / 16][2], const float* 
   return inv;
 }
 
-// An accumulator that sums over staged rows is kept in units of the largest 2^-k so far: a tile of larger values first brings it there (exactly: powers
-// of two), a tile of smaller ones enters with the factor 2^log2w <= 1 on its other operand.  (Below 2^-100 what a half holds of it is zero.)
+// An accumulator that sums over staged rows is kept in units of a 2^-k.  A tile of larger values first brings it to its own (exactly: powers of two); a smaller
+// one enters with the factor 2^log2w <= 1 on its other operand, down to 2^-8 (22 bits are still there: the factors' largest are 2^6 and more); below that
+// the accumulator comes down to the tile, as rows that give the larger tile no weight must not lose the smaller one's bits -- by at most 2^60 from
+// the largest, so that no sum leaves fp32's range.  A tile of zeros changes nothing.
 struct Unit {
-  int e = 0;                                                    // 2^-k's exponent bits, wave-uniform; 0: none yet
+  int e = 0, most = 0;                                          // exponent bits of 2^-k and of the largest so far, wave-uniform; 0: none yet
   template <int N> __device__ __forceinline__ int enter(int t, f32x16 (&acc)[N]) {
-    if (t > e) {
-      const float r = __uint_as_float((unsigned)max(127 + e - t, 0) << 23);        // (the first tile: the accumulators are zeros)
-      e = t;
+    if (t == 0) return 0;
+    most = max(most, t);
+    if (t > e || t < e - 8) {
+      const int to = max(t, most - 60);
+      if (to != e) {
+        const float r = __uint_as_float((unsigned)max(127 + e - to, 0) << 23);     // (the first tile: the accumulators are zeros)
+        e = to;
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[n][i] *= r;
-      return 0;
+          for (int i = 0; i < 16; ++i) acc[n][i] *= r;
+      }
     }
     return max(t - e, -100);
   }

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
     if (hh == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.nparts + part) * 2) = make_float2(begun ? mo : -INFINITY, l);
     return;
   }
-  const float il = l > 0.f ? inv_v / l : 0.f;
+  const float il = l == 0.f ? 0.f : inv_v / l;                    // (0: no key left; a sum that is no number stays none)
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
         else St<bf16_t>::st4((bf16_t*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);
       }
     }
-  if (p.lse && hh == 0) p.lse[row] = l > 0.f ? mo + __log2f(l) : INFINITY;
+  if (p.lse && hh == 0) p.lse[row] = l == 0.f ? INFINITY : mo + __log2f(l);
 }
 
 // ---- a few queries per sample ---------------------------------------------------------------------------------------------------
@@ -557,8 +557,8 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
       a.part_o[(at * a.nparts + part) * p.dh + c] = oo;
       if (c == 0) *reinterpret_cast<float2*>(a.part_ml + (at * a.nparts + part) * 2) = make_float2(mm, ll);
     } else {
-      St<T>::st((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, ll > 0.f ? oo / ll : 0.f);
-      if (p.lse && c == 0) p.lse[at] = ll > 0.f ? mm + __log2f(ll) : INFINITY;
+      St<T>::st((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, ll == 0.f ? 0.f : oo / ll);
+      if (p.lse && c == 0) p.lse[at] = ll == 0.f ? INFINITY : mm + __log2f(ll);
     }
   }
 }
@@ -590,11 +590,11 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
     l += __shfl_xor(l, o, 64); x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); z += __shfl_xor(z, o, 64); w += __shfl_xor(w, o, 64);
   }
   if (run) return;
-  const float il = l > 0.f ? 1.f / l : 0.f;
+  const float il = l == 0.f ? 0.f : 1.f / l;
   const int i = (int)(row % p.L), h = (int)(row / p.L % p.H);
   const long long b = row / p.L / p.H;
   if (c < p.dh) St<T>::st4((T*)p.o + b * p.o_bs + (long long)i * p.ldo + h * p.dh + c, make_float4(x * il, y * il, z * il, w * il));
-  if (p.lse && c == 0) p.lse[row] = l > 0.f ? m + __log2f(l) : INFINITY;
+  if (p.lse && c == 0) p.lse[row] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
 // ---- which kernel, in how many parts ---------------------------------------------------------------------------------------------

@@ -36,6 +36,13 @@ __device__ __forceinline__ void follow(float top, float& f, f32x16 (&acc)[N]) {
       for (int i = 0; i < 16; ++i) acc[t][i] *= r;
   }
 }
+// A weight is computed again as 2^(s - lse), whose error is that of s: some 2^-23 |s|.  Where lse is large enough for that to count, s - lse is kept from
+// passing 0: a weight above 1 would leave a half, and in the end fp32.  (No number stays none.)
+__device__ __forceinline__ bool steep(float lse) { return fabsf(lse) > 0x1p20f && lse < INFINITY; }
+__device__ __forceinline__ void at_most(f32x16& s, float top) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = s[r] > top ? top : s[r];
+}
 constexpr float F0 = 1.2676506002282294e30f;                     // 2^100: before the first dS that is not zero
 
 // stage TK rows of four planes (h1, h2 of two operands) through registers
@@ -103,6 +110,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   dacc += wave * nent;
   const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
   const float lse = live ? p.lse[((long long)b * p.H + h) * p.L + qi] : INFINITY;
+  const bool is_steep = __ballot(steep(lse)) != 0;
   const float D = live ? a.g.dd[((long long)b * p.H + h) * ((p.L + 63) & ~63) + qi] : 0.f;
   u32x4 qf[KS][2], gf[KS][2];
   const float sq = p.scale * LOG2E * own_rows<DHP>(qf, (const float*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh, live, p.dh);
@@ -145,12 +153,15 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
       if (lo || hi) {
         const float c = (lo ? first_bias : last_bias) - lse;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, c));
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, c);
       } else {
         const float* lp = lut + TABLE_PAD + e0 - (lane & 31) + 4 * hh;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, lp[crow(r)]) - lse);
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, lp[crow(r)]) - lse;
       }
+      if (is_steep) at_most(s, 0.f);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
       if (left != ALL) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = row_bit(left, u * 32 + crow(r)) ? s[r] : 0.f;
@@ -227,7 +238,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
 }
 
 // dk and dv.  A wave: 32 keys as columns; Q and dO of the heads that share them staged 64 or 32 queries at a time; S = Q K^T, dP = dO V^T, dV^T += dO^T P,
-// dK^T += Q^T dS.  P carries 2^14.  Few key blocks: a part of their queries (tiles of all the heads) a block, joined by relpos_bwd_sum_kernel.
+// dK^T += Q^T dS.  P carries 2^14.  Few key blocks: a part of their queries (tiles of all the heads) a block, joined by relpos_bwd_rest_kernel.
 template <int DHP>
 __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
   using ST = Stage<DHP>;
@@ -235,7 +246,8 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
   extern __shared__ __attribute__((aligned(16))) char sm[];
   float* rl = reinterpret_cast<float*>(sm + 4 * ST::PLANE);      // the tile's lse
   float* rd = rl + 64;                                           // and D
-  float* lut = rd + 64;
+  int* flag = reinterpret_cast<int*>(rd + 64);                   // whether one of the tile's lse is steep
+  float* lut = rd + 64 + 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
   const int nk = (p.S + KB - 1) / KB, qt = (p.L + 63) >> 6;
   const Work w = work_of(blockIdx.x, nk * a.kparts, p.B * p.Hkv, p.causal, p.kv_len != nullptr);
@@ -277,12 +289,14 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     __syncthreads();
     st.store(sm);
     if (threadIdx.x < TQ) { rl[threadIdx.x] = lreg; rd[threadIdx.x] = dreg; }
+    if (threadIdx.x < 64) *flag = __ballot(lane < TQ && steep(lreg)) != 0;
     if (t == first || t % per == 0) {
       fill_bias(lut, p, h);
       first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E;
       last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
     }
     __syncthreads();
+    const bool is_steep = __builtin_amdgcn_readfirstlane(*flag) != 0;
     const int eq = bits_of(niq), eg = bits_of(nig);
     const float sc = sk * pow2_bits(eq), sp = sv * pow2_bits(eg);
     if (t + 1 < last) load_tile(t + 1);
@@ -304,12 +318,15 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       if (e0 + 31 <= 0 || e0 - 31 >= p.map_n - 1) {
         const float c = (e0 + 31 <= 0 ? first_bias : last_bias) + lg;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, c - lv[r]));
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, c - lv[r]);
       } else {
         const float* lp = lut + TABLE_PAD + e0 + (lane & 31) - 4 * hh;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, lp[-crow(r)] - (lv[r] - lg)));
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, lp[-crow(r)] - (lv[r] - lg));
       }
+      if (is_steep) at_most(s, (float)lg);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
       if (p.causal && k0 + 31 > q0) {
         const int d = key - q0 - 4 * hh;
 #pragma unroll
@@ -428,9 +445,9 @@ Plan plan(const RP& p) {
 
 template <int DHP>
 int launch(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
-  const int planes = 4 * Stage<DHP>::PLANE, lq = 4 * (p.map_n + 2 * TABLE_PAD + 4 * (p.map_n + 2 * DPAD)), lk = 4 * (128 + p.map_n + 2 * TABLE_PAD);
+  const int planes = 4 * Stage<DHP>::PLANE, lq = 4 * (p.map_n + 2 * TABLE_PAD + 4 * (p.map_n + 2 * DPAD)), lk = 4 * (132 + p.map_n + 2 * TABLE_PAD);
   SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_q_kernel<DHP>, planes + 4 * (MAP_MAX + 2 * TABLE_PAD + 4 * (MAP_MAX + 2 * DPAD))));
-  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_kv_kernel<DHP>, planes + 4 * (128 + MAP_MAX + 2 * TABLE_PAD)));
+  SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_kv_kernel<DHP>, planes + 4 * (132 + MAP_MAX + 2 * TABLE_PAD)));
   SMX_LAUNCH(relpos_bwd_q_kernel<DHP>, dim3((unsigned)w.qblocks), dim3(256), planes + lq, st, p, a);
   SMX_LAUNCH(relpos_bwd_kv_kernel<DHP>, dim3((unsigned)w.kblocks), dim3(256), planes + lk, st, p, a);
   return smx_launch_status();

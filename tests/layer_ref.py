@@ -22,9 +22,12 @@ def bucket(num_buckets, max_distance, two_sided, delta):
     return side + half + t
 
 
-def attention(q, k, v, table, rp, nhead, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None, g=None, storage=torch.float32):
+def attention(q, k, v, table, rp, nhead, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None, g=None, storage=torch.float32, apart=0):
     """-> {"o", ("dq", "dk", "dv", "dtable")}, each with its bound: (value, largest error that rounding allows), fp64 on the CPU.
-    Left-out keys are not used, queries with no key give zeros."""
+    Left-out keys are not used, queries with no key give zeros.  fp32 storage: a factor w of a sum over rows (weights, dS) is two halves of w 2^s; the second
+    half's lowest bit is 2^-24, so that w is off by up to 2^-25 2^-s, or by w itself if it is smaller.  2^s brings a row's largest weight to 2^6 at least in the
+    forward (2^-31 of it), weights to 2^14 in dv (2^-39), a column's largest |dS| to 2^9 at least (2^-34 of it); apart: binary orders less where staged
+    tiles differ in size."""
     nkv = nhead if nkv is None else nkv
     B, L, E = q.shape
     S, dh, G = k.shape[1], E // nhead, nhead // nkv
@@ -50,7 +53,8 @@ def attention(q, k, v, table, rp, nhead, nkv=None, causal=False, mask=None, kv_l
         gone = ~see[0] if L else torch.ones(S, dtype=torch.bool)
         if causal:
             see &= delta <= 0
-        which = torch.tensor([rp.bucket(int(x)) for x in delta.flatten().tolist()], dtype=torch.long).view(L, S)
+        lo = int(delta.min()) if delta.numel() else 0
+        which = torch.tensor([rp.bucket(x) for x in range(lo, lo + L + S)], dtype=torch.long)[delta - lo]
         for h in range(nhead):
             c, ck = slice(h * dh, (h + 1) * dh), slice(h // G * dh, (h // G + 1) * dh)
             Q, K, V = q[b, :, c], k[b, :, ck].masked_fill(gone[:, None], 0.0), v[b, :, ck].masked_fill(gone[:, None], 0.0)
@@ -68,6 +72,9 @@ def attention(q, k, v, table, rp, nhead, nkv=None, causal=False, mask=None, kv_l
             pv = p @ V.abs()
             out["o"][0][b, :, c] = o
             out["o"][1][b, :, c] = (2 * T + acc + (u if storage != torch.float32 else 0.0)) * pv + u * o.abs()
+            low = 2.0 ** apart * (1 if storage == torch.float32 else 0)
+            if S:
+                out["o"][1][b, :, c] += torch.minimum(p, low * 2.0 ** -31 * p.amax(-1, keepdim=True)) @ V.abs()
             if g is None:
                 continue
             dO = g[b, :, c]
@@ -75,15 +82,17 @@ def attention(q, k, v, table, rp, nhead, nkv=None, causal=False, mask=None, kv_l
             ds = p * (dP - D)
             ep = (2 * T + 16 * U32) * p
             edP = (prod + (dh + 4) * U32) * (dO.abs() @ V.abs().t())
-            eD = (dh + 4) * U32 * (dO * o).abs().sum(-1, keepdim=True) + (dO.abs() * ((2 * T + acc) * pv + U32 * o.abs())).sum(-1, keepdim=True)
+            eD = (dh + 4) * U32 * (dO * o).abs().sum(-1, keepdim=True) + (dO.abs() * out["o"][1][b, :, c]).sum(-1, keepdim=True)
             eds = ep * (dP - D).abs() + p * (edP + eD) + 4 * U32 * ds.abs()
             accq = (L * G / 4 + 64) * U32 + prod
             out["dq"][0][b, :, c] = scale * ds @ K
-            out["dq"][1][b, :, c] = scale * (eds + acc * ds.abs()) @ K.abs()
+            size = ds.abs()
+            fq, fk = (torch.minimum(size, low * 2.0 ** -34 * size.amax(d, keepdim=True)) for d in (-1, 0))
+            out["dq"][1][b, :, c] = scale * (eds + acc * ds.abs() + fq) @ K.abs()
             out["dk"][0][b, :, ck] += scale * ds.t() @ Q
-            out["dk"][1][b, :, ck] += scale * (eds + accq * ds.abs()).t() @ Q.abs()
+            out["dk"][1][b, :, ck] += scale * (eds + accq * ds.abs() + fk).t() @ Q.abs()
             out["dv"][0][b, :, ck] += p.t() @ dO
-            out["dv"][1][b, :, ck] += (ep + accq * p).t() @ dO.abs()
+            out["dv"][1][b, :, ck] += (ep + accq * p + p.clamp(max=low * 2.0 ** -39)).t() @ dO.abs()
             # a bucket's sum: in fp32 over a tile's diagonal and a block's tiles, then over the blocks
             out["dtable"][0][:, h].index_add_(0, which.flatten(), ds.flatten())
             out["dtable"][1][:, h].index_add_(0, which.flatten(), (eds + ((L + S) / 4 + 64) * U32 * ds.abs()).flatten())

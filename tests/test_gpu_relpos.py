@@ -67,6 +67,10 @@ FORWARD = [
     (1, 4, 2, 513, 513, 32, True, True, False, True),
     (3, 2, 2, 257, 700, 64, True, False, True, False),
     (1, 3, 1, 1100, 1100, 4, False, False, False, False),
+    (2, 8, 4, 385, 385, 32, True, False, False, False),          # 16 heads: their order over the XCDs
+    (1, 8, 8, 8, 2000, 100, True, True, False, False),           # the most queries a token call takes, keys in parts
+    (1, 1, 1, 9, 2000, 100, True, True, False, False),           # the fewest a tile call takes
+    (1, 16, 1, 3, 700, 64, False, False, False, False),          # more query rows on a kv head than one block takes
 ]
 
 
@@ -96,6 +100,9 @@ BACKWARD = [
     (3, 3, 3, 190, 190, 4, True, False, True),
     (1, 4, 4, 640, 640, 64, True, False, False),
     (1, 2, 1, 70, 1500, 32, False, False, False),
+    (1, 1, 1, 1500, 1500, 64, True, False, False),               # both sides in parts
+    (2, 8, 4, 200, 200, 36, True, False, False),
+    (4, 2, 1, 700, 1030, 100, False, True, True),
 ]
 
 
@@ -227,6 +234,41 @@ def test_rows_without_a_key(ops, T, dtype, Lq):
         for n, t in (("dq", tp.grad(q)), ("dk", tp.grad(k)), ("dv", tp.grad(v)), ("dtable", tp.G["t"])):
             near(t, ref[n], n)
         assert float(tp.grad(q)[1:].abs().max()) == 0.0 and float(tp.grad(k)[1:].abs().max()) == 0.0
+
+
+def test_table_gradient_of_many_pairs(ops, T):
+    """a bucket of half a million pairs of mixed signs: independent errors of a few 2^-23 a pair (22-bit products, fp32 scores) stay that in the sum, 2^-19
+    holds sixteen of them; an error of one sign a pair, as small as 2^-25 of it, would grow to 2^-15 of the sum"""
+    from synergize_motion_appearance_amd.tape import Tape
+    B, H, S, dh = 2, 2, 1024, 32
+    q, k, v, g = mk(21, B, H, H, S, S, dh)
+    rp = ops.relpos(32, 128)
+    table, go = torch.randn(32, H, generator=g).cuda(), (torch.randn(B, S, H * dh, generator=g) * 1e-3).cuda()
+    G = {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    o = T.attention_relpos(tp, q, k, v, "t", rp, H)
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    ref = R.attention(q, k, v, table, rp, H, g=go)["dtable"][0]
+    assert float((G["t"].double().cpu() - ref).norm() / ref.norm()) < 2.0 ** -19
+
+
+@pytest.mark.parametrize("a", [(64, 1024, True), (2, 1024, False), (512, 600, True)])
+def test_largest_maps(ops, T, a):
+    from synergize_motion_appearance_amd.tape import Tape
+    B, H, S, dh = 1, 2, 1400, 32
+    q, k, v, g = mk(22, B, H, H, S, S, dh)
+    rp = ops.relpos(*a)
+    table, go = torch.randn(a[0], H, generator=g).cuda(), torch.randn(B, S, H * dh, generator=g).cuda()
+    G = {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    o = T.attention_relpos(tp, q, k, v, "t", rp, H)
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    ref = R.attention(q, k, v, table, rp, H, g=go)
+    for n, t in (("o", o), ("dq", tp.grad(q)), ("dk", tp.grad(k)), ("dv", tp.grad(v)), ("dtable", G["t"])):
+        near(t, ref[n], n)
+    near(ops.attention_relpos(q[:, -1:], k, v, table, rp, H), (ref["o"][0][:, -1:], ref["o"][1][:, -1:]))
 
 
 @pytest.mark.parametrize("start", [-70, 0, 13, 500, 2 ** 30, -2 ** 30])
@@ -368,6 +410,86 @@ def test_other_stream_and_graph(ops, T):
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("scales", [(0.0, 1e-6), (1e-9, 0.0, 1.0), (1.0, 1e-9), (1.0, 1e-9, 1e9, 1e-3, 0.0, 1e-12)], ids=str)
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+def test_tiles_of_very_different_sizes(ops, T, which, scales):
+    """rows of 64 that are zeros (a loss over some tokens only) or 2^30 and more apart; a channel of its own for each 64 keys keeps the weights across them
+    below 2^-50, so that every row's results are of its own tile's size and have that size's accuracy"""
+    from synergize_motion_appearance_amd.tape import Tape
+    n = len(scales)
+    B, H, S, dh = 1, 1, 64 * n, 64
+    q, k, v, g = mk(25, B, H, H, S, S, dh)
+    go = torch.randn(B, S, dh, generator=g).cuda()
+    scale = 1.0
+    for j, f in enumerate(scales):
+        own = slice(64 * j, 64 * j + 64)
+        if which in ("v", "do"):
+            for t in (q, k):
+                t[:, own] *= 0.2
+                t[:, own, :n] = 0.0
+                t[:, own, j] = 7.0                                   # score 49 on the own tile
+        {"q": q, "k": k, "v": v, "do": go}[which][:, own] *= f
+    rp = ops.relpos(32, 128)
+    table = torch.randn(32, H, generator=g).cuda() * 0.1
+    G = {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    o = T.attention_relpos(tp, q, k, v, "t", rp, H, scale=scale if which in ("v", "do") else None)
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    ref = R.attention(q, k, v, table, rp, H, g=go, scale=scale if which in ("v", "do") else None, apart=8)
+    for name, t in (("o", o), ("dq", tp.grad(q)), ("dk", tp.grad(k)), ("dv", tp.grad(v)), ("dtable", G["t"])):
+        near(t, ref[name], name)
+
+
+@pytest.mark.parametrize("Lq, S, dtype", [(1, 40, F32), (1, 3000, F32), (1, 3000, BF), (70, 70, F32), (70, 70, BF), (70, 3000, F32), (70, 3000, BF)])
+def test_no_number_in_no_number_out(ops, Lq, S, dtype):
+    """a query that is no number gives a row of none, and only that; an infinite value or key is seen in every row that sees it"""
+    B, H, dh = 2, 2, 32
+    q, k, v, g = mk(26, B, H, H, Lq, S, dh, dtype)
+    rp = ops.relpos()
+    table = torch.randn(32, H, generator=g).cuda()
+    good = ops.attention_relpos(q, k, v, table, rp, H)
+    bad = q.clone()
+    bad[1, Lq // 2, :dh] = math.nan
+    o = ops.attention_relpos(bad, k, v, table, rp, H)
+    assert torch.isnan(o[1, Lq // 2, :dh]).all()
+    o[1, Lq // 2, :dh] = good[1, Lq // 2, :dh]
+    assert torch.equal(o, good)
+    for t in (k, v) if Lq > 1 else (v,):                             # (a single query's score of an infinite key may be -inf: no weight)
+        w = t.clone()
+        w[1, 5, 3] = math.inf
+        o = ops.attention_relpos(q, w if t is k else k, w if t is v else v, table, rp, H)
+        assert not torch.isfinite(o[1, :, 3]).any() if t is v else not torch.isfinite(o[1, :, :dh]).all(-1).all()
+        assert torch.equal(o[0], good[0]) and torch.equal(o[1, :, dh:], good[1, :, dh:])
+
+
+def test_two_calls_at_once(ops):
+    """calls on two streams, each with workspaces of its own"""
+    B, H, S, dh = 2, 2, 1300, 64
+    q, k, v, g = mk(23, B, H, H, S, S, dh)
+    q2, k2, v2, _ = mk(24, B, H, H, S, S, dh)
+    rp = ops.relpos()
+    table = torch.randn(32, H, generator=g).cuda()
+    want = ops.attention_relpos(q, k, v, table, rp, H).clone(), ops.attention_relpos(q2, k2, v2, table, rp, H).clone()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            x = ops.attention_relpos(q, k, v, table, rp, H)
+        with torch.cuda.stream(b):
+            y = ops.attention_relpos(q2, k2, v2, table, rp, H)
+        torch.cuda.synchronize()
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
+def test_profile_names_the_launch(ops):
+    rp, z = ops.relpos(), torch.zeros(1, 40, 64, device="cuda")
+    with ops.profile() as rec:
+        ops.attention_relpos(z, z, z, torch.zeros(32, 2, device="cuda"), rp, 2)
+        ops.norm_residual(z, z)
+    assert [r[0] for r in rec.rows] == ["attention_relpos", "norm_residual"] and rec.rows[0][1]["flops"] > 0 and rec.rows[1][1]["bytes"] > 0
 
 
 def test_single_tokens_answer_what_the_prompt_answers(ops):
