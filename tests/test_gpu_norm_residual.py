@@ -204,6 +204,26 @@ def test_a_gate_row_for_every_token(ops, T):
         assert rel(a, ref[b]) < 4 * tol(E, n, F32, True), b
 
 
+def test_one_parameter_in_two_places(ops, T):
+    """tied norms: a parameter's gradient is the sum of both places'; a gate that is a norm's scale too"""
+    from synergize_motion_appearance_amd.tape import Tape
+    n, E = 900, 100
+    w, g = mk(11, n, E, F32, "layer", True, True, 0)
+    gx, gy = (torch.randn(n, E, generator=g).cuda() for _ in range(2))
+    P = {"a": w["post"][0], "b": w["post"][1]}
+    for gate in (None, "a"):
+        G = {k: torch.zeros_like(t) for k, t in P.items()}
+        tp = Tape(P, G)
+        xo, y = T.norm_residual(tp, w["x"], w["x"], post=("a", "b"), pre=("a", "b"), gate=gate)
+        tp.acc(xo, gx, owned=False)
+        tp.acc(y, gy, owned=False)
+        tp.backward()
+        ref = R.norm_residual(w["x"], w["x"], post=w["post"], pre=w["post"], gate=None if gate is None else w["post"][0], gx=gx, gy=gy)
+        t = 8 * tol(E, n, F32, True)
+        a = ref["dpost0"] + ref["dpre0"] + (0 if gate is None else ref["dgate"].view(E))
+        assert rel(G["a"], a) < t and rel(G["b"], ref["dpost1"] + ref["dpre1"]) < t and rel(tp.grad(w["x"]), ref["dx"] + ref["dh"]) < t
+
+
 def test_refusals(ops):
     w, _ = mk(6, 12, 64, F32, "layer", True, True, 3)
     for bad in (dict(x=w["x"].half()), dict(h=w["h"].bfloat16()), dict(h=w["h"][:6]), dict(x=w["x"][:, ::2], h=w["h"][:, ::2]), dict(kind="batch"),
