@@ -89,7 +89,8 @@ __device__ __forceinline__ void stats2(Lanes<LPR>& ln, const float (&a)[NV], con
 
 // Forward: x and h are read once, x' and y written once; a row stays in its lanes' registers between the two norms.  With up to 8 columns a lane
 // the parameters stay there too (five rows of fp32 against four of data: read again for every row they would be most of a CU's loads).
-// 61440 x 1280 bf16: 131 us, 4.8 TB/s; one token of 256: 11 us, the launch and the caller's own work.
+// 307200 x 256 bf16: 131 us, 4.8 TB/s; 15999 x 2048 fp32: 98 us, 5.4 TB/s; 8 x 4096 bf16: 11 us, the launch and the caller's own work.  Parameters read again for
+// every row: 45 us instead of 43 at 65536 x 256 fp32.
 template <typename TS, int V, int LPR, int N>
 __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
   constexpr int NV = N * V;
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
 
 // Backward: a block walks `rows` tokens of one gate row, each thread keeping its columns' five parameter sums in registers; the block's sums go to
 // part [groups * nblk][5][E] (dpre gamma, dpre beta, dpost gamma, dpost beta, dgate; those that are wanted), norm_residual_sum_kernel adds the blocks.
-// @@BWD@@
+// 15999 x 2048, six rows of fp32 a token, 786 MB: 189 us, 4.2 TB/s, with 7 us for the blocks' sums.
 template <int V, int LPR, int N>
 __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p) {
   constexpr int NV = N * V, BT = Lanes<LPR>::BT, RPB = Lanes<LPR>::RPB;
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
   for (int k = 0; k < NV; ++k) in[k] = (ln.sub + LPR * (k / V)) * V < p.E;
   const long long t1 = g * p.per + min(p.per, (blk + 1) * (long long)p.rows);
   const float iE = 1.f / p.E;
-  constexpr bool AHEAD = NV <= 8;                    // the next row is on its way during this one's sums
+  constexpr bool AHEAD = NV <= 8;                    // the next row is on its way during this one's sums (with the forward, 65536 x 256: 151 us instead of 194)
   float row[2][4][NV];
   auto load = [&](float (&w)[4][NV], long long t) {
     const long long at = t * p.E;
@@ -330,8 +331,8 @@ __global__ __launch_bounds__(1024) void norm_residual_sum_kernel(const float* __
 }
 
 // Lanes a row and chunks a lane, by the row's 16-byte chunks (columns where rows do not start on 16 bytes): up to a wave's 64 lanes one chunk each, then up to 4
-// a lane, then rows over a block -- of 256 threads for up to 1024 chunks, 512 beyond, so that the backward's five sums of a thread's columns stay
-// in registers.
+// a lane (256 chunks over 256 lanes with their barriers: 52 us instead of 44 at 16384 x 1024 fp32), then rows over a block -- of 256 threads for up to 1024
+// chunks, 512 beyond, so that the backward's five sums of a thread's columns stay in registers.
 template <typename TS, int V, template <typename, int, int, int> class K>
 int by_width(const NRP& p, hipStream_t st) {
   const int n = smx_cdiv(p.E, V);
@@ -365,9 +366,12 @@ template <typename TS, int V, int LPR, int N> struct Bwd {
   }
 };
 
-// tokens a backward block walks: about 512 blocks (their sums are written and read once more), but not fewer tokens than it has rows at a time
+// tokens a backward block walks: about 512 blocks (their sums are written and read once more), 256 of rows that take a block of 512 threads -- one a CU at a time
+// --, but not fewer tokens than it has rows at a time.  Forward and backward with 256 / 512 / 1024 blocks: 65536 x 256 195 / 151 / 144 us, 8192 x 2048
+// 177 / 148 / 158, 4096 x 4096 178 / 160 / 181, 2048 x 8192 194 / 218 / 234, 1024 x 16384 378 / 421 / 499.
 int rows_of(long long T, long long per, int E) {
-  long long r = (T + 511) / 512;
+  const int want = E > 4096 ? 256 : 512;
+  long long r = (T + want - 1) / want;
   const int at_a_time = E <= 32 ? 32 : E <= 64 ? 16 : E <= 128 ? 8 : E <= 1024 ? 4 : 1;
   if (r < at_a_time) r = at_a_time;
   if (r > per) r = per;
