@@ -223,7 +223,8 @@ __device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned n) {
 
 // Which of a head's n blocks, and which of the heads, a block works on.  Blocks of one length: runs of heads by XCD.  With a causal rule a head's blocks differ, 0 the
 // longest: all heads' longest go first (a chip that ends on long blocks waits for them: 1.3 waves a SIMD on average instead of 1.9), the heads of one XCD
-// consecutive ones where they are a multiple of 8.  Ragged samples: heads in turn, so that no XCD has only the short ones.
+// consecutive ones where they are a multiple of 8: 2 x 16 heads of 8192 x 8192 bf16 368 us instead of 405, 4096 x 4096 with its backward 1144 instead
+// of 1235.  Ragged samples: heads in turn, so that no XCD has only the short ones (3 x 6 heads of 1311 and fewer keys: 63 us instead of 84).
 struct Work { int i, head; };
 __device__ __forceinline__ Work work_of(unsigned id, int n, int heads, int causal, bool ragged) {
   if (!causal && !ragged) { id = xcd_order(id, gridDim.x); return {(int)(id % n), (int)(id / n)}; }

@@ -12,7 +12,8 @@ namespace relpos {
 // ---- fp32 operands as halves (relpos.h: Split) ---------------------------------------------------------------------------------
 struct Splits { Split s[4]; int end[4]; };                       // end: running sum of blocks
 
-// 64 rows of one head -> both planes and their 2^-k; gradient rows: D_i = dO_i . o_i too
+// 64 rows of one head -> both planes and their 2^-k; gradient rows: D_i = dO_i . o_i too.  Bound by memory: 2 x 38 x 1024 rows of 8 x 32, 159 MB with the planes,
+// 26 us, 6.2 TB/s (much of it in the 256 MB of cache that all XCDs share).
 template <int DHP>
 __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
   __shared__ float red[4];
@@ -122,7 +123,8 @@ namespace {
 using namespace relpos;
 
 // ---- queries in tiles ----------------------------------------------------------------------------------------------------------
-// two stages of keys in turn, one barrier a step; one where two would leave a CU with one block (fp32 storage, 65 to 96 columns: 106 KB)
+// two stages of keys in turn, one barrier a step; one where two would leave a CU with one block (fp32 storage, 65 to 96 columns: 106 KB).  8 x 16 heads of 1024 x 1024,
+// one / two: fp32 32 columns 98 / 98 us, 64 148 / 148, 96 211 / 243, 128 (in steps of 32 keys) 279 / 279; bf16 64 columns 62.6 / 61.8
 template <int DHP, int NL> constexpr int BUFFERS = NL == 2 && DHP == 96 ? 1 : 2;
 
 // where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage q and the planes of k and v; parts: m, l [row][part], o
@@ -139,6 +141,11 @@ struct Src {
 // Weights are 2^(s - mo), mo finite and followed only when a row outgrows it by 2^8 (and at its first key): the scores leave the products through one fma,
 // and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
+// Bound by the vector units' work on the scores (bias, maximum, 2^x, sum, two halves: some 10 operations each) next to the matrix products, of which only part runs
+// at the same time on 2 or 3 waves a SIMD.  38 x 8 heads of 1024 x 1024 of 32, fp32: 206 us with the split, 198 TFLOP/s of the formula's, 0.47 of
+// what three half-precision products at a large matrix product's rate would take; 2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 358 us, 767 TFLOP/s,
+// 0.61 of that rate.  Three waves a SIMD (bf16 up to 64 columns) against two: 44.7 / 44.9 us for 32 columns, 61.8 / 63.0 for 64.
+// 64 queries a wave instead of 32: 221 us for 205 of that build.
 template <int DHP, int NL>
 __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile_kernel(RP p, Src a) {
   constexpr int TK = STEP<DHP, NL>, NU = TK / 32, KS = DHP / 16, DT = DHP / 32, RB = ROWB<DHP>, NT = 256;
@@ -387,9 +394,11 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
 }
 
 // ---- a few queries per sample ---------------------------------------------------------------------------------------------------
-// A block takes a part of one (sample, kv head)'s keys for RT of its G * L query rows.  LPK lanes hold a key's row, EPL values each, and the same columns of the
+// A block takes a part of one (sample, kv head)'s keys for RT of its G * L query rows (as many passes over the keys as rows / 4, from the caches but the first).  LPK lanes hold a key's row, EPL values each, and the same columns of the
 // RT queries and running outputs; every group of LPK lanes walks keys of its own, four a step, with a running maximum and sum of its own: the only
-// exchanges are the LPK-lane sums of the scores.  The groups are joined through LDS at the end, the parts by relpos_join_kernel.
+// exchanges are the LPK-lane sums of the scores.  The groups are joined through LDS at the end, the parts by relpos_join_kernel.  Bound by the keys' and values'
+// bytes: 16 ragged samples of up to 32768 keys, 4 kv heads of 64 for 16, bf16, 411 MB: 105 us, 3.9 TB/s; for short caches by the launch and
+// the caller's own work (8 samples of 300 keys: 12 us).
 template <typename T, int EPL> struct Row;                       // EPL values as they lie in memory
 template <> struct Row<float, 4> {
   typedef float Raw __attribute__((ext_vector_type(4)));
@@ -564,31 +573,42 @@ __global__ __launch_bounds__(256) void relpos_token_kernel(RP p, Src a) {
 }
 
 // o = sum 2^(m_t - m) o_t / sum 2^(m_t - m) l_t over the parts.  8, 16 or 32 lanes hold a row's columns, four each; up to 8 parts go by one after the other and a
-// wave has several rows, more are dealt to runs of lanes and joined by shuffles.
+// wave has several rows, more are dealt to runs of lanes and joined by shuffles.  The lanes of a row first take a part each for m and the sum of l; the
+// parts' rows follow with four loads in flight (one at a time, 128 parts of 16 rows took longer than the pass over the 67 MB of their keys).
 template <typename T>
 __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
-  const int lanes = p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32, runs = a.nparts <= 8 ? 1 : 64 / lanes, per = lanes * runs;
-  const int lane = threadIdx.x & 63, run = lane % per / lanes, c = lane % lanes * 4;
+  const int lanes = p.dh <= 32 ? 8 : p.dh <= 64 ? 16 : 32, runs = a.nparts <= 8 ? 1 : 64 / lanes, per = lanes * runs, n = a.nparts;
+  const int lane = threadIdx.x & 63, at = lane % per, run = at / lanes, c = lane % lanes * 4;
   const long long row = (blockIdx.x * 4LL + (threadIdx.x >> 6)) * (64 / per) + lane / per;
   if (row >= (long long)p.B * p.H * p.L) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.nparts;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * n;
   float m = -INFINITY;
-  for (int s = run; s < a.nparts; s += runs) m = fmaxf(m, ml[s].x);
-  for (int o = lanes; o < per; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  for (int s = at; s < n; s += per) m = fmaxf(m, ml[s].x);
+  for (int o = 1; o < per; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float mf = m == -INFINITY ? 0.f : m;
   float l = 0.f, x = 0.f, y = 0.f, z = 0.f, w = 0.f;
-  for (int s = run; s < a.nparts; s += runs) {
-    const float2 t = ml[s];
-    const float f = __builtin_amdgcn_exp2f(t.x - mf);
-    l += f * t.y;
-    if (c < p.dh && f > 0.f) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (row * a.nparts + s) * p.dh + c);
-      x += f * v.x; y += f * v.y; z += f * v.z; w += f * v.w;
+  for (int s = at; s < n; s += per) { const float2 t = ml[s]; l += __builtin_amdgcn_exp2f(t.x - mf) * t.y; }
+  for (int o = 1; o < per; o <<= 1) l += __shfl_xor(l, o, 64);
+  if (c < p.dh) {
+    const float* O = a.part_o + row * n * p.dh + c;
+    for (int s0 = run; s0 < n; s0 += 4 * runs) {
+      float f[4];
+      float4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = min(s0 + u * runs, n - 1);
+        f[u] = ml[s].x;
+        v[u] = *reinterpret_cast<const float4*>(O + (long long)s * p.dh);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (s0 + u * runs >= n) break;
+        const float e = __builtin_amdgcn_exp2f(f[u] - mf);
+        x += e * v[u].x; y += e * v[u].y; z += e * v[u].z; w += e * v[u].w;
+      }
     }
   }
-  for (int o = lanes; o < per; o <<= 1) {
-    l += __shfl_xor(l, o, 64); x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); z += __shfl_xor(z, o, 64); w += __shfl_xor(w, o, 64);
-  }
+  for (int o = lanes; o < per; o <<= 1) { x += __shfl_xor(x, o, 64); y += __shfl_xor(y, o, 64); z += __shfl_xor(z, o, 64); w += __shfl_xor(w, o, 64); }
   if (run) return;
   const float il = l == 0.f ? 0.f : 1.f / l;
   const int i = (int)(row % p.L), h = (int)(row / p.L % p.H);
@@ -600,14 +620,19 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RP p, Src a) {
 // ---- which kernel, in how many parts ---------------------------------------------------------------------------------------------
 struct Plan { bool token; int nparts, per, rt; long long blocks; int64_t split_ws, part_ws; };
 
+// Which kernel.  The token kernel's time grows with the rows that share a key (four at a time), the tile kernel's does not up to 32 queries, but fp32 storage has
+// its keys split first.  16 heads of 64, 4 x 4096 keys, us, token / tile: fp32 16 kv heads, 1 query 29 / 82, 4 42 / 82, 8 63 / 82, 32 269 / 86; 4 kv heads, 1 21 / 41, 2 26 / 41,
+// 3 35 / 41, 4 42 / 41, 8 62 / 41; 1 kv head, 1 21 / 34, 2 28 / 33, 3 35 / 34.  bf16 16 kv heads, 1 query 20 / 22, 2 26 / 23, 3 33 / 23; 4 kv heads, 1 19 / 20, 2 21 / 19, 3 31 / 21.
+// Likewise at 8 x 1024 keys of 32, 2 x 8192 of 128 and 32768 of 64.
 Plan plan(const smx_relpos_desc* d, const RP& p) {
   Plan w;
-  w.token = p.L <= 8;
+  const long long rows = (long long)p.G * p.L;
+  w.token = d->bf16 ? p.L == 1 : p.L <= 2 || (p.L <= 12 && rows <= 12);
   w.split_ws = 0;
-  const int rows = p.G * p.L;
-  w.rt = rows >= 8 ? 8 : rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
+  w.rt = rows >= 3 ? 4 : (int)rows;                                   // (8 at a time: 8 rows 110 us instead of 63)
   const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
-  // parts of the keys from 513 keys on, none shorter than 256, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four)
+  // parts of the keys from 513 keys on, none shorter than 256, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four).  In
+  // parts / not, 8 heads of 64: 1024 queries on 4096 keys fp32 52 / 130 us, 128 on 8192 bf16 22 / 154, 1 on 4096 fp32 15 / 64
   long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = p.S <= 512 ? 1 : (p.S + 255) / 256;
   if (np > most) np = most;
   w.per = (int)(((p.S + np - 1) / np + 63) / 64 * 64);
@@ -630,8 +655,7 @@ template <typename T, int EPL, int LPK>
 int token_launch(const RP& p, const Src& a, const Plan& w, hipStream_t st) {
   const int lds = 4 * w.rt * (LPK * EPL + 2) * 4;
   const dim3 grid((unsigned)w.blocks), block(256);
-  if (w.rt == 8) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 8>), grid, block, lds, st, p, a);
-  else if (w.rt == 4) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 4>), grid, block, lds, st, p, a);
+  if (w.rt == 4) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 4>), grid, block, lds, st, p, a);
   else if (w.rt == 2) SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 2>), grid, block, lds, st, p, a);
   else SMX_LAUNCH((relpos_token_kernel<T, EPL, LPK, 1>), grid, block, lds, st, p, a);
   return smx_launch_status();

@@ -68,9 +68,11 @@ FORWARD = [
     (3, 2, 2, 257, 700, 64, True, False, True, False),
     (1, 3, 1, 1100, 1100, 4, False, False, False, False),
     (2, 8, 4, 385, 385, 32, True, False, False, False),          # 16 heads: their order over the XCDs
-    (1, 8, 8, 8, 2000, 100, True, True, False, False),           # the most queries a token call takes, keys in parts
-    (1, 1, 1, 9, 2000, 100, True, True, False, False),           # the fewest a tile call takes
-    (1, 16, 1, 3, 700, 64, False, False, False, False),          # more query rows on a kv head than one block takes
+    (1, 8, 8, 12, 2000, 100, True, True, False, False),          # the most query rows a kv head that fp32 token calls of more than two queries take
+    (1, 1, 1, 13, 2000, 100, True, True, False, False),          # the fewest a tile call takes
+    (1, 16, 1, 2, 700, 64, False, True, False, False),           # more query rows on a kv head than one block takes
+    (2, 6, 2, 1, 700, 64, True, False, True, False),             # rows that leave some of a block's unused
+    (1, 16, 1, 3, 700, 64, False, False, False, False),
 ]
 
 
