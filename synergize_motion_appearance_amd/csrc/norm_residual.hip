@@ -23,7 +23,7 @@ struct NRP {
 };
 
 // LPR lanes hold a row: lane `sub` the V columns of chunks sub, sub + LPR, ... (N of them); a block of BT threads BT / LPR rows at a time.  V is 16 bytes
-// of the storage type, 1 where rows do not start on 16 bytes.
+// of the storage type.
 template <int LPR>
 struct Lanes {
   static constexpr int BT = LPR > 256 ? LPR : 256, RPB = BT / LPR, W = LPR / 64;
@@ -46,25 +46,64 @@ struct Lanes {
   }
 };
 
-template <typename TS, int V> __device__ __forceinline__ void ldv(const TS* p, float* f) {
-  if constexpr (V == 8) { float g[8]; unpack8(*reinterpret_cast<const uint4*>(p), g);
+// U: rows start anywhere and end inside a chunk.  The same 16-byte accesses then, which the card makes at any address of the type; a row's last chunk, of which
+// not all columns are there, is read column by column -- or (S), where the next row is on its way while this one is summed and a branch would wait for it,
+// from `back` columns before, and moved down once it has arrived, zeros behind it.  Forward and backward, us, all rows column by column / last chunks / S:
+// 65536 x 250 183 / 258 / 168, 8192 x 1026 179 / 133 / 128, 2658 x 2470 175 / 90 / 126, 4096 x 4098 729 / 234 / 287 (S: more registers than two waves a SIMD have).
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u4u __attribute__((ext_vector_type(4), aligned(2)));
+template <int V, bool S> __device__ __forceinline__ int back_of(int E, int c) { return S && E >= V ? max(0, c + V - E) : 0; }
+template <typename TS, int V, bool U, bool S> __device__ __forceinline__ void ldr(const TS* row, int c, int E, float* f) {
+  const TS* p = row + c - back_of<V, S>(E, c);
+  if (U && (S ? E : E - c) < V) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = g[e]; }
-  else if constexpr (V == 4) { const float4 v = St<TS>::ld4(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
-  else f[0] = St<TS>::ld(p);
+    for (int e = 0; e < V; ++e) f[e] = e < E - c ? St<TS>::ld(row + c + e) : 0.f;
+  } else if constexpr (sizeof(TS) == 2) {
+    float g[8];
+    if constexpr (U) { const u4u x = *reinterpret_cast<const u4u*>(p); unpack8(make_uint4(x.x, x.y, x.z, x.w), g); }
+    else unpack8(*reinterpret_cast<const uint4*>(p), g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = g[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      if constexpr (U) { const f4u v = *reinterpret_cast<const f4u*>(p + e); f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w; }
+      else { const float4 v = St<float>::ld4((const float*)p + e); f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w; }
+    }
+  }
 }
-template <typename TS, int V> __device__ __forceinline__ void stv(TS* p, const float* f) {
-  if constexpr (V == 8) { const float g[8] = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}; *reinterpret_cast<uint4*>(p) = pack8(g); }
-  else if constexpr (V == 4) St<TS>::st4(p, make_float4(f[0], f[1], f[2], f[3]));
-  else St<TS>::st(p, f[0]);
+template <int V, bool S> __device__ __forceinline__ void down(float* f, int back) {
+  if (!S || !back) return;
+#pragma unroll
+  for (int b = 1; b < V; b <<= 1)
+    if (back & b) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = e + b < V ? f[e + b] : 0.f;
+    }
+}
+template <typename TS, int V, bool U> __device__ __forceinline__ void stv(TS* row, int c, int E, const float* f) {
+  TS* p = row + c;
+  if (U && E - c < V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < E - c) St<TS>::st(p + e, f[e]);
+  } else if constexpr (V == 8) {
+    const float g[8] = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+    const uint4 x = pack8(g);
+    if constexpr (U) *reinterpret_cast<u4u*>(p) = u4u{x.x, x.y, x.z, x.w};
+    else *reinterpret_cast<uint4*>(p) = x;
+  } else if constexpr (U) *reinterpret_cast<f4u*>(p) = f4u{f[0], f[1], f[2], f[3]};
+  else St<TS>::st4(p, make_float4(f[0], f[1], f[2], f[3]));
 }
 // V fp32 parameters, `other` without them
-template <int V> __device__ __forceinline__ void ldp(const float* p, int c, float other, float* f) {
+template <int V, bool U, bool S> __device__ __forceinline__ void ldp(const float* p, int c, int E, float other, float* f) {
   if (!p) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = other;
-  } else if constexpr (V == 8) { ldv<float, 4>(p + c, f); ldv<float, 4>(p + c + 4, f + 4); }
-  else ldv<float, V>(p + c, f);
+  } else {
+    ldr<float, V, U, S>(p, c, E, f);
+    down<V, S>(f, back_of<V, S>(E, c));
+  }
 }
 
 // mean and 1 / sqrt(var + eps) of two rows at a time (b unused: pass zeros): the sums first, then the squares of the deviations -- never a difference of
@@ -91,7 +130,7 @@ __device__ __forceinline__ void stats2(Lanes<LPR>& ln, const float (&a)[NV], con
 // the parameters stay there too (five rows of fp32 against four of data: read again for every row they would be most of a CU's loads).
 // 307200 x 256 bf16: 131 us, 4.8 TB/s; 15999 x 2048 fp32: 98 us, 5.4 TB/s; 8 x 4096 bf16: 11 us, the launch and the caller's own work.  Parameters read again for
 // every row: 45 us instead of 43 at 65536 x 256 fp32.
-template <typename TS, int V, int LPR, int N>
+template <typename TS, int V, int LPR, int N, bool U>
 __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
   constexpr int NV = N * V;
   constexpr bool HOLD = NV <= 8;
@@ -103,10 +142,10 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
   for (int k = 0; k < N; ++k) {
     const int c = (ln.sub + LPR * k) * V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) in[k * V + e] = c < p.E;
+    for (int e = 0; e < V; ++e) in[k * V + e] = c + (U ? e : 0) < p.E;
     if constexpr (HOLD)
-      if (c < p.E) { ldp<V>(p.pg, c, 1.f, pg + k * V); ldp<V>(p.pb, c, 0.f, pb + k * V); ldp<V>(p.ng, c, 1.f, ng + k * V); ldp<V>(p.nb, c, 0.f, nb + k * V);
-                     ldp<V>(p.per == p.T ? p.gate : nullptr, c, 1.f, gt + k * V); }
+      if (c < p.E) { ldp<V, U, false>(p.pg, c, p.E, 1.f, pg + k * V); ldp<V, U, false>(p.pb, c, p.E, 0.f, pb + k * V); ldp<V, U, false>(p.ng, c, p.E, 1.f, ng + k * V); ldp<V, U, false>(p.nb, c, p.E, 0.f, nb + k * V);
+                     ldp<V, U, false>(p.per == p.T ? p.gate : nullptr, c, p.E, 1.f, gt + k * V); }
   }
   const bool same_gate = HOLD && p.per == p.T;
   for (long long t = blockIdx.x * (long long)Lanes<LPR>::RPB + ln.row; t < p.T; t += (long long)gridDim.x * Lanes<LPR>::RPB) {
@@ -118,7 +157,9 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
       const int c = (ln.sub + LPR * k) * V;
 #pragma unroll
       for (int e = 0; e < V; ++e) x[k * V + e] = v[k * V + e] = zero[k * V + e] = 0.f;
-      if (c < p.E) { ldv<TS, V>((const TS*)p.x + at + c, x + k * V); ldv<TS, V>((const TS*)p.h + at + c, v + k * V); }
+      if (c < p.E) {
+        ldr<TS, V, U, false>((const TS*)p.x + at, c, p.E, x + k * V); ldr<TS, V, U, false>((const TS*)p.h + at, c, p.E, v + k * V);
+      }
     }
     float mean = 0.f, r = 1.f, m2, r2;
     if (p.pg) stats2<NV, LPR>(ln, v, zero, in, p.E, p.rms, p.eps, mean, r, m2, r2);
@@ -130,8 +171,8 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
         if constexpr (HOLD) {
 #pragma unroll
           for (int e = 0; e < V; ++e) { a[e] = pg[k * V + e]; b[e] = pb[k * V + e]; g[e] = gt[k * V + e]; }
-        } else { ldp<V>(p.pg, c, 1.f, a); ldp<V>(p.pb, c, 0.f, b); }
-        if (!same_gate) ldp<V>(gate, c, 1.f, g);
+        } else { ldp<V, U, false>(p.pg, c, p.E, 1.f, a); ldp<V, U, false>(p.pb, c, p.E, 0.f, b); }
+        if (!same_gate) ldp<V, U, false>(gate, c, p.E, 1.f, g);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float n = fmaf((v[k * V + e] - mean) * r, a[e], b[e]);
@@ -139,7 +180,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
           St<TS>::st(&w, fmaf(g[e], n, p.rs * x[k * V + e]));
           v[k * V + e] = St<TS>::ld(&w);             // y is the norm of what is stored
         }
-        stv<TS, V>((TS*)p.xo + at + c, v + k * V);
+        stv<TS, V, U>((TS*)p.xo + at, c, p.E, v + k * V);
       }
     }
     if (!p.y) continue;
@@ -152,10 +193,10 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
         if constexpr (HOLD) {
 #pragma unroll
           for (int e = 0; e < V; ++e) { a[e] = ng[k * V + e]; b[e] = nb[k * V + e]; }
-        } else { ldp<V>(p.ng, c, 1.f, a); ldp<V>(p.nb, c, 0.f, b); }
+        } else { ldp<V, U, false>(p.ng, c, p.E, 1.f, a); ldp<V, U, false>(p.nb, c, p.E, 0.f, b); }
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k * V + e] = fmaf((v[k * V + e] - mean) * r, a[e], b[e]);
-        stv<TS, V>((TS*)p.y + at + c, v + k * V);
+        stv<TS, V, U>((TS*)p.y + at, c, p.E, v + k * V);
       }
     }
   }
@@ -164,7 +205,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_kernel(NRP p) {
 // Backward: a block walks `rows` tokens of one gate row, each thread keeping its columns' five parameter sums in registers; the block's sums go to
 // part [groups * nblk][5][E] (dpre gamma, dpre beta, dpost gamma, dpost beta, dgate; those that are wanted), norm_residual_sum_kernel adds the blocks.
 // 15999 x 2048, six rows of fp32 a token, 786 MB: 189 us, 4.2 TB/s, with 7 us for the blocks' sums.
-template <int V, int LPR, int N>
+template <int V, int LPR, int N, bool U>
 __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p) {
   constexpr int NV = N * V, BT = Lanes<LPR>::BT, RPB = Lanes<LPR>::RPB;
   __shared__ float2 red[2 * (LPR > 64 ? LPR / 64 : 1)];
@@ -179,10 +220,11 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
 #pragma unroll
     for (int k = 0; k < NV; ++k) a[i][k] = 0.f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) in[k] = (ln.sub + LPR * (k / V)) * V < p.E;
+  for (int k = 0; k < NV; ++k) in[k] = (ln.sub + LPR * (k / V)) * V + (U ? k % V : 0) < p.E;
   const long long t1 = g * p.per + min(p.per, (blk + 1) * (long long)p.rows);
   const float iE = 1.f / p.E;
   constexpr bool AHEAD = NV <= 8;                    // the next row is on its way during this one's sums (with the forward, 65536 x 256: 151 us instead of 194)
+  constexpr bool SH = U && AHEAD;
   float row[2][4][NV];
   auto load = [&](float (&w)[4][NV], long long t) {
     const long long at = t * p.E;
@@ -194,9 +236,9 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
 #pragma unroll
         for (int e = 0; e < V; ++e) w[i][k * V + e] = 0.f;
       if (col < p.E) {
-        ldv<float, V>((const float*)p.h + at + col, w[1] + k * V);
-        if (p.gx) ldv<float, V>(p.gx + at + col, w[2] + k * V);
-        if (p.gy) { ldv<float, V>((const float*)p.xo + at + col, w[0] + k * V); ldv<float, V>(p.gy + at + col, w[3] + k * V); }
+        ldr<float, V, U, SH>((const float*)p.h + at, col, p.E, w[1] + k * V);
+        if (p.gx) ldr<float, V, U, SH>(p.gx + at, col, p.E, w[2] + k * V);
+        if (p.gy) { ldr<float, V, U, SH>((const float*)p.xo + at, col, p.E, w[0] + k * V); ldr<float, V, U, SH>(p.gy + at, col, p.E, w[3] + k * V); }
       }
     }
   };
@@ -215,6 +257,12 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
         for (int k = 0; k < NV; ++k) row[0][i][k] = row[1][i][k];
       if (t + RPB < t1) load(row[1], t + RPB);
     } else load(row[0], t);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int col = (ln.sub + LPR * k) * V;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) down<V, SH>(row[0][i] + k * V, col < p.E ? back_of<V, SH>(p.E, col) : 0);
+    }
     float mx, rx, mh, rh, s1 = 0.f, s2 = 0.f;
     stats2<NV, LPR>(ln, x, h, in, p.E, p.rms, p.eps, mx, rx, mh, rh);
     if (p.gy) {
@@ -223,7 +271,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
         const int col = (ln.sub + LPR * k) * V;
         float w[V];
         if (col < p.E) {
-          ldp<V>(p.ng, col, 1.f, w);
+          ldp<V, U, SH>(p.ng, col, p.E, 1.f, w);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const int i = k * V + e;
@@ -246,7 +294,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
         float w[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) w[e] = p.rs * c[k * V + e];
-        if (col < p.E) stv<float, V>(p.dx + at + col, w);
+        if (col < p.E) stv<float, V, U>(p.dx + at, col, p.E, w);
       }
     }
     s1 = s2 = 0.f;
@@ -255,7 +303,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
       const int col = (ln.sub + LPR * k) * V;
       float w[V], b[V], gt[V];
       if (col < p.E) {
-        ldp<V>(p.pg, col, 1.f, w); ldp<V>(p.pb, col, 0.f, b); ldp<V>(gate, col, 1.f, gt);
+        ldp<V, U, SH>(p.pg, col, p.E, 1.f, w); ldp<V, U, SH>(p.pb, col, p.E, 0.f, b); ldp<V, U, SH>(gate, col, p.E, 1.f, gt);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const int i = k * V + e;
@@ -276,7 +324,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
     }
     if (p.dh) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V>(p.dh + at + col, c + k * V); }
+      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V, U>(p.dh + at, col, p.E, c + k * V); }
     }
   }
   float* part = p.part + (long long)blockIdx.x * 5 * p.E;
@@ -285,7 +333,7 @@ __global__ __launch_bounds__(Lanes<LPR>::BT) void norm_residual_bwd_kernel(NRP p
     if (!(p.want >> i & 1)) continue;
     if constexpr (LPR > 64) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V>(part + (long long)i * p.E + col, a[i] + k * V); }
+      for (int k = 0; k < N; ++k) { const int col = (ln.sub + LPR * k) * V; if (col < p.E) stv<float, V, U>(part + (long long)i * p.E, col, p.E, a[i] + k * V); }
     } else {                                         // the rows of a wave by shuffles, its four waves through LDS
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -330,38 +378,35 @@ __global__ __launch_bounds__(1024) void norm_residual_sum_kernel(const float* __
   else out[g * E + e] = gate_acc ? out[g * E + e] + s : s;
 }
 
-// Lanes a row and chunks a lane, by the row's 16-byte chunks (columns where rows do not start on 16 bytes): up to a wave's 64 lanes one chunk each, then up to 4
+// Lanes a row and chunks a lane, by the row's 16-byte chunks: up to a wave's 64 lanes one chunk each, then up to 4
 // a lane (256 chunks over 256 lanes with their barriers: 52 us instead of 44 at 16384 x 1024 fp32), then rows over a block -- of 256 threads for up to 1024
 // chunks, 512 beyond, so that the backward's five sums of a thread's columns stay in registers.
-template <typename TS, int V, template <typename, int, int, int> class K>
+template <typename TS, int V, bool U, template <typename, int, int, int, bool> class K>
 int by_width(const NRP& p, hipStream_t st) {
   const int n = smx_cdiv(p.E, V);
-  if (n <= 8) return K<TS, V, 8, 1>::go(p, st);
-  if (n <= 16) return K<TS, V, 16, 1>::go(p, st);
-  if (n <= 32) return K<TS, V, 32, 1>::go(p, st);
-  if (n <= 64) return K<TS, V, 64, 1>::go(p, st);
-  if (n <= 128) return K<TS, V, 64, 2>::go(p, st);
-  if (n <= 256) return K<TS, V, 64, 4>::go(p, st);
-  if (n <= 512) return K<TS, V, 256, 2>::go(p, st);
-  if (n <= 1024) return K<TS, V, 256, 4>::go(p, st);
-  if (n <= 2048) return K<TS, V, 512, 4>::go(p, st);
-  if constexpr (V < 8) {
-    if (n <= 4096) return K<TS, V, 512, 8>::go(p, st);
-    if constexpr (V == 1) return n <= 8192 ? K<TS, V, 512, 16>::go(p, st) : K<TS, V, 512, 32>::go(p, st);
-  }
+  if (n <= 8) return K<TS, V, 8, 1, U>::go(p, st);
+  if (n <= 16) return K<TS, V, 16, 1, U>::go(p, st);
+  if (n <= 32) return K<TS, V, 32, 1, U>::go(p, st);
+  if (n <= 64) return K<TS, V, 64, 1, U>::go(p, st);
+  if (n <= 128) return K<TS, V, 64, 2, U>::go(p, st);
+  if (n <= 256) return K<TS, V, 64, 4, U>::go(p, st);
+  if (n <= 512) return K<TS, V, 256, 2, U>::go(p, st);
+  if (n <= 1024) return K<TS, V, 256, 4, U>::go(p, st);
+  if (n <= 2048) return K<TS, V, 512, 4, U>::go(p, st);
+  if constexpr (V == 4) return K<TS, V, 512, 8, U>::go(p, st);
   return SMX_EINVAL;
 }
 
-template <typename TS, int V, int LPR, int N> struct Fwd {
+template <typename TS, int V, int LPR, int N, bool U> struct Fwd {
   static int go(const NRP& p, hipStream_t st) {
     const long long need = (p.T + Lanes<LPR>::RPB - 1) / Lanes<LPR>::RPB;
-    SMX_LAUNCH((norm_residual_kernel<TS, V, LPR, N>), dim3((unsigned)(need < 4096 ? need : 4096)), dim3(Lanes<LPR>::BT), 0, st, p);
+    SMX_LAUNCH((norm_residual_kernel<TS, V, LPR, N, U>), dim3((unsigned)(need < 4096 ? need : 4096)), dim3(Lanes<LPR>::BT), 0, st, p);
     return smx_launch_status();
   }
 };
-template <typename TS, int V, int LPR, int N> struct Bwd {
+template <typename TS, int V, int LPR, int N, bool U> struct Bwd {
   static int go(const NRP& p, hipStream_t st) {
-    SMX_LAUNCH((norm_residual_bwd_kernel<V, LPR, N>), dim3((unsigned)(p.T / p.per * p.nblk)), dim3(Lanes<LPR>::BT), 0, st, p);
+    SMX_LAUNCH((norm_residual_bwd_kernel<V, LPR, N, U>), dim3((unsigned)(p.T / p.per * p.nblk)), dim3(Lanes<LPR>::BT), 0, st, p);
     return smx_launch_status();
   }
 };
@@ -409,8 +454,8 @@ extern "C" int smx_norm_residual(const smx_norm_residual_desc* d, void* stream) 
   const NRP p = params(d);
   hipStream_t st = (hipStream_t)stream;
   const bool w = wide(p.E, d->bf16 ? 2 : 4, {p.x, p.h, p.xo, p.y, p.pg, p.pb, p.ng, p.nb, p.gate});
-  if (d->bf16) return w ? by_width<bf16_t, 8, Fwd>(p, st) : by_width<bf16_t, 1, Fwd>(p, st);
-  return w ? by_width<float, 4, Fwd>(p, st) : by_width<float, 1, Fwd>(p, st);
+  if (d->bf16) return w ? by_width<bf16_t, 8, false, Fwd>(p, st) : by_width<bf16_t, 8, true, Fwd>(p, st);
+  return w ? by_width<float, 4, false, Fwd>(p, st) : by_width<float, 4, true, Fwd>(p, st);
 }
 
 extern "C" int64_t smx_norm_residual_bwd_ws_floats(int64_t T, int64_t groups, int E) {
@@ -427,7 +472,7 @@ extern "C" int smx_norm_residual_bwd_f32(const smx_norm_residual_desc* d, void* 
   if (!d->ws || ((uintptr_t)d->ws & 15) || d->ws_floats < smx_norm_residual_bwd_ws_floats(d->T, d->groups, d->E)) return SMX_EINVAL;
   const NRP p = params(d);
   hipStream_t st = (hipStream_t)stream;
-  rc = wide(p.E, 4, {p.h, p.xo, p.gx, p.gy, p.dx, p.dh, p.pg, p.pb, p.ng, p.nb, p.gate}) ? by_width<float, 4, Bwd>(p, st) : by_width<float, 1, Bwd>(p, st);
+  rc = wide(p.E, 4, {p.h, p.xo, p.gx, p.gy, p.dx, p.dh, p.pg, p.pb, p.ng, p.nb, p.gate}) ? by_width<float, 4, false, Bwd>(p, st) : by_width<float, 4, true, Bwd>(p, st);
   if (rc != SMX_OK || !p.want) return rc;
   const Outs o = {{d->dpre_gamma, d->dpre_beta, d->dpost_gamma, d->dpost_beta, d->dgate}};
   bool shared = false;                               // one parameter in two places: its sums one launch after the other

@@ -158,7 +158,7 @@ def test_left_over_rows_and_empty(ops):
         assert a.shape == b.shape == (0, 96)
 
 
-@pytest.mark.parametrize("E", [33, 66, 260, 1025])
+@pytest.mark.parametrize("E", [5, 7, 33, 66, 100, 260, 1025, 2470, 4099, 8191, 16383])
 def test_rows_that_start_anywhere(ops, T, E):
     """contiguous views behind an odd number of rows: no 16-byte alignment to rely on"""
     from synergize_motion_appearance_amd.tape import Tape
