@@ -71,28 +71,23 @@ __device__ __forceinline__ f32x16 mfma_levels(const u32x4 (&a)[NL], const u32x4 
   }
   return mfma<NL>(a[0], b[0], c);
 }
-// eight fp32, times w, -> the levels' fragments (bf16: one, rounded to nearest; halves: two).  The second half is one v_fma_mix_f32 a value (v w - h1)
-// and the rounding in pairs; a caller without a factor passes one(), a 1 that the compiler does not see as such: it would fall back to a conversion
-// and a subtraction.
+// eight fp32, times w, -> two halves' fragments.  The second half is one v_fma_mix_f32 a value (v w - h1) and the rounding in pairs; a caller without
+// a factor passes one(), a 1 that the compiler does not see as such: it would fall back to a conversion and a subtraction.
 __device__ __forceinline__ float one() {
   float x = 1.f;
   asm volatile("" : "+s"(x));
   return x;
 }
-template <int NL>
-__device__ __forceinline__ void to_levels(const float* v, float w, u32x4 (&f)[NL]) {
+__device__ __forceinline__ void to_levels(const float* v, float w, u32x4 (&f)[2]) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float a = v[2 * i], b = v[2 * i + 1];
-    if constexpr (NL == 1) h[i] = cvt2_bf16(a, b);
-    else {
-      h[i] = cvt2_f16(a * w, b * w);
-      l[i] = cvt2_f16(fmaf(a, w, -f16lo(h[i])), fmaf(b, w, -f16hi(h[i])));
-    }
+    h[i] = cvt2_f16(a * w, b * w);
+    l[i] = cvt2_f16(fmaf(a, w, -f16lo(h[i])), fmaf(b, w, -f16hi(h[i])));
   }
   f[0] = u32x4{h[0], h[1], h[2], h[3]};
-  if constexpr (NL == 2) f[1] = u32x4{l[0], l[1], l[2], l[3]};
+  f[1] = u32x4{l[0], l[1], l[2], l[3]};
 }
 // the same for weights, whose first half is taken of v itself
 __device__ __forceinline__ void to_halves(const float* v, float w1, u32x4 (&f)[2]) {
@@ -101,6 +96,20 @@ __device__ __forceinline__ void to_halves(const float* v, float w1, u32x4 (&f)[2
   for (int i = 0; i < 4; ++i) {
     h[i] = cvt2_f16(v[2 * i], v[2 * i + 1]);
     l[i] = cvt2_f16(fmaf(v[2 * i], w1, -f16lo(h[i])), fmaf(v[2 * i + 1], w1, -f16hi(h[i])));
+  }
+  f[0] = u32x4{h[0], h[1], h[2], h[3]};
+  f[1] = u32x4{l[0], l[1], l[2], l[3]};
+}
+
+// weights that meet values in bf16: two bf16 parts, together within 2^-16 of the weight (one, within 2^-8, would cost an output as much again as the rounding of
+// the output itself; the row's sum takes the weights as they are)
+__device__ __forceinline__ void to_bf16_parts(const float* v, u32x4 (&f)[2]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i], b = v[2 * i + 1];
+    h[i] = cvt2_bf16(a, b);
+    l[i] = cvt2_bf16(a - __uint_as_float(h[i] << 16), b - __uint_as_float(h[i] & 0xffff0000u));
   }
   f[0] = u32x4{h[0], h[1], h[2], h[3]};
   f[1] = u32x4{l[0], l[1], l[2], l[3]};
@@ -177,7 +186,7 @@ __device__ __forceinline__ float own_rows(u32x4 (&f)[DHP / 16][2], const float* 
   const float sc = pow2_of(other_max(m), inv);
 #pragma unroll
   for (int kk = 0; kk < DHP / 16; ++kk) {
-    to_levels<2>(v[kk], sc, f[kk]);
+    to_levels(v[kk], sc, f[kk]);
   }
   return inv;
 }

@@ -1,7 +1,7 @@
 // Attention with a learned relative position bias by buckets, forward (include/smx.h: smx_attention_relpos):
 //   s_ij = scale q_i . k_j + table[map[clamp(j - pos_i - map_lo)]][h],  P = softmax over the keys that are left,  o_i = sum_j P_ij v_j
 // One pass over the keys with the running maximum and sum of the softmax, scores in log2 units.  Two kernels and what they need:
-//   relpos_tile_kernel   queries in tiles of 32 a wave on the matrix cores (bf16 storage: bf16 products; fp32 storage: f16x3, relpos.h)
+//   relpos_tile_kernel   queries in tiles of 32 a wave on the matrix cores (bf16 storage: bf16 products, weights in two parts; fp32 storage: f16x3, relpos.h)
 //   relpos_token_kernel  a few queries per sample (decoding): bound by reading the cache, plain fp32 products on the vector units
 //   relpos_join_kernel   joins the parts where the keys were split over blocks
 //   relpos_split_kernel  the staged fp32 operands as two halves each
@@ -143,8 +143,9 @@ struct Src {
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
 // Bound by the vector units' work on the scores (bias, maximum, 2^x, sum, two halves: some 10 operations each) next to the matrix products, of which only part runs
 // at the same time on 2 or 3 waves a SIMD.  38 x 8 heads of 1024 x 1024 of 32, fp32: 206 us with the split, 198 TFLOP/s of the formula's, 0.47 of
-// what three half-precision products at a large matrix product's rate would take; 2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 358 us, 767 TFLOP/s,
-// 0.61 of that rate.  Three waves a SIMD (bf16 up to 64 columns) against two: 44.7 / 44.9 us for 32 columns, 61.8 / 63.0 for 64.
+// what three half-precision products at a large matrix product's rate would take; 2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 459 us, 599 TFLOP/s
+// (358 with the weights in one bf16 part, the outputs' error then 1.3 times that of their own rounding).  Three waves a SIMD (bf16 up to 64 columns) against two, 8 x 16 heads of 1024 x 1024: 54.0 / 52.4 us for 32 columns, 75.7 / 76.4
+// for 64, where the long sequence takes 467 / 493.
 // 64 queries a wave instead of 32: 221 us for 205 of that build.
 template <int DHP, int NL>
 __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile_kernel(RP p, Src a) {
@@ -344,15 +345,16 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
         for (int r = 0; r < 16; ++r) { e[r] = __builtin_amdgcn_exp2f(s[u][r]); lt += e[r]; }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          u32x4 pf[NL];
+          u32x4 pf[2];
           if constexpr (NL == 2) to_halves(e + 8 * g, w1, pf);
-          else to_levels<1>(e + 8 * g, 1.f, pf);
+          else to_bf16_parts(e + 8 * g, pf);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
             u32x4 vf[NL];
 #pragma unroll
             for (int x = 0; x < NL; ++x) vf[x] = col_frag<DHP>(st + (NL + x) * PLANE, u * 32 + g * 16, d);
-            o[d] = mfma_levels<NL>(vf, pf, o[d]);
+            if constexpr (NL == 2) o[d] = mfma_levels<2>(vf, pf, o[d]);
+            else { o[d] = mfma<1>(vf[0], pf[1], o[d]); o[d] = mfma<1>(vf[0], pf[0], o[d]); }
           }
         }
       }

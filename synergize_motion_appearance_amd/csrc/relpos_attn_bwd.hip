@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2];
-        to_levels<2>(ds + 8 * g, fk, pf);
+        to_levels(ds + 8 * g, fk, pf);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const u32x4 kf[2] = {col_frag<DHP>(sm, u * 32 + g * 16, d), col_frag<DHP>(sm + ST::PLANE, u * 32 + g * 16, d)};
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
         u32x4 pf[2], sf[2];
         const float e[8] = {s[8 * g], s[8 * g + 1], s[8 * g + 2], s[8 * g + 3], s[8 * g + 4], s[8 * g + 5], s[8 * g + 6], s[8 * g + 7]};
         to_halves(e, w1, pf);
-        to_levels<2>(ds + 8 * g, fq, sf);
+        to_levels(ds + 8 * g, fq, sf);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const u32x4 gt[2] = {col_frag<DHP>(sm + 2 * ST::PLANE, u * 32 + g * 16, d), col_frag<DHP>(sm + 3 * ST::PLANE, u * 32 + g * 16, d)};

@@ -1,0 +1,54 @@
+"""`ops.attention_relpos` and `train_ops.attention_relpos` on a real MI355X: values where arithmetic of fewer bits, very different sizes and places that
+do not count could show, against the formula in fp64 (tests/layer_ref.py)."""
+import pytest
+import torch
+
+from tests import layer_ref as R
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    assert torch.cuda.is_available(), "needs an MI355X"
+    from synergize_motion_appearance_amd import ops as _ops
+    return _ops
+
+
+@pytest.fixture(scope="module")
+def T():
+    from synergize_motion_appearance_amd import train_ops
+    return train_ops
+
+
+def mk(seed, B, H, Hkv, Lq, S, dh, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    return (*(torch.randn(B, n, h * dh, generator=g).to(dtype).cuda() for n, h in ((Lq, H), (S, Hkv), (S, Hkv))), g)
+
+
+def near(got, val, bound, what=""):
+    got = got.detach().double().cpu()
+    assert got.shape == val.shape and torch.isfinite(got).all(), what
+    off = (got - val).abs() - bound
+    assert float(off.max()) <= 0, f"{what}: over its bound by {float(off.max()):.3e}, {int((off > 0).sum())} of {off.numel()}"
+
+
+# B, H, Hkv, L, S, dh, causal, masked, ragged
+PROMPTS = [(1, 2, 1, 2, 40, 32, False, False, False), (2, 4, 2, 70, 70, 64, True, True, False), (3, 2, 2, 33, 300, 80, False, True, True),
+           (1, 2, 1, 130, 2000, 128, False, False, False), (2, 2, 2, 40, 1300, 4, True, False, False), (1, 8, 2, 600, 600, 32, True, False, False)]
+
+
+@pytest.mark.parametrize("c", PROMPTS, ids=str)
+def test_bf16_prompts_are_rounded_once(ops, c):
+    """bf16 storage of several queries: what the weights' two bf16 parts leave (2^-8 of 2^-8 of a weight) and the output's own rounding, next to the bound of fp32
+    arithmetic.  One part alone would be off by up to 2^-8 of a weight."""
+    B, H, Hkv, Lq, S, dh, causal, masked, ragged = c
+    q, k, v, g = mk(31, B, H, Hkv, Lq, S, dh, BF)
+    rp = ops.relpos(32, 128, two_sided=not causal)
+    table = torch.randn(32, H, generator=g).cuda()
+    kw = dict(nkv=Hkv, causal=causal, mask=(torch.rand(B, S, generator=g) < 0.3).cuda() if masked else None,
+              kv_len=torch.tensor([S, S // 2, 1][:B], dtype=torch.int32).cuda() if ragged else None)
+    val, bound = R.attention(q, k, v, table, rp, H, **kw)["o"]
+    spread = R.attention(q, k, v.abs(), table, rp, H, **kw)["o"][0]
+    near(ops.attention_relpos(q, k, v, table, rp, H, **kw), val, bound + 2.0 ** -16 * spread + R.U[BF] * val.abs())
