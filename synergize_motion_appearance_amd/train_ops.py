@@ -576,7 +576,7 @@ def attention_relpos(tp, q, k, v, table, rp, nhead, *, nkv=None, causal=False, m
     if q.dtype != F32:
         raise L.SmxError(f"attention_relpos: the training step is fp32, got {q.dtype}")
     o, lse, d = ops._attention_relpos(q, k, v, tv, rp, nhead, nkv, causal, mask, kv_len, q_start, scale, True)
-    held = (q, k, v, tv, mask, kv_len, lse)              # what the descriptor points at
+    held = (q, k, v, tv, mask, kv_len, lse, rp)          # what the descriptor points at (rp: its map)
 
     def bwd():
         g = tp.take(o)

@@ -52,3 +52,32 @@ def test_bf16_prompts_are_rounded_once(ops, c):
     val, bound = R.attention(q, k, v, table, rp, H, **kw)["o"]
     spread = R.attention(q, k, v.abs(), table, rp, H, **kw)["o"][0]
     near(ops.attention_relpos(q, k, v, table, rp, H, **kw), val, bound + 2.0 ** -16 * spread + R.U[BF] * val.abs())
+
+
+def step(T, q, k, v, table, rp, H, go, **kw):
+    from synergize_motion_appearance_amd.tape import Tape
+    G = {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    o = T.attention_relpos(tp, q, k, v, "t", rp, H, **kw)
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    return o, tp.grad(q), tp.grad(k), tp.grad(v), G["t"]
+
+
+def test_a_map_that_only_the_tape_holds(ops, T):
+    """a RelPos made for one call, its map's size of memory written over between the forward and the backward"""
+    from synergize_motion_appearance_amd.tape import Tape
+    B, H, S, dh = 2, 2, 100, 32
+    q, k, v, g = mk(35, B, H, H, S, S, dh)
+    table, go = torch.randn(24, H, generator=g).cuda(), torch.randn(B, S, H * dh, generator=g).cuda()
+    want = step(T, q, k, v, table, ops.relpos(24, 301), H, go)
+    G = {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    o = T.attention_relpos(tp, q, k, v, "t", ops.RelPos(24, 301), H)
+    n = len(ops.relpos(24, 301).map)
+    over = [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(8)]
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    for x, y in zip((o, tp.grad(q), tp.grad(k), tp.grad(v), G["t"]), want):
+        assert torch.equal(x, y)
+    assert len(over) == 8
