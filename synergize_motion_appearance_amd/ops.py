@@ -1253,6 +1253,9 @@ def attention(q, k, v, nhead, dh, S, *, k_shared=False, mask=None, k_off=0, scal
     return o
 
 
+_MAPS = {}                   # (buckets, distance, two-sided, device) -> the map there, of at most 8 KB, kept for good: launches on any stream and captured graphs read it
+
+
 class RelPos:
     """Buckets of relative positions delta = key position - query position, for `attention_relpos`: the first half of a side's buckets holds
     one distance each, the second half ranges that grow by a constant factor up to `max_distance`; everything beyond shares the last.
@@ -1289,10 +1292,16 @@ class RelPos:
         """the map as an int32 tensor on this device (made at the first call there, which must not be inside a graph capture)"""
         t = self._on.get(device)
         if t is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise L.SmxError("RelPos: its map is copied to a device at the first use there: call it once before the capture")
-            t = self._on[device] = torch.tensor(self.map, dtype=torch.int32, device=device)
-            torch.cuda.current_stream(device).synchronize()   # whole before any stream reads it
+            key = (self.num_buckets, self.max_distance, self.two_sided, device)
+            t = _MAPS.get(key)
+            if t is None:
+                with torch.cuda.device(device):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise L.SmxError("RelPos: its map is copied to a device at the first use there: call it once before the capture")
+                    t = torch.tensor(self.map, dtype=torch.int32, device=device)
+                    torch.cuda.current_stream(device).synchronize()    # whole before any stream reads it
+                t = _MAPS.setdefault(key, t)                   # (two threads at once: both take the one that stays)
+            self._on[device] = t
         return t
 
 

@@ -47,3 +47,39 @@ def test_the_tape_keeps_the_map(calls, monkeypatch):
     monkeypatch.setattr(tp, "acc", lambda *a, **kw: None)
     tp.backward()
     assert calls[-1] == ("smx_attention_relpos_bwd_f32", at)
+
+
+def test_threads_at_the_first_use_share_one_map(calls, monkeypatch):
+    """two threads that both find no map yet: what either is handed is what stays"""
+    import threading
+    meet, made, tensor = threading.Barrier(2, timeout=20), [], torch.tensor
+
+    def both_in(*a, **kw):
+        t = tensor(*a, **kw)
+        made.append(t.data_ptr())
+        meet.wait()
+        return t
+    rp, got = ops.RelPos(8, 22), []
+    monkeypatch.setattr(torch, "tensor", both_in)
+    ts = [threading.Thread(target=lambda: got.append(rp.on(torch.device("cpu")))) for _ in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert len(made) == 2 and len(got) == 2
+    assert got[0] is got[1] and rp.on(torch.device("cpu")) is got[0]
+
+
+def test_a_map_outlives_its_relpos(calls):
+    """a launch on another stream than the one its memory belongs to, or a captured graph, may read a map after its RelPos is gone: maps are never freed,
+    and equal ones are one"""
+    q = torch.randn(1, 6, 8)
+    rp = ops.RelPos(8, 23)
+    ops.attention_relpos(q, q, q, torch.zeros(8, 2), rp, 2)
+    at, m = calls[-1][1], weakref.ref(rp.on(q.device))
+    assert m().data_ptr() == at
+    del rp
+    gc.collect()
+    assert m() is not None and m().data_ptr() == at
+    ops.attention_relpos(q, q, q, torch.zeros(8, 2), ops.RelPos(8, 23), 2)
+    assert calls[-1][1] == at
