@@ -1305,10 +1305,12 @@ class RelPos:
         return t
 
 
-@functools.lru_cache(maxsize=None)
+_relpos = functools.lru_cache(maxsize=None)(RelPos)
+
+
 def relpos(num_buckets=32, max_distance=128, two_sided=True):
-    """the RelPos of these numbers, one object for all callers."""
-    return RelPos(num_buckets, max_distance, two_sided)
+    """the RelPos of these numbers, one object for all callers, however they spell them."""
+    return _relpos(num_buckets, max_distance, bool(two_sided))
 
 
 def _rows3(t, what, B, width, dtype, device):

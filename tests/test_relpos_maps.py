@@ -83,3 +83,11 @@ def test_a_map_outlives_its_relpos(calls):
     assert m() is not None and m().data_ptr() == at
     ops.attention_relpos(q, q, q, torch.zeros(8, 2), ops.RelPos(8, 23), 2)
     assert calls[-1][1] == at
+
+
+def test_one_relpos_for_every_spelling():
+    one = ops.relpos(32, 128, True)
+    assert ops.relpos() is one and ops.relpos(32) is one and ops.relpos(32, 128) is one and ops.relpos(max_distance=128) is one
+    assert ops.relpos(32, 128, two_sided=True) is one and ops.relpos(num_buckets=32, max_distance=128, two_sided=1) is one
+    causal = ops.relpos(32, 128, False)
+    assert causal is not one and ops.relpos(two_sided=False) is causal and ops.relpos(32, two_sided=0, max_distance=128) is causal
