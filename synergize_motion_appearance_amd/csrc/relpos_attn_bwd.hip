@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     const float sc = sk * pow2_bits(eq), sp = sv * pow2_bits(eg);
     if (t + 1 < last) load_tile(t + 1);
     if (k0 >= n || (p.causal && pos0 + i0 + TQ - 1 < k0)) continue;
-    const int lg = 14 + gu.enter(eg, dv);                     // P carries 2^lg
+    const int lp = 14 + gu.enter(eg, dv), lg = max(lp, 0);    // P carries 2^lg, in dv 2^lp: 2^-lp of a far smaller tile, times f, would leave fp32
     const float ig = exp2i(-lg), wq = exp2i(qu.enter(eq, dk)) * ig;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -324,9 +324,9 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, c - lv[r]);
       } else {
-        const float* lp = lut + TABLE_PAD + e0 + (lane & 31) - 4 * hh;
+        const float* bias = lut + TABLE_PAD + e0 + (lane & 31) - 4 * hh;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, lp[-crow(r)] - (lv[r] - lg));
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], sc, bias[-crow(r)] - (lv[r] - lg));
       }
       if (is_steep) at_most(s, (float)lg);
 #pragma unroll
@@ -342,6 +342,11 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
       for (int r = 0; r < 16; ++r) { ds[r] = s[r] * fmaf(dp[r], sp, -dd[r]); top = fmaxf(top, fabsf(ds[r])); }
       follow(top * ig, f, dk);
       const float fq = f * wq;
+      if (lp < 0) {
+        const float w = exp2i(lp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= w;
+      }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 pf[2], sf[2];

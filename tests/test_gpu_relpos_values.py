@@ -81,3 +81,21 @@ def test_a_map_that_only_the_tape_holds(ops, T):
     for x, y in zip((o, tp.grad(q), tp.grad(k), tp.grad(v), G["t"]), want):
         assert torch.equal(x, y)
     assert len(over) == 8
+
+
+@pytest.mark.parametrize("dh", [32, 64, 128])
+def test_dk_of_far_smaller_gradients(ops, T, dh):
+    """output gradients of 64 rows 2^-110 of those before them, and a key that so far has met exact zeros only: its dk is of the small ones' size.  A dS of some 2^-113
+    is carried times 2^100 in two halves, off by at most half of the lowest bit 2^-24: 2^-125."""
+    q, k, v, g = mk(32, 1, 1, 1, 128, 128, dh)
+    go = torch.randn(1, 128, dh, generator=g)
+    go[:, 63] = 0
+    go[:, 64:] *= 2.0 ** -110
+    go = go.cuda()
+    rp = ops.relpos(32, 128, two_sided=False)
+    table = torch.randn(32, 1, generator=g).cuda()
+    out = step(T, q, k, v, table, rp, 1, go, causal=True)
+    val, bound = R.attention(q, k, v, table, rp, 1, causal=True, g=go)["dk"]
+    for t in out:
+        assert torch.isfinite(t).all()
+    near(out[2], val, bound + dh ** -0.5 * 2.0 ** -125 * q.double().cpu().abs().sum(1, keepdim=True), "dk")
