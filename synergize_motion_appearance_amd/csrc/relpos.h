@@ -23,8 +23,8 @@ constexpr int TABLE_PAD = 96;         // entries a 64-key x 32-query tile can re
 // x = (h1 + h2) 2^-k with two IEEE halves: 22 significand bits; a product is h1 g1 + h1 g2 + h2 g1, the dropped h2 g2 is 2^-22 of it.  k brings the largest |x|
 // that shares it to [2^14, 2^15): values down to 2^-16 of that keep all 22 bits, smaller ones are off by at most 2^-40 of it.  Rows that a wave keeps in
 // registers are split there, each with a k of its own (own_rows).  Rows that are staged -- read by every block of the other side -- are split once, by a
-// pass before: planes [B][heads][rows rounded up to 64][dh rounded up to 32] of h1 and of h2 with one k per 64 rows; rows that nobody may see and the
-// columns from dh on are zeros.  Where a product sums over staged rows, the k of the tile joins the factor of the other operand (Unit).
+// pass before: planes [B][heads][rows rounded up to 64][dh rounded up to 32] of h1 and of h2 with one k per 64 rows; keys that nobody may see,
+// queries that see none and the columns from dh on are zeros.  Where a product sums over staged rows, the k of the tile joins the factor of the other operand (Unit).
 struct Split {
   const float* src; long long bs; int ld, heads, rows, kv, flip;  // kv: rows of keys (masks and lengths apply); flip: odd rows negated
   _Float16* hi; _Float16* lo;                                   // planes
@@ -43,6 +43,8 @@ struct RP {
   float scale;
   __device__ __forceinline__ int keys(int b) const { return kv_len ? max(0, min(kv_len[b], S)) : S; }
   __device__ __forceinline__ int pos0(int n) const { return has_start ? q_start : n - L; }
+  // backward: a query with no key left, by the forward's lse.  What it and its gradient hold must not meet the zeros of its weights
+  __device__ __forceinline__ bool empty(int b, int h, int i) const { return lse[((long long)b * H + h) * L + i] == INFINITY; }
   __device__ __forceinline__ int entry(int delta) const { return max(0, min(delta - map_lo, map_n - 1)); }
 };
 

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void relpos_split_kernel(RP p, Splits a) {
   const int n = s.kv ? min(p.keys(b), s.rows) : s.rows;
   constexpr int NI = DHP / 16;                                   // four threads a row, NI float4 each
   const int r = threadIdx.x >> 2, q = threadIdx.x & 3, row = c * 64 + r;
-  const bool in = row < n && !(s.kv && p.mask && p.mask[(long long)b * p.S + row]);
+  const bool in = row < n && !(s.kv ? p.mask && p.mask[(long long)b * p.S + row] : p.empty(b, h, row));
   const long long at = b * s.bs + (long long)row * s.ld + h * p.dh, tile = ((long long)b * s.heads + h) * nt + c;
   float4 x[NI];
   float m = 0.f, D = 0.f;

@@ -114,11 +114,12 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
   dacc += wave * nent;
   const float first_bias = p.table[(long long)p.map[0] * p.H + h] * LOG2E, last_bias = p.table[(long long)p.map[p.map_n - 1] * p.H + h] * LOG2E;
   const float lse = live ? p.lse[((long long)b * p.H + h) * p.L + qi] : INFINITY;
+  const bool sees = lse != INFINITY;                             // the query has a key (what it holds without one does not count)
   const bool is_steep = __ballot(steep(lse)) != 0;
   const float D = live ? a.g.dd[((long long)b * p.H + h) * ((p.L + 63) & ~63) + qi] : 0.f;
   u32x4 qf[KS][2], gf[KS][2];
-  const float sq = p.scale * LOG2E * own_rows<DHP>(qf, (const float*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh, live, p.dh);
-  const float sg = own_rows<DHP>(gf, p.d_o + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh, live, p.dh);
+  const float sq = p.scale * LOG2E * own_rows<DHP>(qf, (const float*)p.q + b * p.q_bs + (long long)qi * p.ldq + h * p.dh, sees, p.dh);
+  const float sg = own_rows<DHP>(gf, p.d_o + ((long long)b * p.L + qi) * p.H * p.dh + h * p.dh, sees, p.dh);
   f32x16 dq[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dq[t] = zero16();

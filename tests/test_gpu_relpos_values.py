@@ -99,3 +99,28 @@ def test_dk_of_far_smaller_gradients(ops, T, dh):
     for t in out:
         assert torch.isfinite(t).all()
     near(out[2], val, bound + dh ** -0.5 * 2.0 ** -125 * q.double().cpu().abs().sum(1, keepdim=True), "dk")
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3e38])
+@pytest.mark.parametrize("which", ["q", "do"])
+def test_queries_without_a_key_do_not_count_in_the_backward(ops, T, which, bad):
+    """padding in front of a short sample, a sample whose mask leaves nothing: what those queries and their output gradients hold changes no gradient by a bit,
+    and their own is zero"""
+    B, H, S, dh = 3, 2, 150, 32
+    q, k, v, g = mk(33, B, H, H, S, S, dh)
+    go = torch.randn(B, S, H * dh, generator=g).cuda()
+    rp = ops.relpos(32, 128, two_sided=False)
+    table = torch.randn(32, H, generator=g).cuda()
+    mask = torch.zeros(B, S, dtype=torch.uint8)
+    mask[1] = 1
+    kw = dict(causal=True, mask=mask.cuda(), kv_len=torch.tensor([S, S, 77], dtype=torch.int32).cuda())
+    empty = torch.zeros(B, S, 1, dtype=torch.bool)
+    empty[1], empty[2, :S - 77] = True, True
+    empty = empty.cuda()
+
+    def with_(x):
+        return step(T, q.masked_fill(empty, x if which == "q" else 0.0), k, v, table, rp, H, go.masked_fill(empty, x if which == "do" else 0.0), **kw)
+    a, b = with_(0.0), with_(bad)
+    for x, y, n in zip(a, b, ("o", "dq", "dk", "dv", "dtable")):
+        assert torch.isfinite(y).all() and torch.equal(x, y), n
+    assert float(b[1].masked_select(empty.expand_as(b[1])).abs().max()) == 0.0
