@@ -692,7 +692,7 @@ int smx_chan_affine_f32(const float* x, int ldx, const float* scale, const float
  *   n_b = kv_len[b] (clamped to 0..S) keys, n_b = S without kv_len;  delta = j - pos;
  *   s_ij = scale * q_i . k_j + table[map[clamp(delta - map_lo, 0, map_n - 1)]][head];  P = softmax over the keys that are left (j < n_b,
  *   not masked, delta <= 0 if causal);  o_i = sum_j P_ij v_j.  A query with no key left: o = 0 and no gradient.
- * What the places of masked keys and of keys behind n_b hold is never used (NaN and infinities too); their dk / dv are written as 0.  Neither is, in the
+ * What the places of masked keys, of keys behind n_b and, if causal, of keys behind the last query hold is never used (NaN and infinities too); their dk / dv are written as 0.  Neither is, in the
  * backward, what a query with no key left and its output gradient hold.
  * q [B][L] rows of H*dh, k / v [B][S] rows of Hkv*dh (head h reads kv head h / (H / Hkv)), row strides ld*, sample strides *_bs in
  * elements (k / v sample stride 0: one context for all samples), ld* <= 2^24.  dh % 4 == 0, dh <= 128; strides % 4 == 0, pointers aligned to four

@@ -41,7 +41,11 @@ struct RP {
   int ldq, ldk, ldv, ldo;
   int B, H, Hkv, G, L, S, dh, map_lo, map_n, nb, causal, has_start, q_start;
   float scale;
-  __device__ __forceinline__ int keys(int b) const { return kv_len ? max(0, min(kv_len[b], S)) : S; }
+  // keys that a query of the sample can see: with a causal rule none behind the last query's position
+  __device__ __forceinline__ int keys(int b) const {
+    const int n = kv_len ? max(0, min(kv_len[b], S)) : S;
+    return causal && has_start ? max(0, min(n, q_start + L)) : n;
+  }
   __device__ __forceinline__ int pos0(int n) const { return has_start ? q_start : n - L; }
   // backward: a query with no key left, by the forward's lse.  What it and its gradient hold must not meet the zeros of its weights
   __device__ __forceinline__ bool empty(int b, int h, int i) const { return lse[((long long)b * H + h) * L + i] == INFINITY; }

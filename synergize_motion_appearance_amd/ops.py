@@ -1384,6 +1384,7 @@ def attention_relpos(q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=
     kv_len int32 [B]: sample b has the first kv_len[b] of the S keys (clamped to 0..S).  Positions: key j is at j, query i at q_start + i,
     by default the queries are the last L of the sample's keys -- all of them in self attention, the newest one with L = 1.
     causal: keys behind the query's position are left out; mask uint8 or bool [B, S], nonzero: key left out.  What left-out keys of `mask` and
-    `kv_len` hold is not used, whatever it is (keys that only the causal rule hides from some queries must hold finite numbers).
+    `kv_len` and keys behind the last query of a causal call hold is not used, whatever it is (keys that the causal rule hides from some queries
+    only must hold finite numbers).
     A query with no key left answers zeros.  -> o [B, L, nhead * dh]."""
     return _attention_relpos(q, k, v, table, rp, nhead, nkv, causal, mask, kv_len, q_start, scale, False)[0]

@@ -571,7 +571,7 @@ def attention(tp, q, k, v, nhead, dh, S, *, mask=None, ctx=None):
 
 def attention_relpos(tp, q, k, v, table, rp, nhead, *, nkv=None, causal=False, mask=None, kv_len=None, q_start=None, scale=None):
     """ops.attention_relpos (fp32); table: parameter reference [rp.num_buckets, nhead].  The gradients of masked keys and of keys behind
-    kv_len are zeros, those of a query with no key left too; shared kv heads collect the sums over their heads."""
+    kv_len or, if causal, behind the last query are zeros, those of a query with no key left too, whatever these hold; shared kv heads collect the sums over their heads."""
     tv, tg, _ = _param(tp, table)
     if q.dtype != F32:
         raise L.SmxError(f"attention_relpos: the training step is fp32, got {q.dtype}")

@@ -124,3 +124,29 @@ def test_queries_without_a_key_do_not_count_in_the_backward(ops, T, which, bad):
     for x, y, n in zip(a, b, ("o", "dq", "dk", "dv", "dtable")):
         assert torch.isfinite(y).all() and torch.equal(x, y), n
     assert float(b[1].masked_select(empty.expand_as(b[1])).abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("Lq", [1, 4, 96])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3e38])
+def test_keys_behind_the_last_query_do_not_count(ops, T, dtype, Lq, bad):
+    """a cache that is longer than what has been written, with a causal rule and the first query's position: no result changes by a bit with what lies behind the
+    last query, and those keys' gradients are zeros"""
+    B, H, S, dh, start = 2, 2, 300, 64, 103
+    q, k, v, g = mk(34, B, H, H, Lq, S, dh, dtype)
+    rp = ops.relpos(32, 128, two_sided=False)
+    table = torch.randn(32, H, generator=g).cuda()
+    go = torch.randn(B, Lq, H * dh, generator=g).cuda()
+    kw = dict(causal=True, q_start=start)
+
+    def with_(x):
+        kk, vv = k.clone(), v.clone()
+        kk[:, start + Lq:], vv[:, start + Lq:] = x, x
+        return step(T, q, kk, vv, table, rp, H, go, **kw) if dtype == F32 else (ops.attention_relpos(q, kk, vv, table, rp, H, **kw),)
+    a, b = with_(0.0), with_(bad)
+    for x, y in zip(a, b):
+        assert torch.isfinite(y).all() and torch.equal(x, y)
+    if dtype == F32:
+        assert float(b[2][:, start + Lq:].abs().max()) == 0.0 and float(b[3][:, start + Lq:].abs().max()) == 0.0
+    ref = R.attention(q, k[:, :start + Lq], v[:, :start + Lq], table, rp, H, storage=dtype, **kw)["o"]
+    near(b[0], *ref)
