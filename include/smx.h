@@ -701,7 +701,8 @@ int smx_chan_affine_f32(const float* x, int ldx, const float* scale, const float
  * lse: [B][H][L] floats or NULL: log2 of the row's softmax sum (+inf for a row with no key), what the backward reads.
  * ws: smx_attention_relpos_ws_bytes(d) bytes, 16-byte aligned (backward: smx_attention_relpos_bwd_ws_bytes).
  * Backward (fp32): o and d_o dense [B][L][H*dh]; dq dense [B][L][H*dh], dk / dv dense [B][S][Hkv*dh] per sample, written; dtable
- * [num_buckets][H] ACCUMULATED into.  Fixed summation orders, no atomics.
+ * [num_buckets][H] ACCUMULATED into.  dq and dtable, or dk and dv, may be NULL: a pass whose results nobody wants is left out.
+ * Fixed summation orders, no atomics.
  * Accuracy: sums and statistics in fp32.  Single tokens: fp32 products.  Otherwise bf16 storage takes products of bf16 values, the weights as two bf16
  * parts (within 2^-16 of the weight; an infinite value leaves no number in the rows that see it); fp32 storage products of 22-bit values: of the 64 rows (or the one row) that share a power of two, values below 2^-16 of the largest are off
  * by up to 2^-40 of it, and an infinity leaves no number in what its 64 rows enter; a weight is off by up to 2^-31 of its row's largest (dv: 2^-39).

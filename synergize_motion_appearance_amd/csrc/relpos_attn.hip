@@ -106,7 +106,7 @@ int check(const smx_relpos_desc* d, RP& p, bool bwd) {
   if (d->q_bs % 4 || d->k_bs % 4 || d->v_bs % 4 || d->o_bs % 4) return SMX_EINVAL;
   const int el = 4 * (d->bf16 ? 2 : 4);
   if (!aligned(d->q, el) || !aligned(d->k, el) || !aligned(d->v, el) || !aligned(d->o, el)) return SMX_EINVAL;
-  if (bwd && (!d->d_o || !d->dq || !d->dk || !d->dv || !d->dtable || !d->lse || d->ldo != d->H * d->dh || d->o_bs != (int64_t)d->L * d->ldo)) return SMX_EINVAL;
+  if (bwd && (!d->d_o || !d->dq != !d->dtable || !d->dk != !d->dv || (!d->dq && !d->dk) || !d->lse || d->ldo != d->H * d->dh || d->o_bs != (int64_t)d->L * d->ldo)) return SMX_EINVAL;
   if (bwd && (!aligned(d->d_o, 16) || !aligned(d->dq, 16) || !aligned(d->dk, 16) || !aligned(d->dv, 16))) return SMX_EINVAL;
   p.q = d->q; p.k = d->k; p.v = d->v; p.o = d->o; p.table = d->table; p.map = d->map; p.mask = d->mask; p.kv_len = d->kv_len;
   p.lse = d->lse; p.d_o = d->d_o; p.dq = d->dq; p.dk = d->dk; p.dv = d->dv; p.dtable = d->dtable;

@@ -384,16 +384,16 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
     }
 }
 
-// What is left once the two passes are done, one launch: the first H blocks dtable, the others gradients from their parts, in order (dq, dk, dv).
+// What is left once the two passes are done, one launch: the first H blocks dtable, if it is wanted, the others gradients from their parts, in order (dq, dk, dv).
 // dtable[bucket][h] += the distances of that bucket: the query blocks' sums in four fixed runs, then a wave a bucket.  Bound by its dependent loads: 13 us after 4 x 8
 // heads of 1024 x 1024.
 struct Sum { const float* src; float* dst; long long size, step; int nparts, end; };      // end: running sum of blocks
-struct Rest { Sum s[3]; const float* part; int rows; };                                  // rows: query blocks (and their parts) of a head and sample
+struct Rest { Sum s[3]; const float* part; int rows, tables; };                          // rows: query blocks (and their parts) of a head and sample; tables: H or 0
 __global__ __launch_bounds__(1024) void relpos_bwd_rest_kernel(RP p, Rest a) {
   __shared__ float ent[4][MAP_MAX + 2 * DPAD];
   __shared__ unsigned short of[MAP_MAX + 2 * DPAD];
-  if ((int)blockIdx.x >= p.H) {
-    int id = blockIdx.x - p.H, t = 0;
+  if ((int)blockIdx.x >= a.tables) {
+    int id = blockIdx.x - a.tables, t = 0;
     while (id >= a.s[t].end) ++t;
     const Sum& s = a.s[t];
     const long long i = ((id - (t ? a.s[t - 1].end : 0)) * 1024LL + threadIdx.x) * 4;
@@ -460,8 +460,8 @@ int launch(const RP& p, const Bwd& a, const Plan& w, hipStream_t st) {
   const int planes = 4 * Stage<DHP>::PLANE, lq = 4 * (p.map_n + 2 * TABLE_PAD + 4 * (p.map_n + 2 * DPAD)), lk = 4 * (132 + p.map_n + 2 * TABLE_PAD);
   SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_q_kernel<DHP>, planes + 4 * (MAP_MAX + 2 * TABLE_PAD + 4 * (MAP_MAX + 2 * DPAD))));
   SMX_HIP(smx_max_dynamic_lds((const void*)relpos_bwd_kv_kernel<DHP>, planes + 4 * (132 + MAP_MAX + 2 * TABLE_PAD)));
-  SMX_LAUNCH(relpos_bwd_q_kernel<DHP>, dim3((unsigned)w.qblocks), dim3(256), planes + lq, st, p, a);
-  SMX_LAUNCH(relpos_bwd_kv_kernel<DHP>, dim3((unsigned)w.kblocks), dim3(256), planes + lk, st, p, a);
+  if (p.dq) SMX_LAUNCH(relpos_bwd_q_kernel<DHP>, dim3((unsigned)w.qblocks), dim3(256), planes + lq, st, p, a);
+  if (p.dk) SMX_LAUNCH(relpos_bwd_kv_kernel<DHP>, dim3((unsigned)w.kblocks), dim3(256), planes + lk, st, p, a);
   return smx_launch_status();
 }
 
@@ -494,8 +494,11 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
   a.dqp = (float*)(ws + w.part + w.dd);
   a.dkv = (float*)(ws + w.part + w.dd + w.dqp);
   a.qparts = w.qparts; a.kparts = w.kparts;
-  const Split all[4] = {a.q, a.g, a.k, a.v};
-  rc = split_launch(p, all, 4, st);
+  Split all[4] = {a.g};                                          // (D of its rows: both passes)
+  int n = 1;
+  if (p.dk) all[n++] = a.q;
+  if (p.dq) { all[n++] = a.k; all[n++] = a.v; }
+  rc = split_launch(p, all, n, st);
   if (rc != SMX_OK) return rc;
   switch (dhp(p.dh)) {
     case 32: rc = launch<32>(p, a, w, st); break;
@@ -504,11 +507,13 @@ extern "C" int smx_attention_relpos_bwd_f32(const smx_relpos_desc* d, void* stre
     default: rc = launch<128>(p, a, w, st);
   }
   if (rc != SMX_OK) return rc;
-  Rest u = {{{a.dqp, p.dq, w.qparts > 1 ? sq : 0, sq, w.qparts, 0}, {a.dkv, p.dk, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0},
-             {a.dkv + sk, p.dv, w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0}}, a.part, (p.L + 127) / 128 * w.qparts};
+  Rest u = {{{a.dqp, p.dq, p.dq && w.qparts > 1 ? sq : 0, sq, w.qparts, 0}, {a.dkv, p.dk, p.dk && w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0},
+             {a.dkv + sk, p.dv, p.dk && w.kparts > 1 ? sk : 0, 2 * sk, w.kparts, 0}}, a.part, (p.L + 127) / 128 * w.qparts, p.dtable ? p.H : 0};
   long long blocks = 0;
   for (Sum& x : u.s) { blocks += (x.size + 4095) / 4096; x.end = (int)blocks; }
-  if (blocks + p.H > 0x7fffffffLL) return SMX_EINVAL;
-  SMX_LAUNCH(relpos_bwd_rest_kernel, dim3((unsigned)(p.H + blocks)), dim3(1024), 0, st, p, u);
+  blocks += u.tables;
+  if (blocks > 0x7fffffffLL) return SMX_EINVAL;
+  if (!blocks) return rc;
+  SMX_LAUNCH(relpos_bwd_rest_kernel, dim3((unsigned)blocks), dim3(1024), 0, st, p, u);
   return smx_launch_status();
 }

@@ -588,9 +588,15 @@ def attention_relpos(tp, q, k, v, table, rp, nhead, *, nkv=None, causal=False, m
             return
         lib = tp.lib
         g = g if g.is_contiguous() and g.data_ptr() % 16 == 0 else _dense(lib, g)
-        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=F32) for t in held[:3])
-        dt = tg if tg is not None else _zeros(tv.shape, tv)
-        d.d_o, d.dq, d.dk, d.dv, d.dtable = g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dt.data_ptr()
+        of_q = tp.needs(q) or tg is not None                 # a pass over the queries (dq, the table), one over the keys (dk, dv)
+        of_kv = tp.needs(k) or tp.needs(v)
+        if not of_q and not of_kv:
+            return
+        dq = torch.empty(q.shape, device=q.device, dtype=F32) if of_q else None
+        dk, dv = (torch.empty(t.shape, device=t.device, dtype=F32) if of_kv else None for t in (k, v))
+        dt = tg if tg is not None or not of_q else _zeros(tv.shape, tv)
+        d.d_o = g.data_ptr()
+        d.dq, d.dk, d.dv, d.dtable = (None if t is None else t.data_ptr() for t in (dq, dk, dv, dt))
         n = lib.smx_attention_relpos_bwd_ws_bytes(d)
         ws = torch.empty((max(n, 16),), device=q.device, dtype=torch.uint8)
         d.ws, d.ws_bytes = ws.data_ptr(), n

@@ -150,3 +150,23 @@ def test_keys_behind_the_last_query_do_not_count(ops, T, dtype, Lq, bad):
         assert float(b[2][:, start + Lq:].abs().max()) == 0.0 and float(b[3][:, start + Lq:].abs().max()) == 0.0
     ref = R.attention(q, k[:, :start + Lq], v[:, :start + Lq], table, rp, H, storage=dtype, **kw)["o"]
     near(b[0], *ref)
+
+
+@pytest.mark.parametrize("stopped", ["q", "k", "kv", "t", "qt", "kvt", "qkv", "qkvt"])
+@pytest.mark.parametrize("S", [90, 1500])                        # (1500: both sides in parts)
+def test_gradients_that_are_wanted_do_not_depend_on_the_others(ops, T, stopped, S):
+    from synergize_motion_appearance_amd.tape import Tape
+    q, k, v, g = mk(36, 1, 2, 1, S, S, 32)
+    table, go = torch.randn(32, 2, generator=g).cuda(), torch.randn(1, S, 64, generator=g).cuda()
+    rp = ops.relpos()
+    want = step(T, q, k, v, table, rp, 2, go, nkv=1)
+    G = {} if "t" in stopped else {"t": torch.zeros_like(table)}
+    tp = Tape({"t": table}, G)
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if n in stopped:
+            tp.stop(t)
+    o = T.attention_relpos(tp, q, k, v, "t", rp, 2, nkv=1)
+    tp.acc(o, go, owned=False)
+    tp.backward()
+    for n, got, ref in zip("qkvt", (tp.grad(q), tp.grad(k), tp.grad(v), G.get("t")), want[1:]):
+        assert got is None if n in stopped else torch.equal(got, ref), n
