@@ -705,7 +705,10 @@ int smx_chan_affine_f32(const float* x, int ldx, const float* scale, const float
  * Fixed summation orders, no atomics.
  * Accuracy: sums and statistics in fp32.  Single tokens: fp32 products.  Otherwise bf16 storage takes products of bf16 values, the weights as two bf16
  * parts (within 2^-16 of the weight; an infinite value leaves no number in the rows that see it); fp32 storage products of 22-bit values: of the 64 rows (or the one row) that share a power of two, values below 2^-16 of the largest are off
- * by up to 2^-40 of it, and an infinity leaves no number in what its 64 rows enter; a weight is off by up to 2^-31 of its row's largest (dv: 2^-39).
+ * by up to 2^-40 of it, and an infinity leaves no number in what its 64 rows enter; a weight is off by up to 2^-31 of its row's largest (dv: 2^-39), a
+ * dS by up to 2^-34 of its query's (dk: its key's) largest or by 2^-125.  That holds while the 64-row tiles that a sum runs over are of one size: in a tile of
+ * smaller values than one before it these are up to 2^8 times that, and what a tile 2^60 and more below the largest before it adds is lost from 2^-91
+ * (dv: 2^-99, dq and dk: 2^-94) of the largest's on.
  * The backward computes the weights again from the scores: a score of size |s| gives one a relative error of some 2^-23 |s|.
  * ===================================================================================== */
 typedef struct smx_relpos_desc {

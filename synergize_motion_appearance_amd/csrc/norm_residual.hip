@@ -380,7 +380,8 @@ __global__ __launch_bounds__(1024) void norm_residual_sum_kernel(const float* __
 
 // Lanes a row and chunks a lane, by the row's 16-byte chunks: up to a wave's 64 lanes one chunk each, then up to 4
 // a lane (256 chunks over 256 lanes with their barriers: 52 us instead of 44 at 16384 x 1024 fp32), then rows over a block -- of 256 threads for up to 1024
-// chunks, 512 beyond, so that the backward's five sums of a thread's columns stay in registers.
+// chunks, 512 beyond, so that the backward's five sums of a thread's columns stay in registers up to 8192 columns.  Beyond, five sums of 32 columns next to the row
+// do not fit (some 320 registers go through scratch): 1024 x 16384 404 us with the forward's 61, 2048 x 8192 202 with 67.
 template <typename TS, int V, bool U, template <typename, int, int, int, bool> class K>
 int by_width(const NRP& p, hipStream_t st) {
   const int n = smx_cdiv(p.E, V);
@@ -413,7 +414,8 @@ template <typename TS, int V, int LPR, int N, bool U> struct Bwd {
 
 // tokens a backward block walks: about 512 blocks (their sums are written and read once more), 256 of rows that take a block of 512 threads -- one a CU at a time
 // --, but not fewer tokens than it has rows at a time.  Forward and backward with 256 / 512 / 1024 blocks: 65536 x 256 195 / 151 / 144 us, 8192 x 2048
-// 177 / 148 / 158, 4096 x 4096 178 / 160 / 181, 2048 x 8192 194 / 218 / 234, 1024 x 16384 378 / 421 / 499.
+// 177 / 148 / 158, 4096 x 4096 178 / 160 / 181, 2048 x 8192 194 / 218 / 234, 1024 x 16384 378 / 421 / 499.  A block ends with its gate row: with a row for every token
+// a block has one token, and the blocks' sums are more than the tensors (5 T E floats): 65536 x 256 1709 us instead of 153.
 int rows_of(long long T, long long per, int E) {
   const int want = E > 4096 ? 256 : 512;
   long long r = (T + want - 1) / want;

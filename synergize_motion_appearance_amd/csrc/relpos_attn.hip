@@ -124,7 +124,7 @@ using namespace relpos;
 
 // ---- queries in tiles ----------------------------------------------------------------------------------------------------------
 // two stages of keys in turn, one barrier a step; one where two would leave a CU with one block (fp32 storage, 65 to 96 columns: 106 KB).  8 x 16 heads of 1024 x 1024,
-// one / two: fp32 32 columns 98 / 98 us, 64 148 / 148, 96 211 / 243, 128 (in steps of 32 keys) 279 / 279; bf16 64 columns 62.6 / 61.8
+// one / two: fp32 32 columns 98 / 98 us, 64 148 / 148, 96 211 / 243, 128 (in steps of 32 keys) 279 / 279; bf16 64 columns (weights in one part) 62.6 / 61.8
 template <int DHP, int NL> constexpr int BUFFERS = NL == 2 && DHP == 96 ? 1 : 2;
 
 // where the operands come from: bf16 storage reads q / k / v themselves, fp32 storage q and the planes of k and v; parts: m, l [row][part], o
@@ -141,11 +141,13 @@ struct Src {
 // Weights are 2^(s - mo), mo finite and followed only when a row outgrows it by 2^8 (and at its first key): the scores leave the products through one fma,
 // and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
-// Bound by the vector units' work on the scores (bias, maximum, 2^x, sum, two halves: some 10 operations each) next to the matrix products, of which only part runs
-// at the same time on 2 or 3 waves a SIMD.  38 x 8 heads of 1024 x 1024 of 32, fp32: 206 us with the split, 198 TFLOP/s of the formula's, 0.47 of
-// what three half-precision products at a large matrix product's rate would take; 2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 459 us, 599 TFLOP/s
-// (358 with the weights in one bf16 part, the outputs' error then 1.3 times that of their own rounding).  Three waves a SIMD (bf16 up to 64 columns) against two, 8 x 16 heads of 1024 x 1024: 54.0 / 52.4 us for 32 columns, 75.7 / 76.4
-// for 64, where the long sequence takes 467 / 493.
+// Bound by the vector units' work on the scores (bias, maximum, 2^x, sum, two parts: some 10 operations each) next to the matrix products, of which only part runs
+// at the same time on 2 or 3 waves a SIMD.  2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 460 us, 597 TFLOP/s; of the SIMDs' cycles the vector units are
+// busy for 0.71, the matrix units for 0.40 (358 us with the weights in one bf16 part, the outputs' error then 1.3 times that of their own rounding).
+// 38 x 8 heads of 1024 x 1024 of 32, fp32: 206 us with the split, 198 TFLOP/s of the formula's, 0.47 of what three half-precision products at a large matrix
+// product's rate would take: vector 0.54, matrix 0.28, a quarter of the waves' time spent waiting, and 2432 blocks on 768 places are 3.2 rounds.
+// Three waves a SIMD (bf16 up to 64 columns) against two, 8 x 16 heads of 1024 x 1024: 54.0 / 52.4 us for 32 columns, 75.7 / 76.4 for 64, where the long
+// sequence takes 467 / 493.
 // 64 queries a wave instead of 32: 221 us for 205 of that build.
 template <int DHP, int NL>
 __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile_kernel(RP p, Src a) {
@@ -633,7 +635,8 @@ Plan plan(const smx_relpos_desc* d, const RP& p) {
   w.split_ws = 0;
   w.rt = rows >= 3 ? 4 : (int)rows;                                   // (8 at a time: 8 rows 110 us instead of 63)
   const long long base = w.token ? (long long)p.B * p.Hkv * ((rows + w.rt - 1) / w.rt) : (long long)p.B * p.H * ((p.L + 127) / 128);
-  // parts of the keys from 513 keys on, none shorter than 256, until the chip's 256 CUs have two blocks each (few queries, bound by the loads in flight: four).  In
+  // parts of the keys from 513 keys on, none shorter than 256, until the chip's 256 CUs have two blocks each (the 32-column and the small bf16 kernels would hold three;
+  // few queries, bound by the loads in flight: four).  Parts are cut from S, so that those behind a shorter sample's end have nothing to do.  In
   // parts / not, 8 heads of 64: 1024 queries on 4096 keys fp32 52 / 130 us, 128 on 8192 bf16 22 / 154, 1 on 4096 fp32 15 / 64
   long long np = ((w.token ? 1024 : 512) + base - 1) / base, most = p.S <= 512 ? 1 : (p.S + 255) / 256;
   if (np > most) np = most;

@@ -84,9 +84,11 @@ __device__ __forceinline__ f32x16 rows_times(const char* t, int plane, int r0, c
 // dQ^T += K^T dS^T with dS^T from the registers.  dS by distance: in a tile that lies beyond the map's ends all pairs are of one entry, a
 // lane adds its own; elsewhere lane t collects the tile's diagonal key - query = t - 31 through lane permutes, register by register, and adds it to the
 // wave's table in LDS -- one lane an entry, tile after tile: a fixed order without atomics.
-// Bound as the forward's tiles are, by the vector work on P and dS next to the products, with two waves a SIMD: 256 registers hold 32 queries' operands (Q, dO, dq)
-// and a tile's S and dS.  2 x 16 heads (4 kv) of 4096 x 4096 of 64, causal: 381 us, 270 TFLOP/s (0.65 of three half-precision products' rate); 4 x 8
-// heads of 1024 x 1024 of 32: 47 us, 137 TFLOP/s, where 768 blocks are 1.5 rounds.  One wave a SIMD without spills at 64 columns: 2% slower; three at 32: 20%;
+// Two waves a SIMD: 256 registers hold 32 queries' operands (Q, dO, dq) and a tile's S and dS (64 columns: 11 more go through scratch).  With so few, neither the
+// matrix units (busy for 0.38 of the cycles) nor the vector units (0.34) are full: a wave waits for 0.35 of its time, for its tile's loads, LDS and
+// barriers, and the causal blocks' lengths leave 1.6 waves a SIMD.  2 x 16 heads (4 kv) of 4096 x 4096 of 64, causal: 367 us, 281 TFLOP/s (0.67 of three
+// half-precision products' rate); 4 x 8 heads of 1024 x 1024 of 32: 47 us, 137 TFLOP/s: 512 blocks of 8 tiles are one round of two a CU, 1.4
+// waves a SIMD on average, which wait for 0.39 of their time.  One wave a SIMD without spills at 64 columns: 2% slower; three at 32: 20%;
 // two waves a block: 30%; 64 queries a wave: 8% at 64 columns, 33% at 32.
 template <int DHP>
 __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP p, Bwd a) {
@@ -243,7 +245,10 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_q_kernel(RP
 }
 
 // dk and dv.  A wave: 32 keys as columns; Q and dO of the heads that share them staged 64 or 32 queries at a time; S = Q K^T, dP = dO V^T, dV^T += dO^T P,
-// dK^T += Q^T dS.  P carries 2^14, so that what is left of a weight is off by at most 2^-39.  The sizes above: 540 us, 254 TFLOP/s; 42 us, 206 TFLOP/s.  Few key blocks: a part of their queries (tiles of all the heads) a block, joined by relpos_bwd_rest_kernel.
+// dK^T += Q^T dS.  P carries 2^14, so that what is left of a weight is off by at most 2^-39.  The sizes above: 535 us, 257 TFLOP/s; 42 us, 206 TFLOP/s.  64 columns keep
+// 33 registers in scratch (384 MB read, 129 written at the first size, 67 of them the parts' dk and dv) and wait for 0.57 of their time; matrix units 0.34, vector units 0.26.  65 columns and more
+// run one wave a SIMD: 2 x 8 heads of 2048 x 2048 with the forward, 80 columns 470 us, 128 647.  Few key blocks: a part of their queries (tiles of all the
+// heads) a block, joined by relpos_bwd_rest_kernel.
 template <int DHP>
 __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(RP p, Bwd a) {
   using ST = Stage<DHP>;
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(256, DHP >= 96 ? 1 : 2) void relpos_bwd_kv_kernel(R
 }
 
 // What is left once the two passes are done, one launch: the first H blocks dtable, if it is wanted, the others gradients from their parts, in order (dq, dk, dv).
-// dtable[bucket][h] += the distances of that bucket: the query blocks' sums in four fixed runs, then a wave a bucket.  Bound by its dependent loads: 13 us after 4 x 8
+// dtable[bucket][h] += the distances of that bucket: the query blocks' sums in four fixed runs, then a wave a bucket.  Bound by its dependent loads on H blocks: 14 us after 4 x 8
 // heads of 1024 x 1024.
 struct Sum { const float* src; float* dst; long long size, step; int nparts, end; };      // end: running sum of blocks
 struct Rest { Sum s[3]; const float* part; int rows, tables; };                          // rows: query blocks (and their parts) of a head and sample; tables: H or 0
