@@ -382,13 +382,13 @@ __global__ __launch_bounds__(256, NL == 1 && DHP <= 64 ? 3 : 2) void relpos_tile
     if (hh == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.nparts + part) * 2) = make_float2(begun ? mo : -INFINITY, l);
     return;
   }
-  const float il = l == 0.f ? 0.f : inv_v / l;                    // (0: no key left; a sum that is no number stays none)
+  const float il = l == 0.f ? 0.f : 1.f / l;                      // (0: no key left; a sum that is no number stays none.  inv_v / l could leave the normal numbers)
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = d * 32 + 8 * g + 4 * hh;
-      const float4 w = make_float4(o[d][4 * g] * il, o[d][4 * g + 1] * il, o[d][4 * g + 2] * il, o[d][4 * g + 3] * il);
+      const float4 w = make_float4(o[d][4 * g] * il * inv_v, o[d][4 * g + 1] * il * inv_v, o[d][4 * g + 2] * il * inv_v, o[d][4 * g + 3] * il * inv_v);
       if (c < p.dh) {
         if constexpr (NL == 2) St<float>::st4((float*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);
         else St<bf16_t>::st4((bf16_t*)p.o + b * p.o_bs + (long long)qi * p.ldo + h * p.dh + c, w);

@@ -170,3 +170,21 @@ def test_gradients_that_are_wanted_do_not_depend_on_the_others(ops, T, stopped, 
     tp.backward()
     for n, got, ref in zip("qkvt", (tp.grad(q), tp.grad(k), tp.grad(v), G.get("t")), want[1:]):
         assert got is None if n in stopped else torch.equal(got, ref), n
+
+
+@pytest.mark.parametrize("Lq", [1, 100])
+@pytest.mark.parametrize("S", [500, 2000])
+@pytest.mark.parametrize("e", [-115, -90, 90])
+def test_far_values_keep_their_bits(ops, T, Lq, S, e):
+    """values (and, in the other direction, output gradients) of size 2^e: results of their size are as accurate as those of size one"""
+    q, k, v, g = mk(37, 2, 2, 1, Lq, S, 32)
+    rp = ops.relpos()
+    table, go = torch.randn(32, 2, generator=g).cuda(), torch.randn(2, Lq, 64, generator=g).cuda()
+    f = 2.0 ** e
+    near(ops.attention_relpos(q, k, v * f, table, rp, 2, nkv=1), *R.attention(q, k, v * f, table, rp, 2, nkv=1)["o"], "o")
+    if abs(e) < 100:                                             # (dS of size 2^-91 and more)
+        out = step(T, q, k, v, table, rp, 2, go * f, nkv=1)
+        ref = R.attention(q, k, v, table, rp, 2, nkv=1, g=go * f)
+        for t, n in zip(out[1:], ("dq", "dk", "dv", "dtable")):
+            val, bound = ref[n]
+            near(t, val, bound + 2.0 ** -125 * S, n)
