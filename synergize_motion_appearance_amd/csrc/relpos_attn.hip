@@ -142,7 +142,7 @@ struct Src {
 // and P stays below 2^8 (fp32 storage: 2^14, below the largest half; its second half is then off by at most 2^-31 of the row's largest weight).
 // The bias of a tile that lies beyond the map's ends is one number; other tiles read it per score from LDS.
 // Bound by the vector units' work on the scores (bias, maximum, 2^x, sum, two parts: some 10 operations each) next to the matrix products, of which only part runs
-// at the same time on 2 or 3 waves a SIMD.  2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 460 us, 597 TFLOP/s; of the SIMDs' cycles the vector units are
+// at the same time on 2 or 3 waves a SIMD.  2 x 16 heads (4 kv) of 8192 x 8192 of 64, causal, bf16: 465 us, 591 TFLOP/s; of the SIMDs' cycles the vector units are
 // busy for 0.71, the matrix units for 0.40 (358 us with the weights in one bf16 part, the outputs' error then 1.3 times that of their own rounding).
 // 38 x 8 heads of 1024 x 1024 of 32, fp32: 206 us with the split, 198 TFLOP/s of the formula's, 0.47 of what three half-precision products at a large matrix
 // product's rate would take: vector 0.54, matrix 0.28, a quarter of the waves' time spent waiting, and 2432 blocks on 768 places are 3.2 rounds.

@@ -7,7 +7,6 @@ import weakref
 import pytest
 import torch
 
-from synergize_motion_appearance_amd import lib as L
 from synergize_motion_appearance_amd import ops, train_ops
 from synergize_motion_appearance_amd.tape import Tape
 
